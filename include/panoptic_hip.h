@@ -41,6 +41,10 @@ enum {
   PP_UNSUPPORTED = 5    /* not an error: this optional fused form does not serve the shape, nothing was launched */
 };
 
+/* Element types and activations of the row operators (pp_group_norm_*, pp_linear_act_*, pp_newton_schulz). */
+enum { PP_F32 = 0, PP_BF16 = 1, PP_F16 = 2 };
+enum { PP_ACT_NONE = 0, PP_ACT_RELU = 1, PP_ACT_LEAKY = 2, PP_ACT_SILU = 3, PP_ACT_GELU = 4 /* exact, by erf */ };
+
 /* Library identity / diagnostics.  pp_version: "panoptic_hip <n> gfx950". */
 const char* pp_version(void);
 const char* pp_last_error(void);
@@ -381,6 +385,25 @@ int pp_bn_train_fwd(const float* x, int64_t n, int32_t c, const float* weight, c
 int pp_bn_train_bwd(const float* x, const float* dy, const float* y_relu, int64_t n, int32_t c,
                     const float* weight, const double* save_mean, const double* save_rstd, float* dx,
                     float* dweight, float* dbias, void* ws, size_t ws_bytes, pp_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Group normalisation over the rows of each batch element, with an activation   (beside pp_bn_train_*: statistics that do not
+ * depend on the rest of the batch.  groups == c is instance normalisation.)
+ * x, y, dy, dx [n,c] of element type `dtype` (PP_F32 | PP_BF16 | PP_F16), c <= 1024, groups divides c.  Batch element s owns the
+ * positions offsets[s] .. offsets[s+1] - 1 (device int64 [b+1], ascending); position p is row order[p] (device int64 [n], each row
+ * once; NULL: row p).  Rows of no batch element get zeros.  weight, bias float32 [c], nullable.  mean, rstd float32 [b,groups] are
+ * kept for the backward (0 for a batch element without rows).
+ * fwd: y = act((x - mean) * rstd * weight + bias), biased variance.   bwd: dx, dweight, dbias (nullable) of the same.
+ * Sums are float64, no atomics: results repeat bit for bit.
+ * ---------------------------------------------------------------------------------------------- */
+size_t pp_group_norm_workspace(int64_t n, int64_t b, int32_t c, int32_t groups, int32_t backward);
+int pp_group_norm_fwd(const void* x, int32_t dtype, int64_t n, int32_t c, int32_t groups, const int64_t* offsets, int64_t b,
+                      const int64_t* order, const float* weight, const float* bias, double eps, int32_t act, float slope, void* y,
+                      float* mean, float* rstd, void* ws, size_t ws_bytes, pp_stream_t stream);
+int pp_group_norm_bwd(const void* x, const void* dy, int32_t dtype, int64_t n, int32_t c, int32_t groups, const int64_t* offsets,
+                      int64_t b, const int64_t* order, const float* weight, const float* bias, const float* mean, const float* rstd,
+                      int32_t act, float slope, void* dx, float* dweight, float* dbias, void* ws, size_t ws_bytes,
+                      pp_stream_t stream);
 
 /* Weight / bias gradient of a skinny Linear layer y = x W^T + b (cin, cout <= 32, millions of rows): dw [cout,cin] =
  * dy^T x, db [cout] = column sums of dy (db nullable).  replaces: the torch.nn.Linear backward (rocBLAS split-K GEMM with

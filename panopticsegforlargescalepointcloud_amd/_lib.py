@@ -99,6 +99,9 @@ SIGNATURES = {
     "pp_bn_train_workspace": (sz, [i64, i32]),
     "pp_bn_train_fwd": (C.c_int, [vp, i64, i32, vp, vp, f64, f64, vp, vp, i32, vp, vp, vp, vp, vp, sz, vp]),
     "pp_bn_train_bwd": (C.c_int, [vp, vp, vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "pp_group_norm_workspace": (sz, [i64, i64, i32, i32, i32]),
+    "pp_group_norm_fwd": (C.c_int, [vp, i32, i64, i32, i32, vp, i64, vp, vp, vp, f64, i32, f32, vp, vp, vp, vp, sz, vp]),
+    "pp_group_norm_bwd": (C.c_int, [vp, vp, i32, i64, i32, i32, vp, i64, vp, vp, vp, vp, vp, i32, f32, vp, vp, vp, vp, sz, vp]),
     "pp_head_mlp": (C.c_int, [vp, i64, i32, vp, i32, vp, vp, vp, vp, i32, i32, vp, vp, vp]),
     "pp_linear_rows": (C.c_int, [vp, vp, vp, i64, i32, i32, i32, vp, vp]),
     "pp_linear_wgrad_workspace": (C.c_size_t, [i64, i32, i32]),

@@ -51,6 +51,38 @@ class FastBatchNorm1d(nn.Module):
         raise ValueError("Non supported number of dimensions {}".format(x.dim()))
 
 
+class _GroupNormActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, offsets, num_groups, weight, bias, eps, act, slope, order):
+        x = x.contiguous()
+        y, mean, rstd = ops.group_norm_fwd(x, offsets, num_groups, weight, bias, eps, act, slope, order)
+        ctx.save_for_backward(x, offsets, weight, bias, mean, rstd, order)
+        ctx.cfg = (num_groups, act, slope)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, offsets, weight, bias, mean, rstd, order = ctx.saved_tensors
+        num_groups, act, slope = ctx.cfg
+        dx, dw, db = ops.group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act, slope, order)
+        return dx, None, None, dw if weight is not None else None, db if bias is not None else None, None, None, None, None
+
+
+def group_norm_act(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, activation="none", slope=0.2, order=None):
+    """y = act(group_norm(x)): statistics over the rows of each batch element and the channels of each group, differentiable in x,
+    weight and bias.  x [n, c] (float32, bfloat16 or float16), weight / bias float32 [c] or None.  Batch element s owns the
+    positions offsets[s] .. offsets[s+1] of the row sequence (int64 [batch + 1] on the device, ascending); position p is row
+    order[p] (int64 [n], each row once) or, without an order, row p.  Rows of no batch element (padding) come out as zeros and
+    get zero gradients.  activation: none, relu, leaky_relu (with `slope`), silu or gelu (exact).  num_groups = c: instance norm.
+    Beside FastBatchNorm1d: the result for a row does not depend on the other batch elements, in training and in inference."""
+    act = ops.activation_id(activation)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _GroupNormActFn.apply(x, offsets, num_groups, weight, bias, eps, act, slope, order)
+    return ops.group_norm_fwd(x, offsets, num_groups, weight, bias, eps, act, slope, order)[0]
+
+
 # forward / input gradient of the skinny Linear layers from the library (PP_LINEAR_ROWS=0: torch GEMMs, A/B runs)
 LINEAR_ROWS = os.environ.get("PP_LINEAR_ROWS", "1") != "0"
 

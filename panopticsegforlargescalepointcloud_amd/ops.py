@@ -4,6 +4,7 @@ PyTorch is plumbing here (allocation, streams); every op below is one or a few l
 gfx950 kernels in csrc/.  All tensors must live on a HIP device; there is no CPU path.
 """
 import ctypes as C
+import functools
 import os
 import threading
 import weakref
@@ -1221,6 +1222,111 @@ def affine_act(x, scale=None, shift=None, act=0, slope=0.0, residual=None):
                                  _ptr(_need(shift, torch.float32, "shift")), int(act), float(slope),
                                  _ptr(_need(residual, torch.float32, "residual")), _ptr(y), _stream()), "pp_affine_act")
     return y
+
+
+# ------------------------------------------------------------------------------------------ row operators
+_ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "leaky_relu": 2, "silu": 3, "gelu": 4}  # gelu: exact (by erf)
+
+
+def activation_id(activation):
+    if activation is None:
+        return 0
+    if activation not in ACTIVATIONS:
+        raise ValueError("activation must be one of %s, got %r" % (", ".join(sorted(ACTIVATIONS)), activation))
+    return ACTIVATIONS[activation]
+
+
+def _on_device_of(fn):
+    """run `fn` with the device of its first tensor current, so that its buffers and its launches go to that device's current
+    stream whichever device the calling thread has selected"""
+    @functools.wraps(fn)
+    def call(x, *args, **kwargs):
+        if not torch.is_tensor(x) or not x.is_cuda:
+            raise _lib.PanopticHipError("%s: the input must be a HIP device tensor (there is no CPU fallback)" % fn.__name__)
+        if x.device.index == torch._C._cuda_getDevice():
+            return fn(x, *args, **kwargs)
+        with torch.cuda.device(x.device):
+            return fn(x, *args, **kwargs)
+    return call
+
+
+def _row_dtype(x, name):
+    code = _ROW_DTYPES.get(x.dtype)
+    if code is None:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, x.dtype))
+    return code
+
+
+def _beside(t, x, dtype, shape, name):
+    """operand `t` (nullable) of a launch on x: same device, the given element type and shape; contiguous"""
+    if t is None:
+        return None
+    if t.device != x.device:
+        raise _lib.PanopticHipError("%s is on %s, the input on %s" % (name, t.device, x.device))
+    if t.dtype != dtype:
+        raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _group_norm_operands(x, offsets, num_groups, weight, bias, order):
+    if x.dim() != 2:
+        raise ValueError("group_norm: x must be [rows, channels], got %s" % (tuple(x.shape),))
+    n, c = x.shape
+    if not 1 <= c <= 1024:
+        raise ValueError("group_norm: 1 to 1024 channels, got %d" % c)
+    if num_groups < 1 or c % num_groups:
+        raise ValueError("group_norm: %d groups do not divide %d channels" % (num_groups, c))
+    if offsets.dim() != 1 or offsets.shape[0] < 1:
+        raise ValueError("group_norm: offsets must be [batch + 1], got %s" % (tuple(offsets.shape),))
+    return (_beside(offsets, x, torch.int64, offsets.shape, "offsets"), _beside(weight, x, torch.float32, (c,), "weight"),
+            _beside(bias, x, torch.float32, (c,), "bias"), _beside(order, x, torch.int64, (n,), "order"))
+
+
+@_on_device_of
+def group_norm_fwd(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, act=0, slope=0.0, order=None):
+    """Group normalisation with an activation over the rows of each batch element (csrc/pp_groupnorm.hip): x [n, c] float32,
+    bfloat16 or float16; batch element s owns positions offsets[s] .. offsets[s+1] (int64 [batch + 1]), position p is row order[p]
+    (int64 [n]) or row p; rows of no batch element come out as zeros.  weight / bias float32 [c] or None.
+    Returns (y, mean, rstd), the statistics float32 [batch, num_groups]."""
+    lib = _lib.load()
+    code = _row_dtype(x, "x")
+    offsets, weight, bias, order = _group_norm_operands(x, offsets, num_groups, weight, bias, order)
+    x = x if x.is_contiguous() else x.contiguous()
+    n, c = x.shape
+    b = offsets.shape[0] - 1
+    y = torch.empty_like(x)
+    stat = torch.empty((2, b, num_groups), dtype=torch.float32, device=x.device)
+    wsb = lib.pp_group_norm_workspace(n, b, c, num_groups, 0)
+    ws = _ws(wsb, x.device)
+    _lib.check(lib.pp_group_norm_fwd(_ptr(x), code, n, c, num_groups, _ptr(offsets), b, _ptr(order), _ptr(weight), _ptr(bias), float(eps),
+                                     int(act), float(slope), _ptr(y), _ptr(stat[0]), _ptr(stat[1]), _ptr(ws), ws.numel(), _stream()),
+               "pp_group_norm_fwd")
+    return y, stat[0], stat[1]
+
+
+@_on_device_of
+def group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act=0, slope=0.0, order=None):
+    """Backward of group_norm_fwd with the statistics it returned: (dx, dweight, dbias), the last two float32 [c]."""
+    lib = _lib.load()
+    code = _row_dtype(x, "x")
+    offsets, weight, bias, order = _group_norm_operands(x, offsets, num_groups, weight, bias, order)
+    x = x if x.is_contiguous() else x.contiguous()
+    n, c = x.shape
+    b = offsets.shape[0] - 1
+    dy = _beside(dy, x, x.dtype, (n, c), "dy")
+    mean = _beside(mean, x, torch.float32, (b, num_groups), "mean")
+    rstd = _beside(rstd, x, torch.float32, (b, num_groups), "rstd")
+    dx = torch.empty_like(x)
+    dwb = torch.empty((2, c), dtype=torch.float32, device=x.device)
+    wsb = lib.pp_group_norm_workspace(n, b, c, num_groups, 1)
+    ws = _ws(wsb, x.device)
+    _lib.check(lib.pp_group_norm_bwd(_ptr(x), _ptr(dy), code, n, c, num_groups, _ptr(offsets), b, _ptr(order), _ptr(weight), _ptr(bias),
+                                     _ptr(mean), _ptr(rstd), int(act), float(slope), _ptr(dx), _ptr(dwb[0]), _ptr(dwb[1]), _ptr(ws),
+                                     ws.numel(), _stream()), "pp_group_norm_bwd")
+    return dx, dwb[0], dwb[1]
 
 
 def linear_rows(x, weight, bias=None, transposed=False):

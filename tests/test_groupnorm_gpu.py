@@ -1,0 +1,318 @@
+"""Group normalisation with an activation (ops.group_norm_fwd / _bwd, modules.group_norm_act) against the definition in 64 bits.
+
+Error bounds.  u = 2^-24; U = half a step of the stored type.  The statistics are fp64 sums rounded to fp32, so the kernel's mean is
+off by u |mean| and 1/std by u relative; x - mean, the product with 1/std and the affine map round once each:
+  |d xh| <= 4 u (rstd (|x| + |mean|) + |xh|),   |d z| <= |w| |d xh| + 2 u (|w xh| + |b|)
+The activations have |act'| <= 1.13 and |act''| <= 0.8; expf and erff are good to 4 u and enter once, with a few roundings around
+them: 16 u |z| for act, 16 u for act'.  At the kink of relu / leaky an element whose |z| is below |d z| may take either slope.
+Backward: h = dy act'(z) w, dx = rstd (h - A - xh B), A = mean(h), B = mean(h xh) in fp64."""
+import math
+
+import pytest
+import torch
+
+from panopticsegforlargescalepointcloud_amd import _lib, modules, ops
+
+pytestmark = pytest.mark.gpu
+
+u = 2.0 ** -24
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
+SLOPE = 0.2
+
+
+def act64(z, kind):
+    if kind == "relu":
+        return z.clamp(min=0)
+    if kind == "leaky_relu":
+        return torch.where(z > 0, z, SLOPE * z)
+    if kind == "silu":
+        return z * torch.sigmoid(z)
+    if kind == "gelu":
+        return 0.5 * z * torch.erfc(-z / math.sqrt(2.0))
+    return z
+
+
+def dact64(z, kind):
+    if kind == "relu":
+        return (z > 0).double()
+    if kind == "leaky_relu":
+        return torch.where(z > 0, 1.0, SLOPE).double()
+    if kind == "silu":
+        s = torch.sigmoid(z)
+        return s * (1 + z * (1 - s))
+    if kind == "gelu":
+        return 0.5 * torch.erfc(-z / math.sqrt(2.0)) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    return torch.ones_like(z)
+
+
+def kinked(kind):
+    return kind in ("relu", "leaky_relu")
+
+
+def reference(x, offsets, groups, w, b, eps, kind, order=None, dy=None):
+    """(y, bound of y) and, with dy, (dx, bound), (dw, bound), (db, bound); everything on the CPU in 64 bits"""
+    X = x.detach().double().cpu()
+    n, c = X.shape
+    W = torch.ones(c, dtype=torch.float64) if w is None else w.detach().double().cpu()
+    B = torch.zeros(c, dtype=torch.float64) if b is None else b.detach().double().cpu()
+    D = None if dy is None else dy.double().cpu()
+    y, ey = torch.zeros_like(X), torch.zeros_like(X)
+    dx, edx = torch.zeros_like(X), torch.zeros_like(X)
+    dw, edw, db, edb = (torch.zeros(c, dtype=torch.float64) for _ in range(4))
+    off = offsets.cpu().tolist()
+    for lo, hi in zip(off[:-1], off[1:]):
+        if hi <= lo:
+            continue
+        rows = torch.arange(lo, hi) if order is None else order.cpu()[lo:hi]
+        v = X[rows].view(hi - lo, groups, -1)
+        mean = v.mean((0, 2), keepdim=True)
+        rstd = 1 / torch.sqrt(((v - mean) ** 2).mean((0, 2), keepdim=True) + eps)
+        flat = lambda t: t.expand_as(v).reshape(hi - lo, c)  # noqa: E731
+        xh = ((v - mean) * rstd).reshape(hi - lo, c)
+        exh = 4 * u * (flat(rstd) * (X[rows].abs() + flat(mean).abs()) + xh.abs())
+        z = xh * W + B
+        ez = W.abs() * exh + 2 * u * ((W * xh).abs() + B.abs())
+        y[rows] = act64(z, kind)
+        ey[rows] = 1.13 * ez + 16 * u * z.abs()
+        if D is None:
+            continue
+        d = D[rows]
+        dz = d * dact64(z, kind)
+        edz = d.abs() * (0.8 * ez + 16 * u)
+        if kinked(kind):
+            edz = edz + d.abs() * (z.abs() <= ez)
+        h, eh = dz * W, edz * W.abs() + 2 * u * (dz * W).abs()
+        g = lambda t: flat(t.view(hi - lo, groups, -1).mean((0, 2), keepdim=True))  # noqa: E731
+        A, Bm = g(h), g(h * xh)
+        eA, eB = g(eh) + 2 * u * A.abs(), g(eh * xh.abs() + h.abs() * exh) + 2 * u * Bm.abs()
+        r = flat(rstd)
+        dx[rows] = r * (h - A - xh * Bm)
+        edx[rows] = r * (eh + eA + exh * Bm.abs() + xh.abs() * eB + 6 * u * (h.abs() + A.abs() + (xh * Bm).abs()))
+        dw += (dz * xh).sum(0)
+        edw += (edz * xh.abs() + dz.abs() * exh).sum(0)
+        db += dz.sum(0)
+        edb += edz.sum(0)
+    if D is None:
+        return (y, ey)
+    return (y, ey), (dx, edx), (dw, edw), (db, edb)
+
+
+def near(got, want, bound, dtype, what):
+    got = got.detach().double().cpu()
+    room = bound * (1 + 1e-6) + HALF_STEP[dtype] * want.abs() * (1 + 2 * u) + HALF_STEP[dtype] * bound + TINY[dtype]
+    over = (got - want).abs() - room
+    assert bool((over <= 0).all()), "%s: off by %.3g at most, %d of %d values outside" % (
+        what, float((got - want).abs().max()), int((over > 0).sum()), over.numel())
+
+
+def case(n, lengths, c, dtype, seed=0, affine=True, shuffle=False, shift=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn((n, c), generator=gen) * (0.5 + torch.rand(c, generator=gen)) + shift * torch.randn(c, generator=gen)
+    dy = torch.randn((n, c), generator=gen)
+    w = (1 + 0.3 * torch.randn(c, generator=gen)) if affine else None
+    b = 0.3 * torch.randn(c, generator=gen) if affine else None
+    offsets = torch.tensor([0] + list(torch.tensor(lengths).cumsum(0).tolist()) if lengths else [0], dtype=torch.int64)
+    order = torch.randperm(n, generator=gen) if shuffle else None
+    up = lambda t: None if t is None else t.cuda()  # noqa: E731
+    return up(x.to(dtype)), up(dy.to(dtype)), up(w), up(b), up(offsets), up(order)
+
+
+def check(n, lengths, c, groups, dtype, kind, seed=0, affine=True, shuffle=False, eps=1e-5, shift=1.0):
+    x, dy, w, b, offsets, order = case(n, lengths, c, dtype, seed, affine, shuffle, shift)
+    act = ops.activation_id(kind)
+    y, mean, rstd = ops.group_norm_fwd(x, offsets, groups, w, b, eps, act, SLOPE, order)
+    dx, dw, db = ops.group_norm_bwd(x, dy, offsets, groups, w, b, mean, rstd, act, SLOPE, order)
+    ry, rdx, rdw, rdb = reference(x, offsets, groups, w, b, eps, kind, order, dy)
+    near(y, *ry, dtype, "y")
+    near(dx, *rdx, dtype, "dx")
+    near(dw, *rdw, torch.float32, "dweight")
+    near(db, *rdb, torch.float32, "dbias")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["none", "relu", "leaky_relu", "silu", "gelu"])
+def test_types_and_activations(dtype, kind):
+    check(1500, [700, 0, 1, 299, 500], 32, 4, dtype, kind, seed=3)
+
+
+@pytest.mark.parametrize("n,lengths,c,groups", [
+    (1, [1], 1, 1),                       # one value: its own mean
+    (1, [1], 16, 16),                     # one row, instance norm: every value is its own mean
+    (5, [1, 1, 1, 1, 1], 24, 3),          # one row per batch element
+    (0, [0, 0], 16, 2),                   # no rows at all
+    (3, [], 8, 2),                        # no batch element: every row is padding
+    (700, [300, 200], 20, 5),             # 200 rows behind the last batch element
+    (513, [100, 0, 0, 413], 7, 7),        # rows that are no multiple of 16 bytes; instance norm
+    (300, [150, 150], 7, 1),
+    (260, [259, 1], 1024, 32),
+    (150, [60, 90], 301, 43),             # wider than a workgroup, single elements
+    (90, [90], 1023, 1),
+    (400, [400], 96, 1),
+    (400, [133, 267], 256, 256),
+    (64, [64], 112, 8),
+    (65, [64, 1], 112, 8),
+])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_shapes(n, lengths, c, groups, dtype):
+    check(n, lengths, c, groups, dtype, "silu", seed=n + c)
+
+
+@pytest.mark.parametrize("n,b", [(70_001, 3), (140_000, 1), (30_000, 2500), (66_000, 37)])
+def test_long_and_many(n, b):
+    """elements longer than a chunk, chunks that hold many elements, some of them empty"""
+    gen = torch.Generator().manual_seed(n)
+    cut = torch.sort(torch.randint(0, n + 1, (b - 1,), generator=gen)).values.tolist()
+    ends = cut + [n]
+    lengths = [e - s for s, e in zip([0] + cut, ends)]
+    check(n, lengths, 16, 4, torch.float32, "gelu", seed=b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_row_order(dtype):
+    check(3001, [1000, 0, 2, 1999], 48, 6, dtype, "relu", seed=9, shuffle=True)
+
+
+def test_without_affine_and_far_from_zero():
+    check(2000, [900, 1100], 32, 8, torch.float32, "none", seed=1, affine=False)
+    check(2000, [900, 1100], 32, 8, torch.float32, "none", seed=2, shift=1000.0)  # mean / std ~ 1000: fp32 sums of squares would lose it
+    x, _, w, b, offsets, _ = case(64, [64], 32, torch.float32)
+    y, mean, rstd = ops.group_norm_fwd(x, offsets, 4, w, None)
+    near(y, *reference(x, offsets, 4, w, None, 1e-5, "none"), torch.float32, "y without bias")
+
+
+def test_one_outlier_among_many():
+    x, _, w, b, offsets, _ = case(100_000, [100_000], 16, torch.float32, shift=0.0)
+    x[0] = 1000.0
+    y, _, _ = ops.group_norm_fwd(x, offsets, 4, w, b)
+    near(y, *reference(x, offsets, 4, w, b, 1e-5, "none"), torch.float32, "y")
+
+
+def test_non_finite_values_stay_in_their_element_and_group():
+    x, dy, w, b, offsets, _ = case(900, [300, 300, 300], 32, torch.float32)
+    clean, m0, r0 = ops.group_norm_fwd(x, offsets, 4, w, b, 1e-5, 3)
+    cdx, _, _ = ops.group_norm_bwd(x, dy, offsets, 4, w, b, m0, r0, 3)
+    x[310, 9], x[450, 25] = float("nan"), float("inf")
+    y, mean, rstd = ops.group_norm_fwd(x, offsets, 4, w, b, 1e-5, 3)
+    dx, _, _ = ops.group_norm_bwd(x, dy, offsets, 4, w, b, mean, rstd, 3)
+    hit = torch.zeros_like(x, dtype=torch.bool)
+    hit[300:600, 8:16] = hit[300:600, 24:32] = True
+    assert torch.isnan(y[hit]).all() and torch.isnan(dx[hit]).all()
+    assert torch.equal(y[~hit], clean[~hit]) and torch.equal(dx[~hit], cdx[~hit])
+
+
+def test_results_repeat_and_do_not_depend_on_the_batch():
+    x, dy, w, b, offsets, _ = case(60_000, [25_000, 35_000], 64, torch.bfloat16)
+    one = ops.group_norm_fwd(x, offsets, 8, w, b, 1e-5, 3)
+    two = ops.group_norm_fwd(x, offsets, 8, w, b, 1e-5, 3)
+    assert all(torch.equal(p, q) for p, q in zip(one, two))
+    back = [ops.group_norm_bwd(x, dy, offsets, 8, w, b, one[1], one[2], 3) for _ in range(2)]
+    assert all(torch.equal(p, q) for p, q in zip(*back))
+
+
+def test_unaligned_and_strided_inputs():
+    base = torch.randn(1 + 400 * 32, device="cuda")
+    x = base[1:].view(400, 32)  # contiguous, 4 bytes behind a 16-byte boundary
+    off = torch.tensor([0, 150, 400], device="cuda")
+    w, b = torch.randn(32, device="cuda"), torch.randn(32, device="cuda")
+    y, mean, rstd = ops.group_norm_fwd(x, off, 4, w, b)
+    near(y, *reference(x, off, 4, w, b, 1e-5, "none"), torch.float32, "unaligned")
+    wide = torch.randn((400, 64), device="cuda")
+    y = ops.group_norm_fwd(wide[:, 16:48], off, 4, w, b)[0]
+    near(y, *reference(wide[:, 16:48], off, 4, w, b, 1e-5, "none"), torch.float32, "strided")
+    x = wide[:, 16:48].contiguous().requires_grad_()
+    out = modules.group_norm_act(x, off, 4, w, b, activation="gelu")
+    out.sum().backward()  # a gradient of stride 0
+    want = reference(x, off, 4, w, b, 1e-5, "gelu", None, torch.ones_like(out))
+    near(x.grad, *want[1], torch.float32, "dx of a sum")
+
+
+def test_gradients_against_differences():
+    """<dx, v> against central differences of the definition in 64 bits along v, for the input and both parameters"""
+    x, dy, w, b, offsets, _ = case(300, [120, 0, 180], 24, torch.float32, seed=5)
+    xr, wr, br = (t.clone().requires_grad_() for t in (x, w, b))
+    y = modules.group_norm_act(xr, offsets, 6, wr, br, activation="silu")
+    y.backward(dy)
+    bounds = reference(x, offsets, 6, w, b, 1e-5, "silu", None, dy)[1:]
+    gen = torch.Generator().manual_seed(1)
+    for leaf, (_, bound), at in ((xr, bounds[0], 0), (wr, bounds[1], 1), (br, bounds[2], 2)):
+        v = torch.randn(leaf.shape, generator=gen, dtype=torch.float64)
+        h, vals = 1e-5, []
+        for sign in (1, -1):
+            moved = [t.double().cpu() for t in (x, w, b)]
+            moved[at] = moved[at] + sign * h * v
+            vals.append((reference(moved[0], offsets, 6, moved[1], moved[2], 1e-5, "silu")[0] * dy.double().cpu()).sum())
+        want = (vals[0] - vals[1]) / (2 * h)
+        got = (leaf.grad.double().cpu() * v).sum()
+        # the kernel's error along v, and the differences' own: h^2 of the third derivative, 1e-16 of the sum over 2 h
+        room = ((bound + u * leaf.grad.double().cpu().abs()) * v.abs()).sum() + 1e-6 * want.abs() + 1e-6
+        assert abs(got - want) <= room, (at, float(got), float(want), float(room))
+
+
+def test_side_stream_and_graph():
+    x, dy, w, b, offsets, order = case(20_000, [9000, 11_000], 32, torch.float32, shuffle=True)
+    want = ops.group_norm_fwd(x, offsets, 8, w, b, 1e-5, 3, 0.0, order)
+    wantb = ops.group_norm_bwd(x, dy, offsets, 8, w, b, want[1], want[2], 3, 0.0, order)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.group_norm_fwd(x, offsets, 8, w, b, 1e-5, 3, 0.0, order)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got[0], want[0])
+    sx, sdy = x.clone(), dy.clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        fy = ops.group_norm_fwd(sx, offsets, 8, w, b, 1e-5, 3, 0.0, order)
+        by = ops.group_norm_bwd(sx, sdy, offsets, 8, w, b, fy[1], fy[2], 3, 0.0, order)
+    for k in range(3):
+        sx.copy_(x * (k + 1) + k)
+        sdy.copy_(dy * (k + 1))
+        g.replay()
+        torch.cuda.synchronize()
+        e = ops.group_norm_fwd(sx, offsets, 8, w, b, 1e-5, 3, 0.0, order)
+        eb = ops.group_norm_bwd(sx, sdy, offsets, 8, w, b, e[1], e[2], 3, 0.0, order)
+        assert all(torch.equal(p, q) for p, q in zip(fy + by, e + eb)), k
+    assert torch.equal(wantb[0], ops.group_norm_bwd(x, dy, offsets, 8, w, b, want[1], want[2], 3, 0.0, order)[0])
+
+
+def test_bad_offsets_and_orders_touch_nothing_outside():
+    """offsets and orders are read on the device: what is out of range there is passed over, the buffers around stay as they are"""
+    n, c = 1000, 32
+    x = torch.randn((n, c), device="cuda")
+    for off in ([0, 4000, 900], [-5, 500, 1000], [0, 900, 100, 1000], [2000, 3000], [1 << 40, -(1 << 40), 7]):
+        y, mean, rstd = ops.group_norm_fwd(x, torch.tensor(off, device="cuda"), 4)
+        ops.group_norm_bwd(x, x, torch.tensor(off, device="cuda"), 4, None, None, mean, rstd)
+    good = torch.tensor([0, n], device="cuda")
+    order = torch.arange(n, device="cuda")
+    order[5], order[7] = -1, 1 << 50
+    y, mean, rstd = ops.group_norm_fwd(x, good, 4, order=order)
+    torch.cuda.synchronize()
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[5] = keep[7] = False
+    assert torch.isfinite(y[keep]).all()
+
+
+def test_refusals():
+    x = torch.randn((10, 12), device="cuda")
+    off = torch.tensor([0, 10], device="cuda")
+    with pytest.raises(ValueError):
+        ops.group_norm_fwd(x, off, 5)
+    with pytest.raises(ValueError):
+        ops.group_norm_fwd(x.view(-1), off, 1)
+    with pytest.raises(ValueError):
+        ops.group_norm_fwd(torch.zeros((2, 1028), device="cuda"), off, 1)
+    with pytest.raises(ValueError):
+        ops.group_norm_fwd(x, off, 4, weight=torch.ones(11, device="cuda"))
+    with pytest.raises(TypeError):
+        ops.group_norm_fwd(x, off, 4, weight=torch.ones(12, device="cuda", dtype=torch.float64))
+    with pytest.raises(TypeError):
+        ops.group_norm_fwd(x.double(), off, 4)
+    with pytest.raises(TypeError):
+        ops.group_norm_fwd(x, off.int(), 4)
+    with pytest.raises(ValueError):
+        ops.group_norm_fwd(x, off, 4, order=torch.arange(9, device="cuda"))
+    with pytest.raises(_lib.PanopticHipError):
+        ops.group_norm_fwd(x, off.cpu(), 4)
+    with pytest.raises(ValueError):
+        modules.group_norm_act(x, off, 4, activation="tanh")

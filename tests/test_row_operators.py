@@ -1,0 +1,49 @@
+"""CPU: argument checks of the row operators -- the C entries refuse bad arguments before anything is launched, the Python entries
+refuse tensors that do not live on a HIP device."""
+import ctypes as C
+
+import pytest
+import torch
+
+from panopticsegforlargescalepointcloud_amd import _lib, modules, ops
+
+INVALID, WORKSPACE = 1, 4
+P = C.c_void_p(4096)  # never read: every call below is refused before a launch
+
+
+def group_norm(**kw):
+    a = dict(x=P, dtype=0, n=10, c=8, groups=2, offsets=P, b=1, order=None, weight=None, bias=None, eps=1e-5, act=0, slope=0.0, y=P,
+             mean=P, rstd=P, ws=P, wsb=1 << 20, stream=None)
+    a.update(kw)
+    return _lib.load().pp_group_norm_fwd(*a.values())
+
+
+@pytest.mark.parametrize("kw", [{"dtype": 3}, {"dtype": -1}, {"act": 5}, {"act": -1}, {"c": 0}, {"c": 1025, "groups": 1}, {"groups": 3},
+                                {"groups": 0}, {"n": -1}, {"b": -1}, {"b": 1 << 40}, {"offsets": None}, {"x": None}, {"y": None},
+                                {"mean": None}, {"ws": None}])
+def test_group_norm_entry_refuses(kw):
+    assert group_norm(**kw) == INVALID
+    assert b"pp_group_norm" in _lib.load().pp_last_error()
+
+
+def test_group_norm_workspace():
+    lib = _lib.load()
+    assert group_norm(wsb=8) == WORKSPACE
+    assert lib.pp_group_norm_workspace(-1, 1, 8, 2, 0) == 0
+    for n in (0, 1, 65536, 65537, 1 << 33):
+        for b in (0, 1, 5000):
+            assert lib.pp_group_norm_workspace(n, b, 64, 8, 1) >= (min(1024, -(-n // 64)) + b) * 2 * 64 * 8 * (n > 0)
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros((4, 8))
+    with pytest.raises(_lib.PanopticHipError):
+        ops.group_norm_fwd(x, torch.tensor([0, 4]), 2)
+    with pytest.raises(_lib.PanopticHipError):
+        modules.group_norm_act(x.requires_grad_(), torch.tensor([0, 4]), 2)
+
+
+def test_activation_names():
+    assert ops.activation_id(None) == ops.activation_id("none") == 0
+    with pytest.raises(ValueError):
+        ops.activation_id("swish2")
