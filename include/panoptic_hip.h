@@ -405,6 +405,21 @@ int pp_group_norm_bwd(const void* x, const void* dy, int32_t dtype, int64_t n, i
                       int32_t act, float slope, void* dx, float* dweight, float* dbias, void* ws, size_t ws_bytes,
                       pp_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Linear layer of any width with bias, activation and residual in its epilogue, and its gradients   (beside pp_linear_rows: <= 32
+ * channels, fp32)
+ * x [n,cin], weight [cout,cin], bias [cout] (nullable), residual [n,cout] (nullable), y [n,cout], all of element type `dtype`.
+ * fwd: y = act(x weight^T + bias) + residual, fp32 accumulation, one rounding.
+ * bwd: dz = dy act'(x weight^T + bias) (recomputed; rounded to the element type), dx = dz weight, dweight = dz^T x, dbias = column
+ *      sums of dz; each of dx, dweight, dbias nullable.  The residual's gradient is dy itself.  Results repeat bit for bit.
+ * ---------------------------------------------------------------------------------------------- */
+int pp_linear_act_fwd(const void* x, int32_t dtype, int64_t n, int32_t cin, const void* weight, int32_t cout, const void* bias,
+                      int32_t act, float slope, const void* residual, void* y, pp_stream_t stream);
+size_t pp_linear_act_bwd_workspace(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_t act);
+int pp_linear_act_bwd(const void* x, const void* dy, int32_t dtype, int64_t n, int32_t cin, const void* weight, int32_t cout,
+                      const void* bias, int32_t act, float slope, void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes,
+                      pp_stream_t stream);
+
 /* Weight / bias gradient of a skinny Linear layer y = x W^T + b (cin, cout <= 32, millions of rows): dw [cout,cin] =
  * dy^T x, db [cout] = column sums of dy (db nullable).  replaces: the torch.nn.Linear backward (rocBLAS split-K GEMM with
  * K = n) of the heads' layers in the training step, PointGroup3heads.py:69-81 / core/common_modules/base_modules.py:35-45.

@@ -102,6 +102,9 @@ SIGNATURES = {
     "pp_group_norm_workspace": (sz, [i64, i64, i32, i32, i32]),
     "pp_group_norm_fwd": (C.c_int, [vp, i32, i64, i32, i32, vp, i64, vp, vp, vp, f64, i32, f32, vp, vp, vp, vp, sz, vp]),
     "pp_group_norm_bwd": (C.c_int, [vp, vp, i32, i64, i32, i32, vp, i64, vp, vp, vp, vp, vp, i32, f32, vp, vp, vp, vp, sz, vp]),
+    "pp_linear_act_fwd": (C.c_int, [vp, i32, i64, i32, vp, i32, vp, i32, f32, vp, vp, vp]),
+    "pp_linear_act_bwd_workspace": (sz, [i32, i64, i32, i32, i32]),
+    "pp_linear_act_bwd": (C.c_int, [vp, vp, i32, i64, i32, vp, i32, vp, i32, f32, vp, vp, vp, vp, sz, vp]),
     "pp_head_mlp": (C.c_int, [vp, i64, i32, vp, i32, vp, vp, vp, vp, i32, i32, vp, vp, vp]),
     "pp_linear_rows": (C.c_int, [vp, vp, vp, i64, i32, i32, i32, vp, vp]),
     "pp_linear_wgrad_workspace": (C.c_size_t, [i64, i32, i32]),

@@ -472,6 +472,7 @@ extern "C" int pp_group_norm_fwd(const void* x, int32_t dtype, int64_t n, int32_
   int rc = gn_check(dtype, n, c, groups, offsets, b, act);
   if (rc != PP_OK) return rc;
   PP_REQUIRE((n == 0 || (x && y)) && (b == 0 || (mean && rstd)) && ws, "pp_group_norm_fwd: null pointer");
+  PP_REQUIRE((uintptr_t)ws % 16 == 0, "pp_group_norm_fwd: the workspace must be 16-byte aligned");
   if (ws_bytes < pp_group_norm_workspace(n, b, c, groups, 0)) {
     pp_set_error("pp_group_norm_fwd: workspace too small");
     return PP_ERR_WORKSPACE;
@@ -490,6 +491,7 @@ extern "C" int pp_group_norm_bwd(const void* x, const void* dy, int32_t dtype, i
   int rc = gn_check(dtype, n, c, groups, offsets, b, act);
   if (rc != PP_OK) return rc;
   PP_REQUIRE((n == 0 || (x && dy && dx)) && (b == 0 || (mean && rstd)) && ws, "pp_group_norm_bwd: null pointer");
+  PP_REQUIRE((uintptr_t)ws % 16 == 0, "pp_group_norm_bwd: the workspace must be 16-byte aligned");
   if (ws_bytes < pp_group_norm_workspace(n, b, c, groups, 1)) {
     pp_set_error("pp_group_norm_bwd: workspace too small");
     return PP_ERR_WORKSPACE;

@@ -1,0 +1,447 @@
+// Linear layer with bias, activation and residual in the epilogue, and its gradients, on [rows, channels] features:
+//   z = x W^T + b,  y = act(z) + r;   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz,  dr = dy
+// All three products run on one tile kernel.  A workgroup of four waves owns a BM x BN tile of the result and walks the contraction
+// in steps of BK: every operand is brought to the LDS as rows of consecutive contraction elements (an operand whose contraction runs
+// down its columns is transposed on the way, in registers), 16 bytes at a time, XOR-swizzled so that the fragment reads of 16 rows
+// spread over all banks; the next step's loads are in flight while this step's fragments are multiplied.
+// fp32 operands are split exactly into three bf16 terms (8 + 8 + 8 bits) when they are staged, and a product is the six bf16 products
+// above 2^-24 of it, accumulated in fp32: an fp32-accurate evaluation at 2.7 times the rate of the fp32 matrix instructions.  A
+// non-finite value makes the results it enters NaN.  bf16 and fp16 operands are multiplied as they are, accumulated in fp32.
+// Nothing is kept for the backward pass but x: z is recomputed from it (the layers are bound by memory, a stored z would cost a write
+// and a read of its own, and its rounding would enter the gradients).  dz is rounded to the element type once, as the matrix
+// instructions take it.  The weight gradient's rows are cut into parts, whose sums are added in a fixed order: results repeat.
+#include "pp_rows.h"
+
+typedef unsigned lin_u32x4 __attribute__((ext_vector_type(4)));
+typedef float lin_f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 lin_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 lin_f16x8 __attribute__((ext_vector_type(8)));
+
+enum { LIN_FWD = 0, LIN_DZ = 1, LIN_STORE = 2, LIN_PART = 3 };
+
+struct LinArgs {
+  const void *a, *b;     // A: m rows of the contraction k (or [k, m] where it runs down the columns), B: n of it (or [k, n])
+  int64_t m, k, lda, ldb, ldo;
+  int n;
+  int va, vb;            // A / B may be read in 16-byte (columns: 8-byte) vectors
+  const void *bias, *extra;  // extra: the residual (LIN_FWD) or dy (LIN_DZ), [m, n] of row length n
+  int act;
+  float slope;
+  void* out;
+  int n_out;             // columns written (LIN_DZ pads its rows with zeros up to here)
+  int vo;                // four neighbouring columns may be stored (and `extra` read) at once
+  float *part, *part_bias;   // LIN_PART: [splits][m][n], [splits][m]
+  int64_t k_per_split;
+};
+
+template <typename T> struct LinType {
+  static constexpr int PLANES = 1, BK = 64, BUFS = 2;
+};
+template <> struct LinType<float> {
+  static constexpr int PLANES = 3, BK = 32, BUFS = 1;
+};
+
+// eight elements of the contraction, in the form they have in the LDS: PLANES x 16 bytes
+template <typename T> struct LinChunk { lin_u32x4 p[LinType<T>::PLANES]; };
+
+__device__ __forceinline__ void lin_pack(const float (&v)[8], LinChunk<float>& c) {
+  unsigned h[8], m[8], l[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {  // truncation: hi + mid + lo is v exactly, and no rounding can overflow
+    h[i] = __float_as_uint(v[i]) & 0xFFFF0000u;
+    const float r = v[i] - __uint_as_float(h[i]);
+    m[i] = __float_as_uint(r) & 0xFFFF0000u;
+    l[i] = __float_as_uint(r - __uint_as_float(m[i]));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c.p[0][i] = __builtin_amdgcn_perm(h[2 * i + 1], h[2 * i], 0x07060302u);
+    c.p[1][i] = __builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x07060302u);
+    c.p[2][i] = __builtin_amdgcn_perm(l[2 * i + 1], l[2 * i], 0x07060302u);
+  }
+}
+__device__ __forceinline__ void lin_pack(const pp_bf16 (&v)[8], LinChunk<pp_bf16>& c) { __builtin_memcpy(&c.p[0], v, 16); }
+__device__ __forceinline__ void lin_pack(const pp_f16 (&v)[8], LinChunk<pp_f16>& c) { __builtin_memcpy(&c.p[0], v, 16); }
+
+__device__ __forceinline__ lin_f32x4 lin_mma(const LinChunk<pp_bf16>& x, const LinChunk<pp_bf16>& y, lin_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lin_bf16x8, x.p[0]), __builtin_bit_cast(lin_bf16x8, y.p[0]), c, 0, 0, 0);
+}
+__device__ __forceinline__ lin_f32x4 lin_mma(const LinChunk<pp_f16>& x, const LinChunk<pp_f16>& y, lin_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(lin_f16x8, x.p[0]), __builtin_bit_cast(lin_f16x8, y.p[0]), c, 0, 0, 0);
+}
+__device__ __forceinline__ lin_f32x4 lin_mma(const LinChunk<float>& x, const LinChunk<float>& y, lin_f32x4 c) {
+#pragma unroll
+  for (int s = 2; s >= 0; --s)  // smallest products first
+#pragma unroll
+    for (int i = 0; i <= s; ++i)
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lin_bf16x8, x.p[i]), __builtin_bit_cast(lin_bf16x8, y.p[s - i]), c, 0, 0, 0);
+  return c;
+}
+
+// LDS position (in 16-byte chunks) of chunk c of row r: rows of CH chunks; 16 neighbouring rows at one c fall on 16 different slots
+template <int CH>
+__device__ __forceinline__ int lin_at(int r, int c) {
+  return r * CH + (c ^ (CH == 8 ? (r >> 1) & 7 : (r >> 2) & 3));
+}
+
+// One operand's part of a step, ROWS rows of BK contraction elements, on its way from memory to the LDS through registers
+template <typename T, bool STRIDED, int ROWS>
+struct LinStage {
+  static constexpr int BK = LinType<T>::BK, CH = BK / 8, PLANES = LinType<T>::PLANES;
+  static constexpr int COLS = sizeof(T) == 2 ? 4 : 2;                      // strided: columns of a unit
+  static constexpr int UNITS = STRIDED ? ROWS / COLS * CH : ROWS * CH;
+  static constexpr int PER = (UNITS + 255) / 256;
+  static constexpr int E = STRIDED ? 8 * COLS : 8;
+  T v[PER][E];
+
+  // row0, k0: the tile's corner; rows, k1: where the operand ends
+  __device__ __forceinline__ void load(const T* __restrict__ src, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t k1, bool vec) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int unit = threadIdx.x + 256 * i;
+      if (UNITS % 256 != 0 && unit >= UNITS) continue;
+      if constexpr (!STRIDED) {
+        const int64_t r = row0 + unit / CH, k = k0 + (unit % CH) * 8;
+        const T* p = src + r * ld + k;
+        if (vec) {
+          constexpr int W = 16 / (int)sizeof(T);
+#pragma unroll
+          for (int h = 0; h < 8 / W; ++h) {
+            lin_u32x4 q = {0u, 0u, 0u, 0u};
+            if (r < rows && k + h * W < k1) q = *(const lin_u32x4*)(p + h * W);
+            __builtin_memcpy(&v[i][h * W], &q, 16);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i][e] = r < rows && k + e < k1 ? p[e] : (T)0.f;
+        }
+      } else {
+        const int64_t c = row0 + (unit % (ROWS / COLS)) * COLS, k = k0 + unit / (ROWS / COLS) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const T* p = src + (k + e) * ld + c;
+          if (vec) {
+            unsigned long long q = 0ull;
+            if (k + e < k1 && c < rows) q = *(const unsigned long long*)p;
+            __builtin_memcpy(&v[i][e * COLS], &q, 8);
+          } else {
+#pragma unroll
+            for (int j = 0; j < COLS; ++j) v[i][e * COLS + j] = k + e < k1 && c + j < rows ? p[j] : (T)0.f;
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void put(lin_u32x4* __restrict__ lds) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int unit = threadIdx.x + 256 * i;
+      if (UNITS % 256 != 0 && unit >= UNITS) continue;
+#pragma unroll
+      for (int j = 0; j < (STRIDED ? COLS : 1); ++j) {
+        T w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = v[i][STRIDED ? e * COLS + j : e];
+        LinChunk<T> c;
+        lin_pack(w, c);
+        const int r = STRIDED ? (unit % (ROWS / COLS)) * COLS + j : unit / CH, ch = STRIDED ? unit / (ROWS / COLS) : unit % CH;
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) lds[p * ROWS * CH + lin_at<CH>(r, ch)] = c.p[p];
+      }
+    }
+  }
+  // strided only: adds the staged values to the sums of the unit's columns
+  __device__ __forceinline__ void add_columns(float (&s)[PER][COLS]) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (UNITS % 256 != 0 && threadIdx.x + 256 * i >= UNITS) continue;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) s[i][j] += (float)v[i][e * COLS + j];
+    }
+  }
+};
+
+template <typename T, int ROWS>
+__device__ __forceinline__ LinChunk<T> lin_fragment(const lin_u32x4* __restrict__ lds, int row, int ch) {
+  constexpr int CH = LinType<T>::BK / 8;
+  LinChunk<T> c;
+#pragma unroll
+  for (int p = 0; p < LinType<T>::PLANES; ++p) c.p[p] = lds[p * ROWS * CH + lin_at<CH>(row, ch)];
+  return c;
+}
+
+// four neighbouring values of a row, fp32
+template <typename T>
+__device__ __forceinline__ void lin_load4(const T* __restrict__ p, int valid, bool vec, float (&v)[4]) {
+  if (vec) {
+    if (valid > 0) pp_load<T, 4>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < valid ? (float)p[i] : 0.f;
+  }
+}
+
+// BM x BN tile, four waves of WM x WN each.  AS / BS: the contraction runs down the columns of A / B
+template <typename T, bool AS, bool BS, int MODE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
+  constexpr int BK = LinType<T>::BK, CH = BK / 8, PLANES = LinType<T>::PLANES, BUFS = LinType<T>::BUFS;
+  constexpr int FM = WM / 16, FN = WN / 16, STEP = PLANES * (BM + BN) * CH;
+  __shared__ lin_u32x4 lds[BUFS * STEP];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
+  const int64_t m0 = (int64_t)blockIdx.x * BM;
+  const int n0 = blockIdx.y * BN;
+  int64_t k = 0, k1 = a.k;
+  if (MODE == LIN_PART) {
+    k = (int64_t)blockIdx.z * a.k_per_split;
+    k1 = k + a.k_per_split < a.k ? k + a.k_per_split : a.k;
+  }
+  const T *pa = (const T*)a.a, *pb = (const T*)a.b;
+  lin_f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = (lin_f32x4){0.f, 0.f, 0.f, 0.f};
+  LinStage<T, AS, BM> sa;
+  LinStage<T, BS, BN> sb;
+  float cols[LinStage<T, AS, BM>::PER][LinStage<T, AS, BM>::COLS] = {};
+  const bool want_bias = MODE == LIN_PART && blockIdx.y == 0 && a.part_bias;
+  if (k < k1) {
+    sa.load(pa, a.lda, m0, a.m, k, k1, a.va);
+    sb.load(pb, a.ldb, n0, a.n, k, k1, a.vb);
+  }
+  for (int step = 0; k < k1; k += BK, ++step) {
+    lin_u32x4* const at = lds + (BUFS == 2 ? (step & 1) * STEP : 0);
+    if (BUFS == 1) __syncthreads();  // the last step's fragments have been read
+    sa.put(at);
+    sb.put(at + PLANES * BM * CH);
+    if (AS && want_bias) sa.add_columns(cols);
+    __syncthreads();
+    if (k + BK < k1) {
+      sa.load(pa, a.lda, m0, a.m, k + BK, k1, a.va);
+      sb.load(pb, a.ldb, n0, a.n, k + BK, k1, a.vb);
+    }
+#pragma unroll
+    for (int kk = 0; kk < BK / 32; ++kk) {
+      const int ch = kk * 4 + (lane >> 4);
+      LinChunk<T> fb[FN];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[j] = lin_fragment<T, BN>(at + PLANES * BM * CH, wn + 16 * j + (lane & 15), ch);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const LinChunk<T> fa = lin_fragment<T, BM>(at, wm + 16 * i + (lane & 15), ch);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = lin_mma(fb[j], fa, acc[i][j]);  // B first: a lane gets four neighbours of one row
+      }
+    }
+  }
+  // lane (l & 15, l >> 4) holds row l & 15 and columns 4 (l >> 4) .. + 3 of every 16 x 16 fragment
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int64_t r = m0 + wm + 16 * i + (lane & 15);
+    if (r >= a.m) continue;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int c = n0 + wn + 16 * j + 4 * (lane >> 4);
+      float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+      if (MODE == LIN_PART) {
+        float* const o = a.part + ((int64_t)blockIdx.z * a.m + r) * a.n + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < a.n) o[e] = v[e];
+        continue;
+      }
+      const int valid = a.n - c;
+      if (MODE == LIN_FWD || MODE == LIN_DZ) {
+        float b[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f};
+        if (a.bias) lin_load4((const T*)a.bias + c, valid, false, b);
+        if (a.extra) lin_load4((const T*)a.extra + r * a.n + c, valid, a.vo, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = MODE == LIN_FWD ? pp_act1(v[e] + b[e], a.act, a.slope) + x[e]
+                                 : (e < valid ? x[e] * pp_dact1(v[e] + b[e], a.act, a.slope) : 0.f);  // (padding is 0, whatever the row holds)
+      }
+      T* const o = (T*)a.out + r * a.ldo + c;
+      if (a.vo) {
+        if (c < a.n_out) pp_store<T, 4>(o, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < a.n_out) o[e] = (T)v[e];
+      }
+    }
+  }
+  if constexpr (MODE == LIN_PART && AS) {
+    if (want_bias) {  // the columns' sums of the threads that staged other parts of the contraction, in their order
+      typedef LinStage<T, AS, BM> S;
+      constexpr int QUADS = BM / S::COLS;
+      float* const red = (float*)lds;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < S::PER; ++i)
+#pragma unroll
+        for (int j = 0; j < S::COLS; ++j) {
+          const int unit = threadIdx.x + 256 * i;
+          if (unit < S::UNITS) red[unit / QUADS * BM + (unit % QUADS) * S::COLS + j] = cols[i][j];
+        }
+      __syncthreads();
+      if (threadIdx.x < BM && m0 + threadIdx.x < a.m) {
+        float s = 0.f;
+        for (int q = 0; q < CH; ++q) s += red[q * BM + threadIdx.x];
+        a.part_bias[(int64_t)blockIdx.z * a.m + m0 + threadIdx.x] = s;
+      }
+    }
+  }
+}
+
+// adds the parts of the weight and bias gradient in their order
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_parts(const float* __restrict__ part, const float* __restrict__ part_bias, int splits,
+                                                      int64_t nw, int64_t nb, T* __restrict__ dw, T* __restrict__ db) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < nw) {
+    double s = 0.0;
+    for (int q = 0; q < splits; ++q) s += (double)part[q * nw + i];
+    dw[i] = (T)(float)s;
+  } else if (i < nw + nb) {
+    double s = 0.0;
+    for (int q = 0; q < splits; ++q) s += (double)part_bias[q * nb + (i - nw)];
+    db[i - nw] = (T)(float)s;
+  }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------------------------------
+template <typename T, bool AS, bool BS, int MODE, int BM, int BN, int WM, int WN>
+static int lin_go(const LinArgs& a, int splits, hipStream_t s) {
+  const int64_t mt = (a.m + BM - 1) / BM;
+  const int nt = ((MODE == LIN_DZ ? a.n_out : a.n) + BN - 1) / BN;
+  PP_REQUIRE(mt <= 0x7FFFFFFF && nt <= 65535 && splits <= 65535, "pp_linear_act: too many tiles");
+  hipLaunchKernelGGL((k_linear_tile<T, AS, BS, MODE, BM, BN, WM, WN>), dim3((unsigned)mt, nt, splits), dim3(256), 0, s, a);
+  PP_LAUNCH_CHECK();
+  return PP_OK;
+}
+template <typename T, bool AS, bool BS, int MODE>
+static int lin_tile(const LinArgs& a, int splits, hipStream_t s) {
+  if (a.n > 64) return lin_go<T, AS, BS, MODE, 128, 128, 64, 64>(a, splits, s);
+  return lin_go<T, AS, BS, MODE, 128, 64, 32, 64>(a, splits, s);
+}
+
+static bool lin_aligned(const void* p, int64_t ld, int bytes, size_t size) { return (uintptr_t)p % bytes == 0 && (ld * size) % bytes == 0; }
+
+// parts of the weight gradient's contraction: about two workgroups per compute unit in all, at least 256 rows each
+static int lin_splits(int64_t n, int cin, int cout) {
+  const int64_t tiles = (int64_t)((cout + 127) / 128) * ((cin + (cin > 64 ? 127 : 63)) / (cin > 64 ? 128 : 64));
+  int64_t s = 512 / tiles;
+  if (s > (n + 255) / 256) s = (n + 255) / 256;
+  return s < 1 ? 1 : (int)s;
+}
+static int64_t lin_ldz(int cout) { return (cout + 7) / 8 * 8; }
+
+extern "C" size_t pp_linear_act_bwd_workspace(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_t act) {
+  if (n < 0 || cin < 1 || cout < 1) return 0;
+  const size_t parts = (size_t)lin_splits(n, cin, cout);
+  return pp_align(parts * cout * cin * 4) + pp_align(parts * cout * 4) +
+         (act == PP_ACT_NONE ? 0 : pp_align((size_t)n * lin_ldz(cout) * pp_dtype_bytes(dtype))) + 256;
+}
+
+static int lin_check(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_t act) {
+  PP_REQUIRE(pp_rows_dtype_ok(dtype), "pp_linear_act: unknown element type");
+  PP_REQUIRE(pp_rows_act_ok(act), "pp_linear_act: unknown activation");
+  PP_REQUIRE(cin >= 1 && cin <= (1 << 20) && cout >= 1 && cout <= (1 << 20), "pp_linear_act: channels out of range");
+  PP_REQUIRE(n >= 0 && n <= ((int64_t)1 << 36), "pp_linear_act: rows out of range");
+  return PP_OK;
+}
+
+template <typename T>
+static LinArgs lin_base(const void* x, int64_t n, int cin, const void* w, int cout, const void* bias, int act, float slope) {
+  LinArgs a{};
+  a.a = x; a.b = w; a.m = n; a.n = cout; a.k = cin; a.lda = cin; a.ldb = cin;
+  a.va = lin_aligned(x, cin, 16, sizeof(T)); a.vb = lin_aligned(w, cin, 16, sizeof(T));
+  a.bias = bias; a.act = act; a.slope = slope;
+  return a;
+}
+
+template <typename T>
+static int lin_forward(const void* x, int64_t n, int cin, const void* w, int cout, const void* bias, int act, float slope,
+                       const void* residual, void* y, hipStream_t s) {
+  LinArgs a = lin_base<T>(x, n, cin, w, cout, bias, act, slope);
+  a.extra = residual; a.out = y; a.ldo = cout; a.n_out = cout;
+  a.vo = cout % 4 == 0 && lin_aligned(y, cout, 4 * sizeof(T), sizeof(T)) && lin_aligned(residual, cout, 4 * sizeof(T), sizeof(T));
+  return lin_tile<T, false, false, LIN_FWD>(a, 1, s);
+}
+
+template <typename T>
+static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const void* w, int cout, const void* bias, int act, float slope,
+                        void* dx, void* dw, void* db, PPArena& ws, hipStream_t s) {
+  const int splits = lin_splits(n, cin, cout);
+  float* part = ws.take<float>((size_t)splits * cout * cin);
+  float* part_bias = ws.take<float>((size_t)splits * cout);
+  const T* dz = (const T*)dy;
+  int64_t ldz = cout;
+  int rc;
+  if (act != PP_ACT_NONE) {
+    ldz = lin_ldz(cout);
+    T* z = ws.take<T>((size_t)n * ldz);
+    PP_REQUIRE(z || n == 0, "pp_linear_act_bwd: workspace layout");
+    dz = z;
+    if (n) {
+      LinArgs a = lin_base<T>(x, n, cin, w, cout, bias, act, slope);
+      a.extra = dy; a.out = z; a.ldo = ldz; a.n_out = (int)ldz;
+      a.vo = cout % 4 == 0 && lin_aligned(dy, cout, 4 * sizeof(T), sizeof(T));
+      if ((rc = lin_tile<T, false, false, LIN_DZ>(a, 1, s)) != PP_OK) return rc;
+    }
+  }
+  PP_REQUIRE(part && part_bias, "pp_linear_act_bwd: workspace layout");
+  if (dx && n) {
+    LinArgs a{};
+    a.a = dz; a.lda = ldz; a.b = w; a.ldb = cin; a.m = n; a.n = cin; a.k = cout; a.out = dx; a.ldo = cin; a.n_out = cin;
+    a.va = lin_aligned(dz, ldz, 16, sizeof(T)); a.vb = lin_aligned(w, cin, 8, sizeof(T));
+    a.vo = cin % 4 == 0 && lin_aligned(dx, cin, 4 * sizeof(T), sizeof(T));
+    if ((rc = lin_tile<T, false, true, LIN_STORE>(a, 1, s)) != PP_OK) return rc;
+  }
+  if (dw || db) {
+    LinArgs a{};
+    a.a = dz; a.lda = ldz; a.b = x; a.ldb = cin; a.m = cout; a.n = cin; a.k = n;
+    a.va = lin_aligned(dz, ldz, 8, sizeof(T)); a.vb = lin_aligned(x, cin, 8, sizeof(T));
+    a.part = part; a.part_bias = part_bias;
+    a.k_per_split = ((n + splits - 1) / splits + 63) / 64 * 64;
+    if ((rc = lin_tile<T, true, true, LIN_PART>(a, splits, s)) != PP_OK) return rc;
+    const int64_t nw = dw ? (int64_t)cout * cin : 0, nb = db ? cout : 0;
+    hipLaunchKernelGGL((k_linear_parts<T>), dim3((unsigned)((nw + nb + 255) / 256)), dim3(256), 0, s, part, part_bias, splits, nw, nb,
+                       (T*)dw, (T*)db);
+    PP_LAUNCH_CHECK();
+  }
+  return PP_OK;
+}
+
+extern "C" int pp_linear_act_fwd(const void* x, int32_t dtype, int64_t n, int32_t cin, const void* weight, int32_t cout, const void* bias,
+                                 int32_t act, float slope, const void* residual, void* y, pp_stream_t stream) {
+  int rc = lin_check(dtype, n, cin, cout, act);
+  if (rc != PP_OK) return rc;
+  PP_REQUIRE(weight && (n == 0 || (x && y)), "pp_linear_act_fwd: null pointer");
+  if (n == 0) return PP_OK;
+  hipStream_t s = pp_s(stream);
+  if (dtype == PP_F32) return lin_forward<float>(x, n, cin, weight, cout, bias, act, slope, residual, y, s);
+  if (dtype == PP_BF16) return lin_forward<pp_bf16>(x, n, cin, weight, cout, bias, act, slope, residual, y, s);
+  return lin_forward<pp_f16>(x, n, cin, weight, cout, bias, act, slope, residual, y, s);
+}
+
+extern "C" int pp_linear_act_bwd(const void* x, const void* dy, int32_t dtype, int64_t n, int32_t cin, const void* weight, int32_t cout,
+                                 const void* bias, int32_t act, float slope, void* dx, void* dweight, void* dbias, void* ws,
+                                 size_t ws_bytes, pp_stream_t stream) {
+  int rc = lin_check(dtype, n, cin, cout, act);
+  if (rc != PP_OK) return rc;
+  PP_REQUIRE(weight && ws && (n == 0 || (x && dy)), "pp_linear_act_bwd: null pointer");
+  PP_REQUIRE((uintptr_t)ws % 16 == 0, "pp_linear_act_bwd: the workspace must be 16-byte aligned");
+  if (ws_bytes < pp_linear_act_bwd_workspace(dtype, n, cin, cout, act)) {
+    pp_set_error("pp_linear_act_bwd: workspace too small");
+    return PP_ERR_WORKSPACE;
+  }
+  PPArena arena(ws, ws_bytes);
+  hipStream_t s = pp_s(stream);
+  if (dtype == PP_F32) return lin_backward<float>(x, dy, n, cin, weight, cout, bias, act, slope, dx, dweight, dbias, arena, s);
+  if (dtype == PP_BF16) return lin_backward<pp_bf16>(x, dy, n, cin, weight, cout, bias, act, slope, dx, dweight, dbias, arena, s);
+  return lin_backward<pp_f16>(x, dy, n, cin, weight, cout, bias, act, slope, dx, dweight, dbias, arena, s);
+}

@@ -112,6 +112,36 @@ class _SkinnyLinearFn(torch.autograd.Function):
         return dx, dw, db
 
 
+class _LinearActFn(torch.autograd.Function):
+    """keeps x, weight and bias only: the backward recomputes the pre-activation (csrc/pp_linear.hip)"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, act, slope, residual):
+        ctx.save_for_backward(x, weight, bias)
+        ctx.cfg = (act, slope)
+        return ops.linear_act_fwd(x, weight, bias, act, slope, residual)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if need[0] or need[1] or need[2]:
+            dx, dw, db = ops.linear_act_bwd(x, dy, weight, bias, *ctx.cfg, want_input=need[0], want_weight=need[1], want_bias=need[2])
+        return dx, dw, db, None, None, dy if need[5] else None
+
+
+def linear_act(x, weight, bias=None, activation="none", slope=0.2, residual=None):
+    """y = act(x W^T + bias) + residual as one launch, differentiable in all four operands.  x [n, cin], weight [cout, cin] (the
+    layout of torch.nn.Linear), bias [cout] or None, residual [n, cout] or None, all of one type (float32, bfloat16, float16).
+    activation: none, relu, leaky_relu (with `slope`), silu or gelu (exact); it acts before the residual is added, as in ResBlock."""
+    act = ops.activation_id(activation)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearActFn.apply(x, weight, bias, act, slope, residual)
+    return ops.linear_act_fwd(x, weight, bias, act, slope, residual)
+
+
 class Linear(nn.Linear):
     """torch.nn.Linear (same parameters, same state_dict keys) whose backward takes the streaming weight gradient when the
     layer is skinny and the input is a large device matrix; everything else is the parent's."""

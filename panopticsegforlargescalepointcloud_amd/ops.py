@@ -1329,6 +1329,49 @@ def group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act=0, 
     return dx, dwb[0], dwb[1]
 
 
+def _linear_act_operands(x, weight, bias):
+    if x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1] or 0 in weight.shape:
+        raise ValueError("linear_act: weight %s does not fit input %s" % (tuple(weight.shape), tuple(x.shape)))
+    return (_beside(weight, x, x.dtype, weight.shape, "weight"), _beside(bias, x, x.dtype, weight.shape[:1], "bias"))
+
+
+@_on_device_of
+def linear_act_fwd(x, weight, bias=None, act=0, slope=0.0, residual=None):
+    """y = act(x W^T + bias) + residual in one launch (csrc/pp_linear.hip): x [n, cin], weight [cout, cin], bias [cout], residual
+    [n, cout], all of one type (float32, bfloat16, float16); any width and any number of rows."""
+    lib = _lib.load()
+    code = _row_dtype(x, "x")
+    weight, bias = _linear_act_operands(x, weight, bias)
+    x = x if x.is_contiguous() else x.contiguous()
+    n, cin = x.shape
+    cout = weight.shape[0]
+    residual = _beside(residual, x, x.dtype, (n, cout), "residual")
+    y = torch.empty((n, cout), dtype=x.dtype, device=x.device)
+    _lib.check(lib.pp_linear_act_fwd(_ptr(x), code, n, cin, _ptr(weight), cout, _ptr(bias), int(act), float(slope), _ptr(residual), _ptr(y),
+                                     _stream()), "pp_linear_act_fwd")
+    return y
+
+
+@_on_device_of
+def linear_act_bwd(x, dy, weight, bias=None, act=0, slope=0.0, want_input=True, want_weight=True, want_bias=True):
+    """Backward of linear_act_fwd: (dx, dweight, dbias), None for what is not wanted; the residual's gradient is dy."""
+    lib = _lib.load()
+    code = _row_dtype(x, "x")
+    weight, bias = _linear_act_operands(x, weight, bias)
+    x = x if x.is_contiguous() else x.contiguous()
+    n, cin = x.shape
+    cout = weight.shape[0]
+    dy = _beside(dy, x, x.dtype, (n, cout), "dy")
+    dx = torch.empty_like(x) if want_input else None
+    dw = torch.empty_like(weight) if want_weight else None
+    db = torch.empty(cout, dtype=x.dtype, device=x.device) if want_bias else None
+    wsb = lib.pp_linear_act_bwd_workspace(code, n, cin, cout, int(act))
+    ws = _ws(wsb, x.device)
+    _lib.check(lib.pp_linear_act_bwd(_ptr(x), _ptr(dy), code, n, cin, _ptr(weight), cout, _ptr(bias), int(act), float(slope), _ptr(dx),
+                                     _ptr(dw), _ptr(db), _ptr(ws), ws.numel(), _stream()), "pp_linear_act_bwd")
+    return dx, dw, db
+
+
 def linear_rows(x, weight, bias=None, transposed=False):
     """y = x W^T + bias (weight [cout, cin]) or, transposed, y = x W (weight [cin, cout] as stored) for skinny layers (<= 32
     channels either side): csrc/pp_dense.hip k_linear_rows instead of a library GEMM."""

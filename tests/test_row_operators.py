@@ -47,3 +47,24 @@ def test_activation_names():
     assert ops.activation_id(None) == ops.activation_id("none") == 0
     with pytest.raises(ValueError):
         ops.activation_id("swish2")
+
+
+def linear(**kw):
+    a = dict(x=P, dtype=0, n=10, cin=8, w=P, cout=8, bias=None, act=0, slope=0.0, residual=None, y=P, stream=None)
+    a.update(kw)
+    return _lib.load().pp_linear_act_fwd(*a.values())
+
+
+@pytest.mark.parametrize("kw", [{"dtype": 3}, {"act": 5}, {"cin": 0}, {"cout": 0}, {"cout": (1 << 20) + 1}, {"n": -1}, {"w": None},
+                                {"x": None}, {"y": None}])
+def test_linear_act_entry_refuses(kw):
+    assert linear(**kw) == INVALID
+
+
+def test_linear_act_backward_entry_refuses():
+    lib = _lib.load()
+    a = [P, P, 0, 10, 8, P, 8, None, 3, 0.0, P, P, P, P, lib.pp_linear_act_bwd_workspace(0, 10, 8, 8, 3), None]
+    for at, value, rc in ((1, None, INVALID), (13, None, INVALID), (14, 100, WORKSPACE), (13, C.c_void_p(4100), INVALID), (8, 7, INVALID)):
+        assert lib.pp_linear_act_bwd(*(a[:at] + [value] + a[at + 1:])) == rc
+    with pytest.raises(_lib.PanopticHipError):
+        modules.linear_act(torch.zeros((4, 8)), torch.zeros((3, 8)))
