@@ -420,6 +420,16 @@ int pp_linear_act_bwd(const void* x, const void* dy, int32_t dtype, int64_t n, i
                       const void* bias, int32_t act, float slope, void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes,
                       pp_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Orthogonalisation of weight updates by Newton-Schulz products   (training.Muon)
+ * g, out [batch,m,n] of element type `dtype`.  X = g / (|g| + eps) per matrix (Frobenius norm), then `steps` times
+ * X <- a X + (b A + c A^2) X with A = X X^T on the shorter side (at most 8192).  Computed on the Gram matrix of the shorter side in
+ * float64; results repeat bit for bit.
+ * ---------------------------------------------------------------------------------------------- */
+size_t pp_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n);
+int pp_newton_schulz(const void* g, int32_t dtype, int64_t batch, int64_t m, int64_t n, int32_t steps, double a, double b, double c,
+                     double eps, void* out, void* ws, size_t ws_bytes, pp_stream_t stream);
+
 /* Weight / bias gradient of a skinny Linear layer y = x W^T + b (cin, cout <= 32, millions of rows): dw [cout,cin] =
  * dy^T x, db [cout] = column sums of dy (db nullable).  replaces: the torch.nn.Linear backward (rocBLAS split-K GEMM with
  * K = n) of the heads' layers in the training step, PointGroup3heads.py:69-81 / core/common_modules/base_modules.py:35-45.

@@ -1372,6 +1372,34 @@ def linear_act_bwd(x, dy, weight, bias=None, act=0, slope=0.0, want_input=True, 
     return dx, dw, db
 
 
+NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+@_on_device_of
+def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7):
+    """Orthogonalises a matrix [m, n] or a batch of them [batch, m, n] (float32, bfloat16, float16): X = g / (|g| + eps), then `steps`
+    times X <- a X + (b A + c A^2) X with A = X X^T (csrc/pp_newtonschulz.hip).  With the default coefficients five steps bring every
+    singular value above 1e-3 of the norm to 0.7 .. 1.2.  Same shape and type as g; the shorter side is at most 8192."""
+    lib = _lib.load()
+    code = _row_dtype(g, "g")
+    if g.dim() not in (2, 3) or 0 in g.shape[-2:]:
+        raise ValueError("newton_schulz: g must be [m, n] or [batch, m, n], got %s" % (tuple(g.shape),))
+    m, n = g.shape[-2:]
+    batch = g.shape[0] if g.dim() == 3 else 1
+    if min(m, n) > 8192:
+        raise ValueError("newton_schulz: the shorter side is at most 8192, got %d" % min(m, n))
+    if steps < 1:
+        raise ValueError("newton_schulz: at least one step, got %d" % steps)
+    a, b, c = coefficients
+    g = g if g.is_contiguous() else g.contiguous()
+    out = torch.empty_like(g)
+    wsb = lib.pp_newton_schulz_workspace(batch, m, n)
+    ws = _ws(wsb, g.device)
+    _lib.check(lib.pp_newton_schulz(_ptr(g), code, batch, m, n, int(steps), float(a), float(b), float(c), float(eps), _ptr(out), _ptr(ws),
+                                    ws.numel(), _stream()), "pp_newton_schulz")
+    return out
+
+
 def linear_rows(x, weight, bias=None, transposed=False):
     """y = x W^T + bias (weight [cout, cin]) or, transposed, y = x W (weight [cin, cout] as stored) for skinny layers (<= 32
     channels either side): csrc/pp_dense.hip k_linear_rows instead of a library GEMM."""

@@ -1,0 +1,132 @@
+"""Newton-Schulz orthogonalisation (ops.newton_schulz) and the optimiser built on it against the iteration in 64 bits.
+
+Error bound.  The steps run in fp64 on the Gram matrix S of the shorter side s.  An error of S grows by at most a^2 = 11.9 a step
+(in the directions where S is near 0; elsewhere the iteration contracts), a product of s terms rounds by s 2^-53 at most, and a step
+has four of them: 4 s 2^-53 (1 + 11.9 + .. + 11.9^(steps - 1)) < 4 s 2^-53 1.1 a^(2 steps - 2), taken relative to the largest value an
+entry can have (the largest singular value, 1.3).  The result is rounded to fp32 and to its type."""
+import pytest
+import torch
+
+from panopticsegforlargescalepointcloud_amd import _lib, ops
+from test_groupnorm_gpu import HALF_STEP, TINY
+
+pytestmark = pytest.mark.gpu
+A, B, C = ops.NEWTON_SCHULZ_COEFFICIENTS
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def iterate(g, steps=5, coefficients=(A, B, C), eps=1e-7):
+    """the definition, one matrix, 64 bits on the CPU"""
+    a, b, c = coefficients
+    x = g.detach().double().cpu()
+    x = x / (x.norm() + eps)
+    tall = x.shape[0] > x.shape[1]
+    x = x.t() if tall else x
+    for _ in range(steps):
+        s = x @ x.t()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x.t() if tall else x
+
+
+def check(g, steps=5, coefficients=(A, B, C), eps=1e-7):
+    out = ops.newton_schulz(g, steps, coefficients, eps)
+    assert out.shape == g.shape and out.dtype == g.dtype
+    U = HALF_STEP[g.dtype]
+    s = min(g.shape[-2:])
+    for o, x in zip(out.view(-1, *g.shape[-2:]), g.view(-1, *g.shape[-2:])):
+        want = iterate(x, steps, coefficients, eps)
+        room = (U + 2.0 ** -24) * want.abs() + 4 * s * 2.0 ** -53 * 1.1 * abs(coefficients[0]) ** (2 * steps - 2) * 1.3 + TINY[g.dtype]
+        over = (o.double().cpu() - want).abs() - room
+        assert bool((over <= 0).all()), (tuple(g.shape), float(over.max()))
+
+
+def matrices(batch, m, n, dtype, seed=0, scale=1e-3):
+    """a few strong directions over a floor of noise"""
+    gen = torch.Generator().manual_seed(seed)
+    k = max(1, min(m, n) // 8)
+    strong = torch.randn((batch, m, k), generator=gen) / (1 + torch.arange(k)) @ torch.randn((batch, k, n), generator=gen)
+    return ((strong + torch.randn((batch, m, n), generator=gen)) * scale).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,m,n", [
+    (1, 1, 1), (1, 1, 9), (2, 9, 1), (3, 5, 5), (1, 16, 64), (2, 64, 64), (4, 65, 64), (1, 63, 200), (2, 130, 75), (3, 432, 16),
+    (2, 1728, 64), (1, 864, 112), (2, 96, 700), (1, 257, 129), (1, 200, 256), (5, 33, 31),
+])
+def test_shapes(batch, m, n, dtype):
+    check(matrices(batch, m, n, dtype, seed=m + n))
+
+
+def test_one_matrix_and_other_polynomials():
+    g = matrices(1, 80, 48, torch.float32)[0]
+    check(g)
+    for steps in (1, 2, 3, 8):
+        check(g, steps=steps)
+    check(g, coefficients=(1.5, -0.5, 0.0))  # the cubic iteration
+    check(g, eps=0.0)
+    check(g, eps=1.0)
+
+
+def test_scales_and_strong_directions():
+    for scale in (1e-18, 1e-6, 1e6, 1e18):  # squares of the small ones vanish in fp32
+        check(matrices(2, 100, 40, torch.float32, scale=scale), eps=0.0)
+    g = torch.randn(60, 1, device="cuda") @ torch.randn(1, 90, device="cuda")  # rank one: all other directions are rounding noise
+    check(g)
+
+
+def test_zero_nan_and_inf_stay_in_their_matrix():
+    g = matrices(4, 70, 90, torch.float32)
+    clean = ops.newton_schulz(g)
+    h = g.clone()
+    h[0] = 0
+    h[1, 3, 4] = float("nan")
+    h[2, 60, 0] = float("inf")
+    out = ops.newton_schulz(h)
+    assert torch.equal(out[0], torch.zeros_like(out[0])) and torch.equal(out[3], clean[3])
+    assert torch.isnan(out[1]).all() and torch.isnan(out[2]).all()
+
+
+def test_singular_values_come_near_one():
+    g = torch.randn(3, 300, 64, device="cuda")
+    sv = torch.linalg.svdvals(ops.newton_schulz(g).double().cpu())
+    assert float(sv.min()) > 0.6 and float(sv.max()) < 1.3
+
+
+def test_batch_strides_repeats_stream_and_graph():
+    g = matrices(6, 200, 96, torch.bfloat16)
+    want = ops.newton_schulz(g)
+    assert torch.equal(want, ops.newton_schulz(g))
+    assert torch.equal(want[2], ops.newton_schulz(g[2])) or torch.allclose(want[2].float(), ops.newton_schulz(g[2]).float(), rtol=2.0 ** -7)
+    assert torch.equal(ops.newton_schulz(g.transpose(1, 2)), ops.newton_schulz(g.transpose(1, 2).contiguous()))
+    assert torch.equal(ops.newton_schulz(g[:, ::2]), ops.newton_schulz(g[:, ::2].contiguous()))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.newton_schulz(g)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    static = g.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.newton_schulz(static)
+    for k in range(3):
+        static.copy_(g.flip(0) * (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.newton_schulz(static)), k
+
+
+def test_refusals():
+    g = torch.randn(8, 8, device="cuda")
+    for bad, err in ((torch.zeros(8, device="cuda"), ValueError), (torch.zeros(2, 2, 2, 2, device="cuda"), ValueError),
+                     (torch.zeros(0, 8, device="cuda"), ValueError), (g.double(), TypeError), (g.cpu(), _lib.PanopticHipError)):
+        with pytest.raises(err):
+            ops.newton_schulz(bad)
+    with pytest.raises(ValueError):
+        ops.newton_schulz(g, steps=0)
+    with pytest.raises(_lib.PanopticHipError):
+        ops.newton_schulz(g, eps=-1.0)
+    with pytest.raises(ValueError):
+        ops.newton_schulz(g, coefficients=(1.0, 2.0))
+    assert ops.newton_schulz(torch.zeros(0, 4, 4, device="cuda")).shape == (0, 4, 4)

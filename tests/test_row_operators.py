@@ -68,3 +68,15 @@ def test_linear_act_backward_entry_refuses():
         assert lib.pp_linear_act_bwd(*(a[:at] + [value] + a[at + 1:])) == rc
     with pytest.raises(_lib.PanopticHipError):
         modules.linear_act(torch.zeros((4, 8)), torch.zeros((3, 8)))
+
+
+def test_newton_schulz_entry_refuses():
+    lib = _lib.load()
+    a = [P, 0, 2, 40, 30, 5, 3.4, -4.7, 2.0, 1e-7, P, P, lib.pp_newton_schulz_workspace(2, 40, 30), None]
+    for at, value, rc in ((1, 4, INVALID), (2, -1, INVALID), (2, 1 << 17, INVALID), (3, 0, INVALID), (4, 1 << 40, INVALID), (5, 0, INVALID),
+                          (5, 101, INVALID), (9, -1.0, INVALID), (0, None, INVALID), (11, C.c_void_p(4104), INVALID), (12, 10, WORKSPACE)):
+        assert lib.pp_newton_schulz(*(a[:at] + [value] + a[at + 1:])) == rc, at
+    assert lib.pp_newton_schulz(*(a[:3] + [9000, 9000] + a[5:])) == INVALID
+    assert lib.pp_newton_schulz_workspace(1, 0, 4) == 0
+    with pytest.raises(_lib.PanopticHipError):
+        ops.newton_schulz(torch.zeros(4, 4))
