@@ -5,6 +5,7 @@ Only the symbols the reference's hot path uses are provided:
   MinkowskiConvolution / MinkowskiConvolutionTranspose (.kernel)      api_modules.py:30-51,259-267
   MinkowskiBatchNorm (.bn = BatchNorm1d, settable momentum)           api_modules.py:40 ; core/schedulers/bn_schedulers.py:6-31
   MinkowskiReLU, MinkowskiNetwork, cat, utils.kaiming_normal_        api_modules.py:41,308 ; applications/minkowski.py:104-111
+  MinkowskiGroupNorm / MinkowskiInstanceNorm: normalisation that does not depend on the batch (`norm: group` in a backbone's sections)
   (MinkowskiLinear, MinkowskiSigmoid, MinkowskiGlobalPooling, MinkowskiBroadcastMultiplication: imported by
    api_modules.py:176-186 for SE blocks that no panoptic config uses; provided as thin modules.)
 
@@ -22,6 +23,7 @@ import torch
 from torch import nn
 
 from .. import ops
+from ..functional import group_norm_act
 from . import utils  # noqa: F401
 
 
@@ -262,6 +264,7 @@ class CoordinateManager:
         self.levels = {}
         self.maps = {}
         self._pending_same = {}
+        self._batch_rows, self._batch_rows_stream, self._batch_size = {}, {}, None
         self._lock = threading.RLock()
         self._ready = {}
         self._log = None
@@ -401,6 +404,32 @@ class CoordinateManager:
             elif isinstance(it, (tuple, list)):
                 flat.extend(t for t in it if torch.is_tensor(t))
         self._consumed_here(*flat)
+
+    def batch_rows(self, ts):
+        """(offsets, order) of a level's rows by batch element: element s owns the rows order[offsets[s]:offsets[s+1]] (int64 on the
+        device; order None: the rows are all one element's).  Built at the first request -- the physical order of a level's rows
+        (windows sorted by neighbour mask) mixes the elements that meet in a window -- and kept for the other layers."""
+        coords = self.level(ts).coords
+        with self._lock:
+            got = self._batch_rows.get(ts)
+            if got is None:
+                if self._batch_size is None:  # one host read per manager
+                    self._batch_size = int(self.orig_coords[:, 0].max()) + 1 if self.orig_coords.shape[0] else 0
+                n = coords.shape[0]
+                if self._batch_size <= 1:
+                    got = (torch.tensor([0, n][: self._batch_size + 1], dtype=torch.int64, device=coords.device), None)
+                else:
+                    offs, rows, _ = ops.group_by_key(coords[:, 0].contiguous(), self._batch_size)
+                    got = (offs.to(torch.int64), rows[:n])
+                self._batch_rows[ts] = got
+                self._batch_rows_stream[ts] = _raw_stream()
+                self._built(("batch_rows", ts))
+        self._use(("batch_rows", ts))
+        if self._batch_rows_stream[ts] != _raw_stream():
+            for t in got:
+                if t is not None:
+                    t.record_stream(_current_stream())
+        return got
 
     def level(self, ts):
         self._use(("level", ts))
@@ -1114,6 +1143,33 @@ class MinkowskiBatchNorm(nn.Module):
 
     def __repr__(self):
         return "MinkowskiBatchNorm(%s)" % self.bn.extra_repr()
+
+
+class MinkowskiGroupNorm(nn.Module):
+    """Group normalisation over the rows of each batch element and the channels of each group, with an optional activation (none, relu,
+    leaky_relu, silu, gelu) in the same launches.  Parameters gn.weight / gn.bias (float32).  Training and inference compute the same,
+    and a row's result does not depend on the other batch elements -- what BatchNorm needs several cylinders per GPU for."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation=None, slope=0.2):
+        super().__init__()
+        self.gn = nn.GroupNorm(num_groups, num_channels, eps=eps, affine=affine)
+        ops.activation_id(activation)  # refuses unknown names at construction
+        self.activation, self.slope = activation, slope
+
+    def forward(self, x):
+        offsets, order = x.coordinate_manager.batch_rows(x.tensor_stride)
+        return x._like(group_norm_act(x.feats, offsets, self.gn.num_groups, self.gn.weight, self.gn.bias, eps=self.gn.eps,
+                                      activation=self.activation, slope=self.slope, order=order))
+
+    def __repr__(self):
+        return "%s(%s, activation=%s)" % (type(self).__name__, self.gn.extra_repr(), self.activation)
+
+
+class MinkowskiInstanceNorm(MinkowskiGroupNorm):
+    """one group per channel"""
+
+    def __init__(self, num_features, eps=1e-5, affine=True, activation=None, slope=0.2):
+        super().__init__(num_features, num_features, eps=eps, affine=affine, activation=activation, slope=slope)
 
 
 class MinkowskiReLU(nn.Module):

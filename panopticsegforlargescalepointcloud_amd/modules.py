@@ -17,6 +17,7 @@ from torch import nn
 
 from . import MinkowskiEngine as ME
 from . import ops
+from .functional import group_norm_act, linear_act  # noqa: F401
 
 
 class Seq(nn.Sequential):
@@ -51,38 +52,6 @@ class FastBatchNorm1d(nn.Module):
         raise ValueError("Non supported number of dimensions {}".format(x.dim()))
 
 
-class _GroupNormActFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, offsets, num_groups, weight, bias, eps, act, slope, order):
-        x = x.contiguous()
-        y, mean, rstd = ops.group_norm_fwd(x, offsets, num_groups, weight, bias, eps, act, slope, order)
-        ctx.save_for_backward(x, offsets, weight, bias, mean, rstd, order)
-        ctx.cfg = (num_groups, act, slope)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, offsets, weight, bias, mean, rstd, order = ctx.saved_tensors
-        num_groups, act, slope = ctx.cfg
-        dx, dw, db = ops.group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act, slope, order)
-        return dx, None, None, dw if weight is not None else None, db if bias is not None else None, None, None, None, None
-
-
-def group_norm_act(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, activation="none", slope=0.2, order=None):
-    """y = act(group_norm(x)): statistics over the rows of each batch element and the channels of each group, differentiable in x,
-    weight and bias.  x [n, c] (float32, bfloat16 or float16), weight / bias float32 [c] or None.  Batch element s owns the
-    positions offsets[s] .. offsets[s+1] of the row sequence (int64 [batch + 1] on the device, ascending); position p is row
-    order[p] (int64 [n], each row once) or, without an order, row p.  Rows of no batch element (padding) come out as zeros and
-    get zero gradients.  activation: none, relu, leaky_relu (with `slope`), silu or gelu (exact).  num_groups = c: instance norm.
-    Beside FastBatchNorm1d: the result for a row does not depend on the other batch elements, in training and in inference."""
-    act = ops.activation_id(activation)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
-        return _GroupNormActFn.apply(x, offsets, num_groups, weight, bias, eps, act, slope, order)
-    return ops.group_norm_fwd(x, offsets, num_groups, weight, bias, eps, act, slope, order)[0]
-
-
 # forward / input gradient of the skinny Linear layers from the library (PP_LINEAR_ROWS=0: torch GEMMs, A/B runs)
 LINEAR_ROWS = os.environ.get("PP_LINEAR_ROWS", "1") != "0"
 
@@ -112,34 +81,27 @@ class _SkinnyLinearFn(torch.autograd.Function):
         return dx, dw, db
 
 
-class _LinearActFn(torch.autograd.Function):
-    """keeps x, weight and bias only: the backward recomputes the pre-activation (csrc/pp_linear.hip)"""
+class LinearAct(nn.Linear):
+    """torch.nn.Linear (same parameters, same state_dict keys) with the activation and a residual in its epilogue: one launch forward,
+    the pre-activation recomputed backward (functional.linear_act).  Takes row matrices [n, in_features] and sparse tensors, whose
+    residual is a sparse tensor on the same coordinate map."""
 
-    @staticmethod
-    def forward(ctx, x, weight, bias, act, slope, residual):
-        ctx.save_for_backward(x, weight, bias)
-        ctx.cfg = (act, slope)
-        return ops.linear_act_fwd(x, weight, bias, act, slope, residual)
+    def __init__(self, in_features, out_features, bias=True, activation="none", slope=0.2, **kwargs):
+        super().__init__(in_features, out_features, bias=bias, **kwargs)
+        ops.activation_id(activation)  # refuses unknown names at construction
+        self.activation, self.slope = activation, slope
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx = dw = db = None
-        if need[0] or need[1] or need[2]:
-            dx, dw, db = ops.linear_act_bwd(x, dy, weight, bias, *ctx.cfg, want_input=need[0], want_weight=need[1], want_bias=need[2])
-        return dx, dw, db, None, None, dy if need[5] else None
+    def forward(self, x, residual=None):
+        if not isinstance(x, ME.SparseTensor):
+            return linear_act(x, self.weight, self.bias, self.activation, self.slope, residual)
+        if residual is not None:
+            if residual.coordinate_manager is not x.coordinate_manager or residual.tensor_stride != x.tensor_stride:
+                raise ValueError("LinearAct: the residual must share the coordinate map")
+            residual = residual.feats
+        return x._like(linear_act(x.feats, self.weight, self.bias, self.activation, self.slope, residual))
 
-
-def linear_act(x, weight, bias=None, activation="none", slope=0.2, residual=None):
-    """y = act(x W^T + bias) + residual as one launch, differentiable in all four operands.  x [n, cin], weight [cout, cin] (the
-    layout of torch.nn.Linear), bias [cout] or None, residual [n, cout] or None, all of one type (float32, bfloat16, float16).
-    activation: none, relu, leaky_relu (with `slope`), silu or gelu (exact); it acts before the residual is added, as in ResBlock."""
-    act = ops.activation_id(activation)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        return _LinearActFn.apply(x, weight, bias, act, slope, residual)
-    return ops.linear_act_fwd(x, weight, bias, act, slope, residual)
+    def extra_repr(self):
+        return "%s, activation=%s" % (super().extra_repr(), self.activation)
 
 
 class Linear(nn.Linear):
@@ -195,33 +157,50 @@ def fused_head(head, x, log_softmax=False, want_argmax=False):
 FUSE_SHORTCUT = os.environ.get("PP_FUSE_SHORTCUT", "1") != "0"
 
 
-class ResBlock(ME.MinkowskiNetwork):
-    """conv3-BN-ReLU-conv3-BN-ReLU, plus (1x1 conv-BN of the input | the input); ReLU BEFORE the add, none after."""
+def _norm_relu(channels, norm, num_groups):
+    """the (normalisation, ReLU) pair behind a convolution.  norm "batch": the reference's BatchNorm and ReLU modules; "group": group
+    normalisation with the ReLU fused (statistics per batch element: independent of how many cylinders a batch holds), an Identity
+    in the ReLU's place so that module indices do not depend on the choice"""
+    if norm == "batch":
+        return ME.MinkowskiBatchNorm(channels), ME.MinkowskiReLU()
+    if norm == "group":
+        return ME.MinkowskiGroupNorm(num_groups, channels, activation="relu"), Identity()
+    raise ValueError("norm must be batch or group, got %r" % (norm,))
 
-    def __init__(self, input_nc, output_nc, convolution, dimension=3):
+
+class ResBlock(ME.MinkowskiNetwork):
+    """conv3-BN-ReLU-conv3-BN-ReLU, plus (1x1 conv-BN of the input | the input); ReLU BEFORE the add, none after.
+    norm="group": group normalisation (num_groups groups) in the place of BN."""
+
+    def __init__(self, input_nc, output_nc, convolution, dimension=3, norm="batch", num_groups=8):
         ME.MinkowskiNetwork.__init__(self, dimension)
+        n1, r1 = _norm_relu(output_nc, norm, num_groups)
+        n2, r2 = _norm_relu(output_nc, norm, num_groups)
+        self.norm = norm
         self.block = (
             Seq()
             .append(convolution(in_channels=input_nc, out_channels=output_nc, kernel_size=3, stride=1, dilation=1,
                                 bias=False, dimension=dimension))
-            .append(ME.MinkowskiBatchNorm(output_nc))
-            .append(ME.MinkowskiReLU())
+            .append(n1)
+            .append(r1)
             .append(convolution(in_channels=output_nc, out_channels=output_nc, kernel_size=3, stride=1, dilation=1,
                                 bias=False, dimension=dimension))
-            .append(ME.MinkowskiBatchNorm(output_nc))
-            .append(ME.MinkowskiReLU())
+            .append(n2)
+            .append(r2)
         )
         if input_nc != output_nc:
             self.downsample = (
                 Seq()
                 .append(convolution(in_channels=input_nc, out_channels=output_nc, kernel_size=1, stride=1, dilation=1,
                                     bias=False, dimension=dimension))
-                .append(ME.MinkowskiBatchNorm(output_nc))
+                .append(ME.MinkowskiBatchNorm(output_nc) if norm == "batch" else ME.MinkowskiGroupNorm(num_groups, output_nc))
             )
         else:
             self.downsample = None
 
     def forward(self, x):
+        if self.norm != "batch":  # (group norm has no folded form: convolution, then normalisation and ReLU in one)
+            return self.block(x) + (self.downsample(x) if self.downsample else x)
         if not self.training and not torch.is_grad_enabled():
             b = self.block
             h = ME.conv_bn_act(x, b[0], b[1], relu=True)
@@ -358,26 +337,34 @@ _res_blocks = sys.modules[__name__]
 class ResNetDown(ME.MinkowskiNetwork):
     CONVOLUTION = ME.MinkowskiConvolution
 
-    def __init__(self, down_conv_nn=[], kernel_size=2, dilation=1, dimension=3, stride=2, N=1, block="ResBlock", **kwargs):
+    def __init__(self, down_conv_nn=[], kernel_size=2, dilation=1, dimension=3, stride=2, N=1, block="ResBlock", norm="batch",
+                 num_groups=8, **kwargs):
+        if norm != "batch" and block != "ResBlock":
+            raise ValueError("norm=%r is built for ResBlock, not for %s" % (norm, block))
         block = getattr(_res_blocks, block)
+        more = {} if norm == "batch" else {"norm": norm, "num_groups": num_groups}
         ME.MinkowskiNetwork.__init__(self, dimension)
         conv1_output = down_conv_nn[0] if stride > 1 else down_conv_nn[1]
+        norm_in, relu_in = _norm_relu(conv1_output, norm, num_groups)
+        self.norm = norm
         self.conv_in = (
             Seq()
             .append(self.CONVOLUTION(in_channels=down_conv_nn[0], out_channels=conv1_output, kernel_size=kernel_size,
                                      stride=stride, dilation=dilation, bias=False, dimension=dimension))
-            .append(ME.MinkowskiBatchNorm(conv1_output))
-            .append(ME.MinkowskiReLU())
+            .append(norm_in)
+            .append(relu_in)
         )
         if N > 0:
             self.blocks = Seq()
             for _ in range(N):
-                self.blocks.append(block(conv1_output, down_conv_nn[1], self.CONVOLUTION, dimension=dimension))
+                self.blocks.append(block(conv1_output, down_conv_nn[1], self.CONVOLUTION, dimension=dimension, **more))
                 conv1_output = down_conv_nn[1]
         else:
             self.blocks = None
 
     def _conv_in(self, x, skip=None):
+        if self.norm != "batch":
+            return self.conv_in(x if skip is None else ME.cat(x, skip))
         if not self.training and not torch.is_grad_enabled():
             return ME.conv_bn_act(x, self.conv_in[0], self.conv_in[1], relu=True, skip=skip)
         if skip is not None:

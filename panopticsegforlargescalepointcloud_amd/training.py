@@ -180,6 +180,77 @@ def enable_sync_bn(group=True):
     ops.SYNC_BN_GROUP = group if group else None
 
 
+def matrix_parameters(model):
+    """(matrices, others) of a model's parameters: convolution kernels and weights of linear layers for `Muon`, and the rest --
+    vectors, and matrices with one row or column -- for an optimizer that works on single values."""
+    matrices, others = [], []
+    for p in model.parameters():
+        (matrices if p.dim() >= 2 and min(_matrix_shape(p)) > 1 else others).append(p)
+    return matrices, others
+
+
+def _matrix_shape(p):
+    """a weight as a matrix: kernels [K, Cin, Cout] as [K Cin, Cout], weights of linear layers as they are"""
+    return (p.numel() // p.shape[-1] if p.dim() > 2 else p.shape[0]), p.shape[-1]
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update is orthogonalised: U = g + momentum * m (nesterov) or m, with m <- momentum * m + g, and
+    p <- (1 - lr * weight_decay) p - lr * scale * NS(U) with NS the Newton-Schulz iteration of ops.newton_schulz (all singular values
+    near 1).  scale = 0.2 sqrt(max(m, n)) gives the update the size that Adam's has (0.2 per entry).  For parameters of at least two dimensions (`matrix_parameters`); kernels
+    [K, Cin, Cout] are taken as matrices [K Cin, Cout].  The weights of one shape are orthogonalised in one call.  Momentum is kept in
+    float32.  Usable wherever training.train_step takes an optimizer."""
+
+    def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5):
+        if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0 or ns_steps < 1:
+            raise ValueError("Muon: lr and weight_decay >= 0, momentum in [0, 1), ns_steps >= 1")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=ns_steps))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                raise ValueError("Muon: parameters need at least two dimensions, got shape %s" % (tuple(p.shape),))
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)  # (gives the momentum the parameters' type: put back what was saved)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(saved, [p for g in self.param_groups for p in g["params"]]):
+            if "momentum_buffer" in state_dict["state"].get(i, {}):
+                self.state[p]["momentum_buffer"] = state_dict["state"][i]["momentum_buffer"].to(p.device, torch.float32, copy=True)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            by_shape = {}
+            for p in group["params"]:
+                if p.grad is not None:
+                    if p.grad.is_sparse:
+                        raise RuntimeError("Muon does not take sparse gradients")
+                    by_shape.setdefault((p.device, p.dtype, _matrix_shape(p)), []).append(p)
+            for (_, _, (m, n)), ps in by_shape.items():
+                buffers = []
+                for p in ps:
+                    state = self.state[p]
+                    if "momentum_buffer" not in state:
+                        state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                    buffers.append(state["momentum_buffer"])
+                grads = [p.grad.float() for p in ps]
+                torch._foreach_mul_(buffers, group["momentum"])
+                torch._foreach_add_(buffers, grads)
+                updates = torch._foreach_add(grads, buffers, alpha=group["momentum"]) if group["nesterov"] else buffers
+                out = ops.newton_schulz(torch.stack([u.reshape(m, n) for u in updates]), steps=group["ns_steps"])
+                if group["weight_decay"]:
+                    torch._foreach_mul_(ps, 1.0 - group["lr"] * group["weight_decay"])
+                deltas = [o.view(p.shape).to(p.dtype) for o, p in zip(out, ps)]
+                torch._foreach_add_(ps, deltas, alpha=-group["lr"] * 0.2 * max(m, n) ** 0.5)
+        return loss
+
+
 def train_step(model, data, optimizer, epoch, device, world_size=1, group=None, reducer=None):
     """set_input -> forward -> loss -> backward (gradient all-reduces overlapped) -> optimizer step.  Returns the local
     loss.  Pass a GradientReducer built once over model.parameters() to overlap; without one the reduction runs after
