@@ -30,7 +30,7 @@ struct LinArgs {
   void* out;
   int n_out;             // columns written (LIN_DZ pads its rows with zeros up to here)
   int vo;                // four neighbouring columns may be stored (and `extra` read) at once
-  float *part, *part_bias;   // LIN_PART: [splits][m][n], [splits][m]
+  float *part, *part_bias;   // LIN_PART: [splits][m][n], [splits][m]; LIN_DZ: part_bias[row tile][n]
   int64_t k_per_split;
 };
 
@@ -238,6 +238,7 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
     }
   }
   // lane (l & 15, l >> 4) holds row l & 15 and columns 4 (l >> 4) .. + 3 of every 16 x 16 fragment
+  float zs[FN][4] = {};
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int64_t r = m0 + wm + 16 * i + (lane & 15);
@@ -263,6 +264,10 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
           v[e] = MODE == LIN_FWD ? pp_act1(v[e] + b[e], a.act, a.slope) + x[e]
                                  : (e < valid ? x[e] * pp_dact1(v[e] + b[e], a.act, a.slope) : 0.f);  // (padding is 0, whatever the row holds)
       }
+      if (MODE == LIN_DZ) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) zs[j][e] += v[e];
+      }
       T* const o = (T*)a.out + r * a.ldo + c;
       if (a.vo) {
         if (c < a.n_out) pp_store<T, 4>(o, v);
@@ -270,6 +275,27 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (c + e < a.n_out) o[e] = (T)v[e];
+      }
+    }
+  }
+  if constexpr (MODE == LIN_DZ) {
+    if (a.part_bias) {  // the bias gradient takes dz before its rounding: rows of a fragment, then the waves above each other
+      float* const red = (float*)lds;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = zs[j][e];
+#pragma unroll
+          for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
+          if ((lane & 15) == 0) red[wm / WM * BN + wn + 16 * j + 4 * (lane >> 4) + e] = v;
+        }
+      __syncthreads();
+      if (threadIdx.x < BN && n0 + (int)threadIdx.x < a.n) {
+        float v = 0.f;
+        for (int q = 0; q < BM / WM; ++q) v += red[q * BN + threadIdx.x];
+        a.part_bias[(int64_t)blockIdx.x * a.n + n0 + threadIdx.x] = v;
       }
     }
   }
@@ -296,19 +322,23 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
   }
 }
 
-// adds the parts of the weight and bias gradient in their order
+// out[i] = sum of part[q][i] over the q of this group (blockIdx.y of gridDim.y), S slices of a block's threads over q, added in order
 template <typename T>
-__global__ __launch_bounds__(256) void k_linear_parts(const float* __restrict__ part, const float* __restrict__ part_bias, int splits,
-                                                      int64_t nw, int64_t nb, T* __restrict__ dw, T* __restrict__ db) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < nw) {
-    double s = 0.0;
-    for (int q = 0; q < splits; ++q) s += (double)part[q * nw + i];
-    dw[i] = (T)(float)s;
-  } else if (i < nw + nb) {
-    double s = 0.0;
-    for (int q = 0; q < splits; ++q) s += (double)part_bias[q * nb + (i - nw)];
-    db[i - nw] = (T)(float)s;
+__global__ __launch_bounds__(256) void k_linear_sum(const float* __restrict__ part, int64_t parts, int64_t n, int S, T* __restrict__ out) {
+  __shared__ double red[256];
+  const int cols = 256 / S, cl = threadIdx.x % cols, sl = threadIdx.x / cols;
+  const int64_t i = (int64_t)blockIdx.x * cols + cl;
+  const int64_t per = (parts + gridDim.y - 1) / gridDim.y, q0 = blockIdx.y * per, q1 = q0 + per < parts ? q0 + per : parts;
+  double s = 0.0;
+  if (i < n) {
+#pragma unroll 4
+    for (int64_t q = q0 + sl; q < q1; q += S) s += (double)part[q * n + i];
+  }
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (sl == 0 && i < n) {
+    for (int k = 1; k < S; ++k) s += red[k * cols + cl];
+    out[(int64_t)blockIdx.y * n + i] = (T)(float)s;
   }
 }
 
@@ -337,13 +367,33 @@ static int lin_splits(int64_t n, int cin, int cout) {
   if (s > (n + 255) / 256) s = (n + 255) / 256;
   return s < 1 ? 1 : (int)s;
 }
+#define LIN_SUM_GROUPS 32
 static int64_t lin_ldz(int cout) { return (cout + 7) / 8 * 8; }
+
+static int64_t lin_bias_parts(int64_t n, int splits, int act) { return act == PP_ACT_NONE ? splits : (n + 127) / 128; }
 
 extern "C" size_t pp_linear_act_bwd_workspace(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_t act) {
   if (n < 0 || cin < 1 || cout < 1) return 0;
   const size_t parts = (size_t)lin_splits(n, cin, cout);
-  return pp_align(parts * cout * cin * 4) + pp_align(parts * cout * 4) +
+  return pp_align(parts * cout * cin * 4) + pp_align((size_t)(lin_bias_parts(n, (int)parts, act) + LIN_SUM_GROUPS) * cout * 4) +
          (act == PP_ACT_NONE ? 0 : pp_align((size_t)n * lin_ldz(cout) * pp_dtype_bytes(dtype))) + 256;
+}
+
+// sums of `parts` rows of n values; more than a few hundred rows go through LIN_SUM_GROUPS partial rows behind them
+template <typename T>
+static int lin_sum(float* part, int64_t parts, int64_t n, T* out, hipStream_t s) {
+  if (parts > 512) {
+    float* const mid = part + parts * n;
+    hipLaunchKernelGGL((k_linear_sum<float>), dim3((unsigned)((n + 15) / 16), LIN_SUM_GROUPS), dim3(256), 0, s, part, parts, n, 16, mid);
+    part = mid;
+    parts = LIN_SUM_GROUPS;
+  }
+  int S = 1;
+  while (S < 16 && S < parts) S *= 2;
+  const int64_t cols = 256 / S;
+  hipLaunchKernelGGL((k_linear_sum<T>), dim3((unsigned)((n + cols - 1) / cols), 1), dim3(256), 0, s, part, parts, n, S, out);
+  PP_LAUNCH_CHECK();
+  return PP_OK;
 }
 
 static int lin_check(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_t act) {
@@ -376,8 +426,10 @@ template <typename T>
 static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const void* w, int cout, const void* bias, int act, float slope,
                         void* dx, void* dw, void* db, PPArena& ws, hipStream_t s) {
   const int splits = lin_splits(n, cin, cout);
+  const int64_t bias_parts = lin_bias_parts(n, splits, act);
   float* part = ws.take<float>((size_t)splits * cout * cin);
-  float* part_bias = ws.take<float>((size_t)splits * cout);
+  float* part_bias = ws.take<float>((size_t)(bias_parts + LIN_SUM_GROUPS) * cout);
+  PP_REQUIRE(part && part_bias, "pp_linear_act_bwd: workspace layout");
   const T* dz = (const T*)dy;
   int64_t ldz = cout;
   int rc;
@@ -390,10 +442,10 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
       LinArgs a = lin_base<T>(x, n, cin, w, cout, bias, act, slope);
       a.extra = dy; a.out = z; a.ldo = ldz; a.n_out = (int)ldz;
       a.vo = cout % 4 == 0 && lin_aligned(dy, cout, 4 * sizeof(T), sizeof(T));
+      a.part_bias = db ? part_bias : nullptr;
       if ((rc = lin_tile<T, false, false, LIN_DZ>(a, 1, s)) != PP_OK) return rc;
     }
   }
-  PP_REQUIRE(part && part_bias, "pp_linear_act_bwd: workspace layout");
   if (dx && n) {
     LinArgs a{};
     a.a = dz; a.lda = ldz; a.b = w; a.ldb = cin; a.m = n; a.n = cin; a.k = cout; a.out = dx; a.ldo = cin; a.n_out = cin;
@@ -401,19 +453,16 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
     a.vo = cin % 4 == 0 && lin_aligned(dx, cin, 4 * sizeof(T), sizeof(T));
     if ((rc = lin_tile<T, false, true, LIN_STORE>(a, 1, s)) != PP_OK) return rc;
   }
-  if (dw || db) {
+  if (dw || (db && act == PP_ACT_NONE)) {
     LinArgs a{};
     a.a = dz; a.lda = ldz; a.b = x; a.ldb = cin; a.m = cout; a.n = cin; a.k = n;
     a.va = lin_aligned(dz, ldz, 8, sizeof(T)); a.vb = lin_aligned(x, cin, 8, sizeof(T));
-    a.part = part; a.part_bias = part_bias;
+    a.part = part; a.part_bias = db && act == PP_ACT_NONE ? part_bias : nullptr;
     a.k_per_split = ((n + splits - 1) / splits + 63) / 64 * 64;
     if ((rc = lin_tile<T, true, true, LIN_PART>(a, splits, s)) != PP_OK) return rc;
-    const int64_t nw = dw ? (int64_t)cout * cin : 0, nb = db ? cout : 0;
-    hipLaunchKernelGGL((k_linear_parts<T>), dim3((unsigned)((nw + nb + 255) / 256)), dim3(256), 0, s, part, part_bias, splits, nw, nb,
-                       (T*)dw, (T*)db);
-    PP_LAUNCH_CHECK();
+    if (dw && (rc = lin_sum<T>(part, splits, (int64_t)cout * cin, (T*)dw, s)) != PP_OK) return rc;
   }
-  return PP_OK;
+  return db ? lin_sum<T>(part_bias, bias_parts, cout, (T*)db, s) : PP_OK;
 }
 
 extern "C" int pp_linear_act_fwd(const void* x, int32_t dtype, int64_t n, int32_t cin, const void* weight, int32_t cout, const void* bias,

@@ -36,13 +36,37 @@ __device__ __forceinline__ void pp_store(T* __restrict__ p, const float (&v)[VEC
   }
 }
 
+// exp(x): the hardware's exp2 on x log2(e); the rounding of that product costs |x| 2^-24 of the result, and a result below 2^-126 is 0
+__device__ __forceinline__ float pp_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2.  With t = min(|z|, 6): Phi(-t) = 2^-q(t), q of degree 9 fitted (least squares, reweighted towards
+// the smallest largest error of Phi) to -log2 Phi(-t) on [0, 6].  |error| <= 1.5 2^-24 everywhere, 2.5e-5 of the value in the
+// negative tail (where 1 + erf loses all of its bits); 17 instructions, without the two branches of erff that both run in a wave
+// whose values differ -- group norm with gelu over 2.5 M rows of 96 channels, bf16: 350 us a pass with erff, see pp_groupnorm.hip
+__device__ __forceinline__ float pp_phi(float z) {
+  const float t = fminf(fabsf(z), 6.f);
+  float q = -1.524596626722996e-07f;
+  q = fmaf(q, t, 3.834877588815289e-06f);
+  q = fmaf(q, t, -3.800627018790692e-05f);
+  q = fmaf(q, t, 0.00015954984701238573f);
+  q = fmaf(q, t, 0.00022161900415085256f);
+  q = fmaf(q, t, -0.007183804642409086f);
+  q = fmaf(q, t, 0.0525796078145504f);
+  q = fmaf(q, t, 0.4591817855834961f);
+  q = fmaf(q, t, 1.1511082649230957f);
+  q = fmaf(q, t, 0.9999999403953552f);
+  const float e = __builtin_amdgcn_exp2f(-q);
+  return z > 0.f ? 1.f - e : (z <= 0.f ? e : z);  // (NaN stays NaN)
+}
+__device__ __forceinline__ float pp_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + pp_exp(-z)); }
+
 // y = act(z).  `act` is uniform over a launch: the branch costs one scalar compare per vector of elements
 __device__ __forceinline__ float pp_act1(float z, int act, float slope) {
   switch (act) {
     case PP_ACT_RELU: return z < 0.f ? 0.f : z;  // (NaN stays NaN)
     case PP_ACT_LEAKY: return z > 0.f ? z : slope * z;
-    case PP_ACT_SILU: return z / (1.f + expf(-z));
-    case PP_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case PP_ACT_SILU: return z * pp_sigmoid(z);
+    case PP_ACT_GELU: return z * pp_phi(z);
     default: return z;
   }
 }
@@ -52,11 +76,10 @@ __device__ __forceinline__ float pp_dact1(float z, int act, float slope) {
     case PP_ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case PP_ACT_LEAKY: return z > 0.f ? 1.f : slope;
     case PP_ACT_SILU: {
-      const float s = 1.f / (1.f + expf(-z));
-      return s * (1.f + z * (1.f - s));
+      const float s = pp_sigmoid(z);
+      return s * fmaf(z, 1.f - s, 1.f);
     }
-    case PP_ACT_GELU:
-      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    case PP_ACT_GELU: return fmaf(z * 0.39894228040143268f, pp_exp(-0.5f * z * z), pp_phi(z));
     default: return 1.f;
   }
 }
