@@ -10,7 +10,7 @@
 // Nothing is kept for the backward pass but x: z is recomputed from it (the layers are bound by memory, a stored z would cost a write
 // and a read of its own, and its rounding would enter the gradients).  dz is rounded to the element type once, as the matrix
 // instructions take it.  The weight gradient's rows are cut into parts, whose sums are added in a fixed order: results repeat.
-#include "pp_rows.h"
+#include "pp_gemm.h"
 
 typedef unsigned lin_u32x4 __attribute__((ext_vector_type(4)));
 typedef float lin_f32x4 __attribute__((ext_vector_type(4)));
@@ -30,7 +30,7 @@ struct LinArgs {
   void* out;
   int n_out;             // columns written (LIN_DZ pads its rows with zeros up to here)
   int vo;                // four neighbouring columns may be stored (and `extra` read) at once
-  float *part, *part_bias;   // LIN_PART: [splits][m][n], [splits][m]; LIN_DZ: part_bias[row tile][n]
+  float *part, *part_bias;   // LIN_PART: part[splits][m][n]; LIN_DZ: part_bias[row tile][n] (nullable)
   int64_t k_per_split;
 };
 
@@ -150,17 +150,6 @@ struct LinStage {
       }
     }
   }
-  // strided only: adds the staged values to the sums of the unit's columns
-  __device__ __forceinline__ void add_columns(float (&s)[PER][COLS]) const {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (UNITS % 256 != 0 && threadIdx.x + 256 * i >= UNITS) continue;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int j = 0; j < COLS; ++j) s[i][j] += (float)v[i][e * COLS + j];
-    }
-  }
 };
 
 template <typename T, int ROWS>
@@ -182,6 +171,76 @@ __device__ __forceinline__ void lin_load4(const T* __restrict__ p, int valid, bo
     for (int i = 0; i < 4; ++i) v[i] = i < valid ? (float)p[i] : 0.f;
   }
 }
+
+// What becomes of four neighbouring columns c .. c + 3 of row r of a product.  j: the lane's column fragment (of FN)
+template <typename T, int MODE, int FN>
+struct LinEpilogue {
+  static constexpr bool COLUMN_SUMS = MODE == LIN_DZ;
+  LinArgs a;
+  int split;
+  float zs[COLUMN_SUMS ? FN : 1][4];  // sums of dz over the lane's rows, before its rounding: the bias gradient's
+
+  __device__ __forceinline__ void block(int64_t, int64_t, int split_, int64_t) {
+    split = split_;
+#pragma unroll
+    for (int j = 0; j < (COLUMN_SUMS ? FN : 1); ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) zs[j][e] = 0.f;
+  }
+  __device__ __forceinline__ void put(int64_t r, int64_t c, int j, float (&v)[4]) {
+    const int valid = (int)(a.n - c < 4 ? a.n - c : 4);
+    if (MODE == LIN_PART) {
+      float* const o = a.part + ((int64_t)split * a.m + r) * a.n + c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < valid) o[e] = v[e];
+      return;
+    }
+    if (MODE == LIN_FWD || MODE == LIN_DZ) {
+      float b[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f};
+      if (a.bias) lin_load4((const T*)a.bias + c, valid, false, b);
+      if (a.extra) lin_load4((const T*)a.extra + r * a.n + c, valid, a.vo, x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] = MODE == LIN_FWD ? pp_act1(v[e] + b[e], a.act, a.slope) + x[e]
+                               : (e < valid ? x[e] * pp_dact1(v[e] + b[e], a.act, a.slope) : 0.f);  // (padding is 0, whatever the row holds)
+    }
+    if (MODE == LIN_DZ) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) zs[j][e] += v[e];
+    }
+    T* const o = (T*)a.out + r * a.ldo + c;
+    if (a.vo) {
+      if (c < a.n_out) pp_store<T, 4>(o, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < a.n_out) o[e] = (T)v[e];
+    }
+  }
+  // column sums of a BM x BN tile: the rows of a fragment, then the waves above each other.  red: LDS that nobody reads any more
+  template <int BM, int BN, int WM, int WN>
+  __device__ __forceinline__ void done(float* red, int wm, int wn, int64_t n0, int64_t row_tile) {
+    if (!a.part_bias) return;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = zs[j][e];
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
+        if ((lane & 15) == 0) red[wm / WM * BN + wn + 16 * j + 4 * (lane >> 4) + e] = v;
+      }
+    __syncthreads();
+    for (int t = threadIdx.x; t < BN; t += blockDim.x)
+      if (n0 + t < a.n) {
+        float v = 0.f;
+        for (int q = 0; q < BM / WM; ++q) v += red[q * BN + t];
+        a.part_bias[row_tile * a.n + n0 + t] = v;
+      }
+  }
+};
 
 // BM x BN tile, four waves of WM x WN each.  AS / BS: the contraction runs down the columns of A / B
 template <typename T, bool AS, bool BS, int MODE, int BM, int BN, int WM, int WN>
@@ -206,8 +265,6 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
     for (int j = 0; j < FN; ++j) acc[i][j] = (lin_f32x4){0.f, 0.f, 0.f, 0.f};
   LinStage<T, AS, BM> sa;
   LinStage<T, BS, BN> sb;
-  float cols[LinStage<T, AS, BM>::PER][LinStage<T, AS, BM>::COLS] = {};
-  const bool want_bias = MODE == LIN_PART && blockIdx.y == 0 && a.part_bias;
   if (k < k1) {
     sa.load(pa, a.lda, m0, a.m, k, k1, a.va);
     sb.load(pb, a.ldb, n0, a.n, k, k1, a.vb);
@@ -217,7 +274,6 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
     if (BUFS == 1) __syncthreads();  // the last step's fragments have been read
     sa.put(at);
     sb.put(at + PLANES * BM * CH);
-    if (AS && want_bias) sa.add_columns(cols);
     __syncthreads();
     if (k + BK < k1) {
       sa.load(pa, a.lda, m0, a.m, k + BK, k1, a.va);
@@ -238,87 +294,21 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
     }
   }
   // lane (l & 15, l >> 4) holds row l & 15 and columns 4 (l >> 4) .. + 3 of every 16 x 16 fragment
-  float zs[FN][4] = {};
+  LinEpilogue<T, MODE, FN> epi;
+  epi.a = a;
+  epi.block(m0, n0, blockIdx.z, 0);
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int64_t r = m0 + wm + 16 * i + (lane & 15);
-    if (r >= a.m) continue;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      const int c = n0 + wn + 16 * j + 4 * (lane >> 4);
       float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      if (MODE == LIN_PART) {
-        float* const o = a.part + ((int64_t)blockIdx.z * a.m + r) * a.n + c;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e < a.n) o[e] = v[e];
-        continue;
-      }
-      const int valid = a.n - c;
-      if (MODE == LIN_FWD || MODE == LIN_DZ) {
-        float b[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f};
-        if (a.bias) lin_load4((const T*)a.bias + c, valid, false, b);
-        if (a.extra) lin_load4((const T*)a.extra + r * a.n + c, valid, a.vo, x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = MODE == LIN_FWD ? pp_act1(v[e] + b[e], a.act, a.slope) + x[e]
-                                 : (e < valid ? x[e] * pp_dact1(v[e] + b[e], a.act, a.slope) : 0.f);  // (padding is 0, whatever the row holds)
-      }
-      if (MODE == LIN_DZ) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) zs[j][e] += v[e];
-      }
-      T* const o = (T*)a.out + r * a.ldo + c;
-      if (a.vo) {
-        if (c < a.n_out) pp_store<T, 4>(o, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e < a.n_out) o[e] = (T)v[e];
-      }
+      if (r < a.m) epi.put(r, n0 + wn + 16 * j + 4 * (lane >> 4), j, v);
     }
   }
   if constexpr (MODE == LIN_DZ) {
-    if (a.part_bias) {  // the bias gradient takes dz before its rounding: rows of a fragment, then the waves above each other
-      float* const red = (float*)lds;
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = zs[j][e];
-#pragma unroll
-          for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
-          if ((lane & 15) == 0) red[wm / WM * BN + wn + 16 * j + 4 * (lane >> 4) + e] = v;
-        }
-      __syncthreads();
-      if (threadIdx.x < BN && n0 + (int)threadIdx.x < a.n) {
-        float v = 0.f;
-        for (int q = 0; q < BM / WM; ++q) v += red[q * BN + threadIdx.x];
-        a.part_bias[(int64_t)blockIdx.x * a.n + n0 + threadIdx.x] = v;
-      }
-    }
-  }
-  if constexpr (MODE == LIN_PART && AS) {
-    if (want_bias) {  // the columns' sums of the threads that staged other parts of the contraction, in their order
-      typedef LinStage<T, AS, BM> S;
-      constexpr int QUADS = BM / S::COLS;
-      float* const red = (float*)lds;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < S::PER; ++i)
-#pragma unroll
-        for (int j = 0; j < S::COLS; ++j) {
-          const int unit = threadIdx.x + 256 * i;
-          if (unit < S::UNITS) red[unit / QUADS * BM + (unit % QUADS) * S::COLS + j] = cols[i][j];
-        }
-      __syncthreads();
-      if (threadIdx.x < BM && m0 + threadIdx.x < a.m) {
-        float s = 0.f;
-        for (int q = 0; q < CH; ++q) s += red[q * BM + threadIdx.x];
-        a.part_bias[(int64_t)blockIdx.z * a.m + m0 + threadIdx.x] = s;
-      }
-    }
+    __syncthreads();
+    epi.template done<BM, BN, WM, WN>((float*)lds, wm, wn, n0, blockIdx.x);
   }
 }
 
@@ -342,6 +332,22 @@ __global__ __launch_bounds__(256) void k_linear_sum(const float* __restrict__ pa
   }
 }
 
+// column sums of a part of the rows of [n, c]: part[blockIdx.y][c]; 64 columns a block, four rows side by side
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_columns(const T* __restrict__ x, int64_t n, int c, int64_t rows_per_part, float* __restrict__ part) {
+  __shared__ float red[256];
+  const int col = blockIdx.x * 64 + (threadIdx.x & 63), rl = threadIdx.x >> 6;
+  const int64_t r0 = blockIdx.y * rows_per_part, r1 = r0 + rows_per_part < n ? r0 + rows_per_part : n;
+  float s = 0.f;
+  if (col < c) {
+#pragma unroll 8
+    for (int64_t r = r0 + rl; r < r1; r += 4) s += (float)x[r * c + col];
+  }
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (rl == 0 && col < c) part[(int64_t)blockIdx.y * c + col] = red[threadIdx.x] + red[threadIdx.x + 64] + red[threadIdx.x + 128] + red[threadIdx.x + 192];
+}
+
 // ---- launches ---------------------------------------------------------------------------------------------------------------------
 template <typename T, bool AS, bool BS, int MODE, int BM, int BN, int WM, int WN>
 static int lin_go(const LinArgs& a, int splits, hipStream_t s) {
@@ -352,30 +358,69 @@ static int lin_go(const LinArgs& a, int splits, hipStream_t s) {
   PP_LAUNCH_CHECK();
   return PP_OK;
 }
+static bool lin_aligned(const void* p, int64_t ld, int bytes, size_t size) { return (uintptr_t)p % bytes == 0 && (ld * size) % bytes == 0; }
+
+// The wide kernel (pp_gemm.h) serves 16-bit operands whose rows start on 16 bytes, where the matrix pipe bounds: from 192 columns and
+// 128 of the contraction on (narrower results spend their time on reading A once, which the tile kernel above does as well)
+#define LIN_WIDE_COLUMNS 192
+template <typename T, bool AS, bool BS, int MODE>
+static bool lin_wide(const LinArgs& a) {
+  if (sizeof(T) != 2) return false;
+  return a.n >= LIN_WIDE_COLUMNS && a.k >= 128 && a.m >= 128 && lin_aligned(a.a, a.lda, 16, 2) && lin_aligned(a.b, a.ldb, 16, 2) && a.n_out == a.n;
+}
+static int64_t lin_tiles(int64_t m, int64_t n, int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); }
+
+template <typename T, bool AS, bool BS, int MODE, int BM, int BN, int WM, int WN>
+static int lin_go_wide(const LinArgs& a, int splits, hipStream_t s) {
+  LinEpilogue<T, MODE, WN / 16> e{};
+  e.a = a;
+  GemmArgs g{};
+  g.a[0] = a.a; g.b[0] = a.b; g.segments = 1; g.m = a.m; g.n = a.n; g.k = a.k; g.lda = a.lda; g.ldb = a.ldb;
+  g.splits = splits; g.k_per_split = splits > 1 ? a.k_per_split : (a.k + GM_BK - 1) / GM_BK * GM_BK;
+  const int64_t tiles = ((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN);
+  PP_REQUIRE(tiles <= 0x7FFFFFFF && splits <= 65535, "pp_linear_act: too many tiles");
+  hipLaunchKernelGGL((k_gemm<T, AS, BS, BM, BN, WM, WN, LinEpilogue<T, MODE, WN / 16>>), dim3((unsigned)tiles, splits, 1),
+                     dim3(BM / WM * (BN / WN) * 64), 0, s, g, e);
+  PP_LAUNCH_CHECK();
+  return PP_OK;
+}
+
+// rows of a workgroup's tile: large tiles where they fill the chip (256 x 256 tiles of half the chip's units, parts counted)
+template <typename T, bool AS, bool BS, int MODE>
+static int lin_tile_rows(const LinArgs& a, int splits) {
+  return lin_wide<T, AS, BS, MODE>(a) && lin_tiles(a.m, a.n, 256) * splits >= 128 ? 256 : 128;
+}
 template <typename T, bool AS, bool BS, int MODE>
 static int lin_tile(const LinArgs& a, int splits, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (lin_wide<T, AS, BS, MODE>(a)) {
+      if (lin_tile_rows<T, AS, BS, MODE>(a, splits) == 256) return lin_go_wide<T, AS, BS, MODE, 256, 256, 128, 64>(a, splits, s);
+      return lin_go_wide<T, AS, BS, MODE, 128, 128, 64, 64>(a, splits, s);
+    }
+  }
   if (a.n > 64) return lin_go<T, AS, BS, MODE, 128, 128, 64, 64>(a, splits, s);
   return lin_go<T, AS, BS, MODE, 128, 64, 32, 64>(a, splits, s);
 }
 
-static bool lin_aligned(const void* p, int64_t ld, int bytes, size_t size) { return (uintptr_t)p % bytes == 0 && (ld * size) % bytes == 0; }
 
-// parts of the weight gradient's contraction: about two workgroups per compute unit in all, at least 256 rows each
-static int lin_splits(int64_t n, int cin, int cout) {
-  const int64_t tiles = (int64_t)((cout + 127) / 128) * ((cin + (cin > 64 ? 127 : 63)) / (cin > 64 ? 128 : 64));
-  int64_t s = 512 / tiles;
-  if (s > (n + 255) / 256) s = (n + 255) / 256;
+// parts of the weight gradient's contraction: about two workgroups of the tile kernel per compute unit (one of the wide kernel's), at
+// least 256 (512) rows each
+static int lin_splits(int64_t n, int cin, int cout, bool wide) {
+  const int64_t tiles = wide ? lin_tiles(cout, cin, 256) : (int64_t)((cout + 127) / 128) * ((cin + (cin > 64 ? 127 : 63)) / (cin > 64 ? 128 : 64));
+  const int64_t rows = wide ? 512 : 256;
+  int64_t s = (wide ? 256 : 512) / tiles;
+  if (s > (n + rows - 1) / rows) s = (n + rows - 1) / rows;
   return s < 1 ? 1 : (int)s;
 }
 #define LIN_SUM_GROUPS 32
+#define LIN_COLUMN_PARTS 64
 static int64_t lin_ldz(int cout) { return (cout + 7) / 8 * 8; }
-
-static int64_t lin_bias_parts(int64_t n, int splits, int act) { return act == PP_ACT_NONE ? splits : (n + 127) / 128; }
 
 extern "C" size_t pp_linear_act_bwd_workspace(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_t act) {
   if (n < 0 || cin < 1 || cout < 1) return 0;
-  const size_t parts = (size_t)lin_splits(n, cin, cout);
-  return pp_align(parts * cout * cin * 4) + pp_align((size_t)(lin_bias_parts(n, (int)parts, act) + LIN_SUM_GROUPS) * cout * 4) +
+  const size_t p0 = (size_t)lin_splits(n, cin, cout, false), p1 = (size_t)lin_splits(n, cin, cout, true), parts = p0 > p1 ? p0 : p1;
+  const size_t bias = act == PP_ACT_NONE ? LIN_COLUMN_PARTS : (size_t)((n + 127) / 128) + LIN_SUM_GROUPS;
+  return pp_align(parts * cout * cin * 4) + pp_align(bias * cout * 4) +
          (act == PP_ACT_NONE ? 0 : pp_align((size_t)n * lin_ldz(cout) * pp_dtype_bytes(dtype))) + 256;
 }
 
@@ -425,13 +470,12 @@ static int lin_forward(const void* x, int64_t n, int cin, const void* w, int cou
 template <typename T>
 static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const void* w, int cout, const void* bias, int act, float slope,
                         void* dx, void* dw, void* db, PPArena& ws, hipStream_t s) {
-  const int splits = lin_splits(n, cin, cout);
-  const int64_t bias_parts = lin_bias_parts(n, splits, act);
-  float* part = ws.take<float>((size_t)splits * cout * cin);
-  float* part_bias = ws.take<float>((size_t)(bias_parts + LIN_SUM_GROUPS) * cout);
+  const int p0 = lin_splits(n, cin, cout, false), p1 = lin_splits(n, cin, cout, true);
+  float* part = ws.take<float>((size_t)(p0 > p1 ? p0 : p1) * cout * cin);
+  float* part_bias = ws.take<float>((act == PP_ACT_NONE ? LIN_COLUMN_PARTS : (size_t)((n + 127) / 128) + LIN_SUM_GROUPS) * cout);
   PP_REQUIRE(part && part_bias, "pp_linear_act_bwd: workspace layout");
   const T* dz = (const T*)dy;
-  int64_t ldz = cout;
+  int64_t ldz = cout, bias_parts = 0;
   int rc;
   if (act != PP_ACT_NONE) {
     ldz = lin_ldz(cout);
@@ -443,8 +487,15 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
       a.extra = dy; a.out = z; a.ldo = ldz; a.n_out = (int)ldz;
       a.vo = cout % 4 == 0 && lin_aligned(dy, cout, 4 * sizeof(T), sizeof(T));
       a.part_bias = db ? part_bias : nullptr;
+      const int rows = lin_tile_rows<T, false, false, LIN_DZ>(a, 1);
+      bias_parts = (n + rows - 1) / rows;
       if ((rc = lin_tile<T, false, false, LIN_DZ>(a, 1, s)) != PP_OK) return rc;
     }
+  } else if (db && n) {
+    bias_parts = n < 16 * LIN_COLUMN_PARTS ? 1 : LIN_COLUMN_PARTS;
+    hipLaunchKernelGGL((k_linear_columns<T>), dim3((unsigned)((cout + 63) / 64), (unsigned)bias_parts), dim3(256), 0, s, (const T*)dy, n, cout,
+                       (n + bias_parts - 1) / bias_parts, part_bias);
+    PP_LAUNCH_CHECK();
   }
   if (dx && n) {
     LinArgs a{};
@@ -453,14 +504,15 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
     a.vo = cin % 4 == 0 && lin_aligned(dx, cin, 4 * sizeof(T), sizeof(T));
     if ((rc = lin_tile<T, false, true, LIN_STORE>(a, 1, s)) != PP_OK) return rc;
   }
-  if (dw || (db && act == PP_ACT_NONE)) {
+  if (dw) {
     LinArgs a{};
     a.a = dz; a.lda = ldz; a.b = x; a.ldb = cin; a.m = cout; a.n = cin; a.k = n;
     a.va = lin_aligned(dz, ldz, 8, sizeof(T)); a.vb = lin_aligned(x, cin, 8, sizeof(T));
-    a.part = part; a.part_bias = db && act == PP_ACT_NONE ? part_bias : nullptr;
+    a.part = part; a.n_out = cin;
+    const int splits = lin_wide<T, true, true, LIN_PART>(a) ? p1 : p0;
     a.k_per_split = ((n + splits - 1) / splits + 63) / 64 * 64;
     if ((rc = lin_tile<T, true, true, LIN_PART>(a, splits, s)) != PP_OK) return rc;
-    if (dw && (rc = lin_sum<T>(part, splits, (int64_t)cout * cin, (T*)dw, s)) != PP_OK) return rc;
+    if ((rc = lin_sum<T>(part, splits, (int64_t)cout * cin, (T*)dw, s)) != PP_OK) return rc;
   }
   return db ? lin_sum<T>(part_bias, bias_parts, cout, (T*)db, s) : PP_OK;
 }

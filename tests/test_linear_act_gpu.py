@@ -77,6 +77,7 @@ def test_types_and_activations(dtype, kind):
 @pytest.mark.parametrize("n,cin,cout", [
     (0, 16, 16), (1, 1, 1), (1, 64, 64), (2, 7, 3), (64, 112, 7), (64, 7, 112), (127, 33, 65), (129, 128, 129), (1000, 4, 16),
     (513, 75, 133), (260, 1024, 20), (90, 20, 1030), (300, 130, 64), (4097, 16, 5), (20_001, 64, 32), (9000, 36, 200), (33, 2050, 17),
+    (700, 200, 392), (1030, 512, 264), (16_500, 128, 512),
 ])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_shapes(n, cin, cout, dtype):
@@ -84,7 +85,8 @@ def test_shapes(n, cin, cout, dtype):
 
 
 @pytest.mark.parametrize("n,cin,cout", [(1, 5, 9), (131, 64, 64), (300, 75, 133), (640, 192, 96), (1025, 40, 260), (5000, 16, 24),
-                                        (12_000, 130, 70)])
+                                        (12_000, 130, 70), (700, 200, 392), (1030, 512, 264), (16_500, 128, 512), (70_000, 256, 512),
+                                        (520, 264, 1160)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_whole_numbers_are_exact(n, cin, cout, dtype):
     g = torch.Generator().manual_seed(n)
