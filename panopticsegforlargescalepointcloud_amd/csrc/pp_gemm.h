@@ -104,14 +104,51 @@ struct GemmStage {
   }
 };
 
-// Epi: init(...) is the caller's; block(ti, tj, split, batch) is called once, put(row, column, v) for every lane's four neighbouring
-// columns of a row (row < m; columns may pass n), done(lds) at the end by all threads
+// A wave's WM x 64 results to memory.  A lane holds row l & 15 and columns 4 (l >> 4) .. + 3 of every 16 x 16 fragment; through ROWS
+// rows of the wave's own LDS (256 bytes a row, 16-byte chunk c of row r in slot c ^ (r & 15): no bank conflicts either way) it gets
+// eight neighbouring columns instead, eight lanes a row: whole lines to memory, and one short loop of epilogue code.  (Working on
+// the fragments where they lie, the unrolled epilogue was 100 KB of code that ran once a tile, and took as long as the products:
+// 8192 x 1024 -> 4096 with silu 104 us, of which 83 us without the loads of the loop.)
+// Epi: block(first of the lane's columns, split, batch) once; load(row, Row&) asks for what a row's epilogue reads, put(row, Row, v)
+// finishes it (rows may pass the end: both check)
+template <int FM, int FN, int ROWS, typename Epi>
+__device__ __forceinline__ void gm_epilogue(Epi& epi, const gm_f32x4 (&acc)[FM][FN], float* __restrict__ lds, int64_t row0, int64_t col0, int split,
+                                            int64_t batch) {
+  static_assert(FN == 4 && ROWS % 16 == 0 && FM * 16 % ROWS == 0, "a wave's columns are 64");
+  const int lane = threadIdx.x & 63;
+  epi.block(col0 + 8 * (lane & 7), split, batch);
+#pragma unroll
+  for (int p = 0; p < FM * 16 / ROWS; ++p) {
+#pragma unroll
+    for (int i = 0; i < ROWS / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        *(gm_f32x4*)(lds + (16 * i + (lane & 15)) * 64 + ((4 * j + (lane >> 4)) ^ (lane & 15)) * 4) = acc[p * (ROWS / 16) + i][j];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+    for (int t = 0; t < ROWS / 8; ++t) {
+      const int lr = 8 * t + (lane >> 3);
+      const int64_t r = row0 + p * ROWS + lr;
+      typename Epi::Row row;
+      epi.load(r, row);
+      const gm_f32x4 lo = *(const gm_f32x4*)(lds + lr * 64 + ((2 * (lane & 7)) ^ (lr & 15)) * 4);
+      const gm_f32x4 hi = *(const gm_f32x4*)(lds + lr * 64 + ((2 * (lane & 7) + 1) ^ (lr & 15)) * 4);
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      epi.put(r, row, v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 template <typename T, bool AC, bool BC, int BM, int BN, int WM, int WN, typename Epi>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, BM * BN > 128 * 128 ? 1 : 2) void k_gemm(GemmArgs g, Epi epi) {
   constexpr int WAVES = BM / WM * (BN / WN), FM = WM / 16, FN = WN / 16;
   constexpr int A_BYTES = BM * GM_BK * 2, STAGE = (BM + BN) * GM_BK * 2;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  static_assert((STAGE & (STAGE - 1)) == 0, "the stages alternate by a bit of the address");
+  __shared__ __attribute__((aligned(2 * STAGE))) char lds[2 * STAGE];
+  const int wave = threadIdx.x >> 6;
   const int64_t tm = (g.m + BM - 1) / BM, tn = (g.n + BN - 1) / BN;
   // neighbouring tiles on one XCD's cache: every XCD gets a contiguous range of tiles, walked in bands of eight tile rows
   const unsigned t = pp_xcd_remap(blockIdx.x, gridDim.x);
@@ -135,13 +172,25 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, BM * BN > 128 * 128 ? 1 :
   sa.init(m0, g.m, g.lda);
   sb.init(n0, g.n, g.ldb);
   const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-  const int64_t oa = batch * g.a_batch + (AC ? m0 : m0 * g.lda), ob = batch * g.b_batch + (BC ? n0 : n0 * g.ldb);
-  auto fetch = [&](int64_t s) {
-    const int q = (int)(s / steps);
-    const int64_t k = k0 + (s - q * steps) * GM_BK;
-    const unsigned at = base + (unsigned)(s & 1) * STAGE;
-    sa.fetch((const T*)g.a[q] + oa + (AC ? k * g.lda : k), k1 - k, at);
-    sb.fetch((const T*)g.b[q] + ob + (BC ? k * g.ldb : k), k1 - k, at + A_BYTES);
+  // the corner of the next step to be fetched, what is left of its segment, and the stage it goes to
+  const int64_t oa = batch * g.a_batch + (AC ? m0 + k0 * g.lda : m0 * g.lda + k0), ob = batch * g.b_batch + (BC ? n0 + k0 * g.ldb : n0 * g.ldb + k0);
+  const int64_t da = AC ? GM_BK * g.lda : GM_BK, db = BC ? GM_BK * g.ldb : GM_BK;
+  const T *pa = (const T*)g.a[0] + oa, *pb = (const T*)g.b[0] + ob;
+  int64_t left = k1 - k0;
+  int segment = 0;
+  unsigned to = base;
+  auto fetch = [&]() {
+    sa.fetch(pa, left, to);
+    sb.fetch(pb, left, to + A_BYTES);
+    pa += da;
+    pb += db;
+    left -= GM_BK;
+    to ^= STAGE;
+    if (left <= 0 && ++segment < g.segments) {
+      pa = (const T*)g.a[segment] + oa;
+      pb = (const T*)g.b[segment] + ob;
+      left = k1 - k0;
+    }
   };
   const int wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
   gm_f32x4 acc[FM][FN];
@@ -149,35 +198,48 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64, BM * BN > 128 * 128 ? 1 :
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = (gm_f32x4){0.f, 0.f, 0.f, 0.f};
-  if (total > 0) fetch(0);
-  for (int64_t s = 0; s < total; ++s) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this step's stage is in the LDS ...
-    __syncthreads();                                  // ... for every wave, and the other one has been read by all
-    if (s + 1 < total) fetch(s + 1);
-    const char* const at = lds + (s & 1) * STAGE;
+  // fragments are read one half step ahead of the MFMAs that take them, the stage behind them one step ahead of that: the wait and
+  // the barrier stand between the halves, when this stage has been read to its end and the next one has had a step's time to arrive
+  gm_u32x4 fa[2][FM], fb[2][FN];
+  const char* at = lds;
+  auto read = [&](int half) {
 #pragma unroll
-    for (int kk = 0; kk < GM_BK; kk += 32) {
-      gm_u32x4 fb[FN];
+    for (int j = 0; j < FN; ++j) fb[half][j] = GemmStage<BC, BN, WAVES>::fragment(at + A_BYTES, wn + 16 * j, 32 * half);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = GemmStage<BC, BN, WAVES>::fragment(at + A_BYTES, wn + 16 * j, kk);
+    for (int i = 0; i < FM; ++i) fa[half][i] = GemmStage<AC, BM, WAVES>::fragment(at, wm + 16 * i, 32 * half);
+  };
+  auto multiply = [&](int half) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const gm_u32x4 fa = GemmStage<AC, BM, WAVES>::fragment(at, wm + 16 * i, kk);
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = gm_mma(fb[j], fa, acc[i][j], T());  // B first: a lane gets neighbours of one row
-      }
+      for (int j = 0; j < FN; ++j) acc[i][j] = gm_mma(fb[half][j], fa[half][i], acc[i][j], T());  // B first: a lane gets neighbours of one row
+  };
+  if (total > 0) {
+    fetch();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (total > 1) fetch();
+    read(0);
+    for (int64_t s = 1; s < total; ++s) {
+      read(1);
+      __builtin_amdgcn_sched_barrier(0);  // (left alone, the scheduler moves the reads behind the products, in front of the wait)
+      multiply(0);
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the next stage has arrived, this one has been read ...
+      __syncthreads();                                            // ... by every wave
+      if (s + 1 < total) fetch();
+      at = lds + ((s & 1) ? STAGE : 0);
+      read(0);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(1);
     }
+    read(1);
+    multiply(0);
+    multiply(1);
   }
-  epi.block(m0, n0, split, batch);
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int64_t r = m0 + wm + 16 * i + (lane & 15);
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      if (r < g.m) epi.put(r, n0 + wn + 16 * j + 4 * (lane >> 4), j, v);
-    }
-  }
+  __syncthreads();  // the stages are free
+  constexpr int ROWS = 2 * STAGE / WAVES >= 64 * 64 * 4 ? 64 : 32;
+  gm_epilogue<FM, FN, ROWS>(epi, acc, (float*)lds + wave * ROWS * 64, m0 + wm, n0 + wn, split, batch);
   if constexpr (Epi::COLUMN_SUMS) {
     __syncthreads();
     epi.template done<BM, BN, WM, WN>((float*)lds, wm, wn, n0, (int64_t)ti);

@@ -12,10 +12,6 @@
 // instructions take it.  The weight gradient's rows are cut into parts, whose sums are added in a fixed order: results repeat.
 #include "pp_gemm.h"
 
-typedef unsigned lin_u32x4 __attribute__((ext_vector_type(4)));
-typedef float lin_f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 lin_bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 lin_f16x8 __attribute__((ext_vector_type(8)));
 
 enum { LIN_FWD = 0, LIN_DZ = 1, LIN_STORE = 2, LIN_PART = 3 };
 
@@ -29,7 +25,7 @@ struct LinArgs {
   float slope;
   void* out;
   int n_out;             // columns written (LIN_DZ pads its rows with zeros up to here)
-  int vo;                // four neighbouring columns may be stored (and `extra` read) at once
+  int vo;                // eight neighbouring columns may be stored (and `extra` read) in 16-byte pieces
   float *part, *part_bias;   // LIN_PART: part[splits][m][n]; LIN_DZ: part_bias[row tile][n] (nullable)
   int64_t k_per_split;
 };
@@ -42,7 +38,7 @@ template <> struct LinType<float> {
 };
 
 // eight elements of the contraction, in the form they have in the LDS: PLANES x 16 bytes
-template <typename T> struct LinChunk { lin_u32x4 p[LinType<T>::PLANES]; };
+template <typename T> struct LinChunk { gm_u32x4 p[LinType<T>::PLANES]; };
 
 __device__ __forceinline__ void lin_pack(const float (&v)[8], LinChunk<float>& c) {
   unsigned h[8], m[8], l[8];
@@ -63,18 +59,18 @@ __device__ __forceinline__ void lin_pack(const float (&v)[8], LinChunk<float>& c
 __device__ __forceinline__ void lin_pack(const pp_bf16 (&v)[8], LinChunk<pp_bf16>& c) { __builtin_memcpy(&c.p[0], v, 16); }
 __device__ __forceinline__ void lin_pack(const pp_f16 (&v)[8], LinChunk<pp_f16>& c) { __builtin_memcpy(&c.p[0], v, 16); }
 
-__device__ __forceinline__ lin_f32x4 lin_mma(const LinChunk<pp_bf16>& x, const LinChunk<pp_bf16>& y, lin_f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lin_bf16x8, x.p[0]), __builtin_bit_cast(lin_bf16x8, y.p[0]), c, 0, 0, 0);
+__device__ __forceinline__ gm_f32x4 lin_mma(const LinChunk<pp_bf16>& x, const LinChunk<pp_bf16>& y, gm_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gm_bf16x8, x.p[0]), __builtin_bit_cast(gm_bf16x8, y.p[0]), c, 0, 0, 0);
 }
-__device__ __forceinline__ lin_f32x4 lin_mma(const LinChunk<pp_f16>& x, const LinChunk<pp_f16>& y, lin_f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(lin_f16x8, x.p[0]), __builtin_bit_cast(lin_f16x8, y.p[0]), c, 0, 0, 0);
+__device__ __forceinline__ gm_f32x4 lin_mma(const LinChunk<pp_f16>& x, const LinChunk<pp_f16>& y, gm_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(gm_f16x8, x.p[0]), __builtin_bit_cast(gm_f16x8, y.p[0]), c, 0, 0, 0);
 }
-__device__ __forceinline__ lin_f32x4 lin_mma(const LinChunk<float>& x, const LinChunk<float>& y, lin_f32x4 c) {
+__device__ __forceinline__ gm_f32x4 lin_mma(const LinChunk<float>& x, const LinChunk<float>& y, gm_f32x4 c) {
 #pragma unroll
   for (int s = 2; s >= 0; --s)  // smallest products first
 #pragma unroll
     for (int i = 0; i <= s; ++i)
-      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lin_bf16x8, x.p[i]), __builtin_bit_cast(lin_bf16x8, y.p[s - i]), c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gm_bf16x8, x.p[i]), __builtin_bit_cast(gm_bf16x8, y.p[s - i]), c, 0, 0, 0);
   return c;
 }
 
@@ -107,8 +103,8 @@ struct LinStage {
           constexpr int W = 16 / (int)sizeof(T);
 #pragma unroll
           for (int h = 0; h < 8 / W; ++h) {
-            lin_u32x4 q = {0u, 0u, 0u, 0u};
-            if (r < rows && k + h * W < k1) q = *(const lin_u32x4*)(p + h * W);
+            gm_u32x4 q = {0u, 0u, 0u, 0u};
+            if (r < rows && k + h * W < k1) q = *(const gm_u32x4*)(p + h * W);
             __builtin_memcpy(&v[i][h * W], &q, 16);
           }
         } else {
@@ -132,7 +128,7 @@ struct LinStage {
       }
     }
   }
-  __device__ __forceinline__ void put(lin_u32x4* __restrict__ lds) const {
+  __device__ __forceinline__ void put(gm_u32x4* __restrict__ lds) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int unit = threadIdx.x + 256 * i;
@@ -153,7 +149,7 @@ struct LinStage {
 };
 
 template <typename T, int ROWS>
-__device__ __forceinline__ LinChunk<T> lin_fragment(const lin_u32x4* __restrict__ lds, int row, int ch) {
+__device__ __forceinline__ LinChunk<T> lin_fragment(const gm_u32x4* __restrict__ lds, int row, int ch) {
   constexpr int CH = LinType<T>::BK / 8;
   LinChunk<T> c;
 #pragma unroll
@@ -161,77 +157,89 @@ __device__ __forceinline__ LinChunk<T> lin_fragment(const lin_u32x4* __restrict_
   return c;
 }
 
-// four neighbouring values of a row, fp32
-template <typename T>
-__device__ __forceinline__ void lin_load4(const T* __restrict__ p, int valid, bool vec, float (&v)[4]) {
-  if (vec) {
-    if (valid > 0) pp_load<T, 4>(p, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < valid ? (float)p[i] : 0.f;
-  }
-}
-
-// What becomes of four neighbouring columns c .. c + 3 of row r of a product.  j: the lane's column fragment (of FN)
-template <typename T, int MODE, int FN>
+// What becomes of eight neighbouring columns of a row of a product (gm_epilogue)
+template <typename T, int MODE>
 struct LinEpilogue {
-  static constexpr bool COLUMN_SUMS = MODE == LIN_DZ;
+  static constexpr bool COLUMN_SUMS = MODE == LIN_DZ, FUSED = MODE == LIN_FWD || MODE == LIN_DZ;
+  struct Row {
+    float x[FUSED ? 8 : 1];
+  };
   LinArgs a;
-  int split;
-  float zs[COLUMN_SUMS ? FN : 1][4];  // sums of dz over the lane's rows, before its rounding: the bias gradient's
+  int split, valid;
+  int64_t c;
+  float b[FUSED ? 8 : 1];
+  float zs[COLUMN_SUMS ? 8 : 1];  // sums of dz over the lane's rows, before its rounding: the bias gradient's
 
-  __device__ __forceinline__ void block(int64_t, int64_t, int split_, int64_t) {
+  __device__ __forceinline__ void block(int64_t first_column, int split_, int64_t) {
     split = split_;
+    c = first_column;
+    valid = a.n - c < 8 ? (int)(a.n - c) : 8;
 #pragma unroll
-    for (int j = 0; j < (COLUMN_SUMS ? FN : 1); ++j)
+    for (int e = 0; e < (FUSED ? 8 : 1); ++e) b[e] = FUSED && a.bias && e < valid ? (float)((const T*)a.bias)[c + e] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) zs[j][e] = 0.f;
+    for (int e = 0; e < (COLUMN_SUMS ? 8 : 1); ++e) zs[e] = 0.f;
   }
-  __device__ __forceinline__ void put(int64_t r, int64_t c, int j, float (&v)[4]) {
-    const int valid = (int)(a.n - c < 4 ? a.n - c : 4);
-    if (MODE == LIN_PART) {
-      float* const o = a.part + ((int64_t)split * a.m + r) * a.n + c;
+  __device__ __forceinline__ void load(int64_t r, Row& w) const {
+    if constexpr (FUSED) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < valid) o[e] = v[e];
-      return;
-    }
-    if (MODE == LIN_FWD || MODE == LIN_DZ) {
-      float b[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (a.bias) lin_load4((const T*)a.bias + c, valid, false, b);
-      if (a.extra) lin_load4((const T*)a.extra + r * a.n + c, valid, a.vo, x);
+      for (int e = 0; e < 8; ++e) w.x[e] = 0.f;
+      if (!a.extra || r >= a.m) return;
+      const T* p = (const T*)a.extra + r * a.n + c;
+      if (a.vo) {
+        if (valid > 0) pp_load<T, 8>(p, w.x);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        v[e] = MODE == LIN_FWD ? pp_act1(v[e] + b[e], a.act, a.slope) + x[e]
-                               : (e < valid ? x[e] * pp_dact1(v[e] + b[e], a.act, a.slope) : 0.f);  // (padding is 0, whatever the row holds)
+        for (int e = 0; e < 8; ++e)
+          if (e < valid) w.x[e] = (float)p[e];
+      }
     }
-    if (MODE == LIN_DZ) {
+  }
+  __device__ __forceinline__ void put(int64_t r, Row& w, float (&v)[8]) {
+    if (r >= a.m) return;
+    if constexpr (FUSED) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) zs[j][e] += v[e];
+      for (int e = 0; e < 8; ++e) v[e] += b[e];
+      if (MODE == LIN_FWD) {
+        pp_act(v, a.act, a.slope);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += w.x[e];
+      } else {
+        pp_dact(w.x, v, a.act, a.slope);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = e < valid ? w.x[e] : 0.f;  // (padding is 0, whatever the row holds)
+          zs[e] += v[e];
+        }
+      }
     }
-    T* const o = (T*)a.out + r * a.ldo + c;
+    if constexpr (MODE == LIN_PART) {
+      store<float>(a.part + ((int64_t)split * a.m + r) * a.n + c, v, valid);
+    } else {
+      store<T>((T*)a.out + r * a.ldo + c, v, (int)(a.n_out - c < 8 ? a.n_out - c : 8));
+    }
+  }
+  template <typename O>
+  __device__ __forceinline__ void store(O* __restrict__ o, const float (&v)[8], int count) const {
     if (a.vo) {
-      if (c < a.n_out) pp_store<T, 4>(o, v);
+      if (count > 0) pp_store<O, 8>(o, v);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c + e < a.n_out) o[e] = (T)v[e];
+      for (int e = 0; e < 8; ++e)
+        if (e < count) o[e] = (O)v[e];
     }
   }
-  // column sums of a BM x BN tile: the rows of a fragment, then the waves above each other.  red: LDS that nobody reads any more
+  // column sums of a BM x BN tile: the lanes of a column, then the waves above each other.  red: LDS that nobody reads any more
   template <int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void done(float* red, int wm, int wn, int64_t n0, int64_t row_tile) {
     if (!a.part_bias) return;
     const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
+    for (int e = 0; e < 8; ++e) {
+      float v = zs[e];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float v = zs[j][e];
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
-        if ((lane & 15) == 0) red[wm / WM * BN + wn + 16 * j + 4 * (lane >> 4) + e] = v;
-      }
+      for (int d = 8; d < 64; d <<= 1) v += __shfl_xor(v, d);
+      if (lane < 8) red[wm / WM * BN + wn + 8 * lane + e] = v;
+    }
     __syncthreads();
     for (int t = threadIdx.x; t < BN; t += blockDim.x)
       if (n0 + t < a.n) {
@@ -247,7 +255,7 @@ template <typename T, bool AS, bool BS, int MODE, int BM, int BN, int WM, int WN
 __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
   constexpr int BK = LinType<T>::BK, CH = BK / 8, PLANES = LinType<T>::PLANES, BUFS = LinType<T>::BUFS;
   constexpr int FM = WM / 16, FN = WN / 16, STEP = PLANES * (BM + BN) * CH;
-  __shared__ lin_u32x4 lds[BUFS * STEP];
+  __shared__ gm_u32x4 lds[BUFS * STEP];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
   const int64_t m0 = (int64_t)blockIdx.x * BM;
@@ -258,11 +266,11 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
     k1 = k + a.k_per_split < a.k ? k + a.k_per_split : a.k;
   }
   const T *pa = (const T*)a.a, *pb = (const T*)a.b;
-  lin_f32x4 acc[FM][FN];
+  gm_f32x4 acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = (lin_f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < FN; ++j) acc[i][j] = (gm_f32x4){0.f, 0.f, 0.f, 0.f};
   LinStage<T, AS, BM> sa;
   LinStage<T, BS, BN> sb;
   if (k < k1) {
@@ -270,7 +278,7 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
     sb.load(pb, a.ldb, n0, a.n, k, k1, a.vb);
   }
   for (int step = 0; k < k1; k += BK, ++step) {
-    lin_u32x4* const at = lds + (BUFS == 2 ? (step & 1) * STEP : 0);
+    gm_u32x4* const at = lds + (BUFS == 2 ? (step & 1) * STEP : 0);
     if (BUFS == 1) __syncthreads();  // the last step's fragments have been read
     sa.put(at);
     sb.put(at + PLANES * BM * CH);
@@ -293,19 +301,10 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
       }
     }
   }
-  // lane (l & 15, l >> 4) holds row l & 15 and columns 4 (l >> 4) .. + 3 of every 16 x 16 fragment
-  LinEpilogue<T, MODE, FN> epi;
+  LinEpilogue<T, MODE> epi;
   epi.a = a;
-  epi.block(m0, n0, blockIdx.z, 0);
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int64_t r = m0 + wm + 16 * i + (lane & 15);
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      if (r < a.m) epi.put(r, n0 + wn + 16 * j + 4 * (lane >> 4), j, v);
-    }
-  }
+  __syncthreads();
+  gm_epilogue<FM, FN, 32>(epi, acc, (float*)lds + wave * 32 * 64, m0 + wm, n0 + wn, blockIdx.z, 0);
   if constexpr (MODE == LIN_DZ) {
     __syncthreads();
     epi.template done<BM, BN, WM, WN>((float*)lds, wm, wn, n0, blockIdx.x);
@@ -330,6 +329,24 @@ __global__ __launch_bounds__(256) void k_linear_sum(const float* __restrict__ pa
     for (int k = 1; k < S; ++k) s += red[k * cols + cl];
     out[(int64_t)blockIdx.y * n + i] = (T)(float)s;
   }
+}
+
+// the same for few parts of a large matrix: four neighbouring values a thread
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_sum4(const float* __restrict__ part, int parts, int64_t n, T* __restrict__ out) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
+  for (int q = 0; q < parts; ++q) {
+    const float4 v = *(const float4*)(part + q * n + i);
+    s[0] += (double)v.x;
+    s[1] += (double)v.y;
+    s[2] += (double)v.z;
+    s[3] += (double)v.w;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[i + e] = (T)(float)s[e];
 }
 
 // column sums of a part of the rows of [n, c]: part[blockIdx.y][c]; 64 columns a block, four rows side by side
@@ -372,14 +389,14 @@ static int64_t lin_tiles(int64_t m, int64_t n, int t) { return ((m + t - 1) / t)
 
 template <typename T, bool AS, bool BS, int MODE, int BM, int BN, int WM, int WN>
 static int lin_go_wide(const LinArgs& a, int splits, hipStream_t s) {
-  LinEpilogue<T, MODE, WN / 16> e{};
+  LinEpilogue<T, MODE> e{};
   e.a = a;
   GemmArgs g{};
   g.a[0] = a.a; g.b[0] = a.b; g.segments = 1; g.m = a.m; g.n = a.n; g.k = a.k; g.lda = a.lda; g.ldb = a.ldb;
   g.splits = splits; g.k_per_split = splits > 1 ? a.k_per_split : (a.k + GM_BK - 1) / GM_BK * GM_BK;
   const int64_t tiles = ((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN);
   PP_REQUIRE(tiles <= 0x7FFFFFFF && splits <= 65535, "pp_linear_act: too many tiles");
-  hipLaunchKernelGGL((k_gemm<T, AS, BS, BM, BN, WM, WN, LinEpilogue<T, MODE, WN / 16>>), dim3((unsigned)tiles, splits, 1),
+  hipLaunchKernelGGL((k_gemm<T, AS, BS, BM, BN, WM, WN, LinEpilogue<T, MODE>>), dim3((unsigned)tiles, splits, 1),
                      dim3(BM / WM * (BN / WN) * 64), 0, s, g, e);
   PP_LAUNCH_CHECK();
   return PP_OK;
@@ -427,6 +444,11 @@ extern "C" size_t pp_linear_act_bwd_workspace(int32_t dtype, int64_t n, int32_t 
 // sums of `parts` rows of n values; more than a few hundred rows go through LIN_SUM_GROUPS partial rows behind them
 template <typename T>
 static int lin_sum(float* part, int64_t parts, int64_t n, T* out, hipStream_t s) {
+  if (parts <= 16 && n % 4 == 0 && n >= 65536) {
+    hipLaunchKernelGGL((k_linear_sum4<T>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, part, (int)parts, n, out);
+    PP_LAUNCH_CHECK();
+    return PP_OK;
+  }
   if (parts > 512) {
     float* const mid = part + parts * n;
     hipLaunchKernelGGL((k_linear_sum<float>), dim3((unsigned)((n + 15) / 16), LIN_SUM_GROUPS), dim3(256), 0, s, part, parts, n, 16, mid);
@@ -463,7 +485,7 @@ static int lin_forward(const void* x, int64_t n, int cin, const void* w, int cou
                        const void* residual, void* y, hipStream_t s) {
   LinArgs a = lin_base<T>(x, n, cin, w, cout, bias, act, slope);
   a.extra = residual; a.out = y; a.ldo = cout; a.n_out = cout;
-  a.vo = cout % 4 == 0 && lin_aligned(y, cout, 4 * sizeof(T), sizeof(T)) && lin_aligned(residual, cout, 4 * sizeof(T), sizeof(T));
+  a.vo = cout % 8 == 0 && lin_aligned(y, cout, 16, sizeof(T)) && lin_aligned(residual, cout, 16, sizeof(T));
   return lin_tile<T, false, false, LIN_FWD>(a, 1, s);
 }
 
@@ -485,7 +507,7 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
     if (n) {
       LinArgs a = lin_base<T>(x, n, cin, w, cout, bias, act, slope);
       a.extra = dy; a.out = z; a.ldo = ldz; a.n_out = (int)ldz;
-      a.vo = cout % 4 == 0 && lin_aligned(dy, cout, 4 * sizeof(T), sizeof(T));
+      a.vo = cout % 8 == 0 && lin_aligned(dy, cout, 16, sizeof(T));
       a.part_bias = db ? part_bias : nullptr;
       const int rows = lin_tile_rows<T, false, false, LIN_DZ>(a, 1);
       bias_parts = (n + rows - 1) / rows;
@@ -501,7 +523,7 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
     LinArgs a{};
     a.a = dz; a.lda = ldz; a.b = w; a.ldb = cin; a.m = n; a.n = cin; a.k = cout; a.out = dx; a.ldo = cin; a.n_out = cin;
     a.va = lin_aligned(dz, ldz, 16, sizeof(T)); a.vb = lin_aligned(w, cin, 8, sizeof(T));
-    a.vo = cin % 4 == 0 && lin_aligned(dx, cin, 4 * sizeof(T), sizeof(T));
+    a.vo = cin % 8 == 0 && lin_aligned(dx, cin, 16, sizeof(T));
     if ((rc = lin_tile<T, false, true, LIN_STORE>(a, 1, s)) != PP_OK) return rc;
   }
   if (dw) {
@@ -509,6 +531,7 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
     a.a = dz; a.lda = ldz; a.b = x; a.ldb = cin; a.m = cout; a.n = cin; a.k = n;
     a.va = lin_aligned(dz, ldz, 8, sizeof(T)); a.vb = lin_aligned(x, cin, 8, sizeof(T));
     a.part = part; a.n_out = cin;
+    a.vo = cin % 8 == 0;  // (the parts are fp32 and start on 256 bytes)
     const int splits = lin_wide<T, true, true, LIN_PART>(a) ? p1 : p0;
     a.k_per_split = ((n + splits - 1) / splits + 63) / 64 * 64;
     if ((rc = lin_tile<T, true, true, LIN_PART>(a, splits, s)) != PP_OK) return rc;

@@ -84,5 +84,26 @@ __device__ __forceinline__ float pp_dact1(float z, int act, float slope) {
   }
 }
 
+// the same of N values; the branch on `act` stands outside, which also keeps the code short
+template <int N>
+__device__ __forceinline__ void pp_act(float (&z)[N], int act, float slope) {
+#define PP_EACH(ACT) \
+  case ACT:          \
+    _Pragma("unroll") for (int i = 0; i < N; ++i) z[i] = pp_act1(z[i], ACT, slope); \
+    break;
+  switch (act) { PP_EACH(PP_ACT_RELU) PP_EACH(PP_ACT_LEAKY) PP_EACH(PP_ACT_SILU) PP_EACH(PP_ACT_GELU) default: break; }
+#undef PP_EACH
+}
+// d[i] *= act'(z[i])
+template <int N>
+__device__ __forceinline__ void pp_dact(float (&d)[N], const float (&z)[N], int act, float slope) {
+#define PP_EACH(ACT) \
+  case ACT:          \
+    _Pragma("unroll") for (int i = 0; i < N; ++i) d[i] *= pp_dact1(z[i], ACT, slope); \
+    break;
+  switch (act) { PP_EACH(PP_ACT_RELU) PP_EACH(PP_ACT_LEAKY) PP_EACH(PP_ACT_SILU) PP_EACH(PP_ACT_GELU) default: break; }
+#undef PP_EACH
+}
+
 static inline bool pp_rows_dtype_ok(int dtype) { return dtype == PP_F32 || dtype == PP_BF16 || dtype == PP_F16; }
 static inline bool pp_rows_act_ok(int act) { return act >= PP_ACT_NONE && act <= PP_ACT_GELU; }
