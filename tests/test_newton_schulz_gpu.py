@@ -51,7 +51,7 @@ def matrices(batch, m, n, dtype, seed=0, scale=1e-3):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("batch,m,n", [
     (1, 1, 1), (1, 1, 9), (2, 9, 1), (3, 5, 5), (1, 16, 64), (2, 64, 64), (4, 65, 64), (1, 63, 200), (2, 130, 75), (3, 432, 16),
-    (2, 1728, 64), (1, 864, 112), (2, 96, 700), (1, 257, 129), (1, 200, 256), (5, 33, 31),
+    (2, 1728, 64), (1, 864, 112), (2, 96, 700), (1, 257, 129), (1, 200, 256), (5, 33, 31), (2, 500, 128), (1, 127, 1000), (1, 1001, 97), (2, 48, 333), (1, 80, 81),
 ])
 def test_shapes(batch, m, n, dtype):
     check(matrices(batch, m, n, dtype, seed=m + n))
