@@ -1,144 +1,14 @@
 // Orthogonalisation of a batch of matrices by Newton-Schulz products: X = G / (|G| + eps), then `steps` times
 //   X <- X (a I + b S + c S^2),  S = X^T X                  (on the shorter side: S = X X^T, X from the left, where G is wide)
-// All of it is a polynomial of the first S.  With P = a I + b S + c S^2 the next S is P S P, and the result is X Q with Q the product
+// Two forms.  Up to a short side of NS_PANEL_MAX: all of it is a polynomial of the first S.  With P = a I + b S + c S^2 the next S is P S P, and the result is X Q with Q the product
 // of all P: the long matrix is read twice (for S, and to be multiplied by Q) instead of three times a step, and the steps work on
 // matrices of the short side only.  S, P and Q are symmetric and commute, so half of each product's tiles is computed and mirrored.
 // S is held and multiplied in fp64: in the directions of small singular values P is a I, so rounding errors of S grow by a^2 = 11.9 a
 // step there; fp64 leaves 1e-12 of them after five steps, fp32 would leave 1e-2.  |G|^2 is the trace of S.
-#include "pp_rows.h"
+// Above it: the iteration as it is written, on the bf16 matrix pipe with operands in two or three planes (further down).
+#include "pp_gemm.h"
 
 typedef double ns_f64x4 __attribute__((ext_vector_type(4)));
-
-#define NS_TILE 64
-#define NS_BK 16
-
-enum { NS_GRAM = 0, NS_CHAIN = 1, NS_APPLY = 2 };
-
-// one product R = A B of a launch; element (row, k) of A at a[row * ars + k * aks], (k, col) of B at b[col * brs + k * bks]
-struct NsJob {
-  const void *a, *b;
-  void* out;
-  const double* add;  // NS_CHAIN: out = c0 I + c1 add + c2 R (nullable: c2 R)
-  double c0, c1, c2;
-  int pow1, pow2;     // powers of the batch element's alpha that multiply c1 and c2 (the first step works on the unscaled S)
-};
-struct NsArgs {
-  NsJob job[2];
-  int jobs;
-  int64_t rows, cols, k;       // of R
-  int64_t ars, aks, brs, bks, ors;
-  int64_t a_batch, b_batch, out_batch;
-  const double* alpha;         // [batch]
-  int splits;
-  int64_t k_per_split;
-  int symmetric;               // only tiles on and below the diagonal are computed; NS_CHAIN mirrors them
-};
-
-// four values a thread brings of a NS_TILE x NS_BK part: rows run along the threads where they are neighbours in memory, else k does
-template <typename T>
-__device__ __forceinline__ void ns_load(const T* __restrict__ p, int64_t rs, int64_t ks, int64_t row0, int64_t rows, int64_t k0, int64_t k1,
-                                        double (&v)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = rs == 1 ? threadIdx.x & 63 : (threadIdx.x >> 4) + 16 * i, k = rs == 1 ? (threadIdx.x >> 6) + 4 * i : threadIdx.x & 15;
-    v[i] = row0 + r < rows && k0 + k < k1 ? (double)p[(row0 + r) * rs + (k0 + k) * ks] : 0.0;
-  }
-}
-__device__ __forceinline__ void ns_put(double* __restrict__ lds, int64_t rs, const double (&v)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = rs == 1 ? threadIdx.x & 63 : (threadIdx.x >> 4) + 16 * i, k = rs == 1 ? (threadIdx.x >> 6) + 4 * i : threadIdx.x & 15;
-    lds[k * (NS_TILE + 16) + r] = v[i];  // rows of 80 doubles: four k of a fragment fall on both halves of the banks
-  }
-}
-
-template <typename TA, typename TB, typename TO, int MODE>
-__global__ __launch_bounds__(256) void k_ns_tile(NsArgs g) {
-  __shared__ double sa[2][NS_BK * (NS_TILE + 16)], sb[2][NS_BK * (NS_TILE + 16)];
-  int64_t ti, tj;
-  if (g.symmetric) {  // blockIdx.x counts the tiles on and below the diagonal, row by row
-    ti = (int64_t)((sqrt(8.0 * (double)blockIdx.x + 1.0) - 1.0) * 0.5);
-    while ((ti + 1) * (ti + 2) / 2 <= (int64_t)blockIdx.x) ++ti;
-    while (ti * (ti + 1) / 2 > (int64_t)blockIdx.x) --ti;
-    tj = (int64_t)blockIdx.x - ti * (ti + 1) / 2;
-  } else {
-    const int64_t tc = (g.cols + NS_TILE - 1) / NS_TILE;
-    ti = blockIdx.x / tc;
-    tj = blockIdx.x - ti * tc;
-  }
-  const int which = MODE == NS_CHAIN ? blockIdx.y : 0;
-  const int split = MODE == NS_GRAM ? blockIdx.y : 0;
-  const int64_t batch = blockIdx.z;
-  const NsJob& job = g.job[which];
-  const TA* a = (const TA*)job.a + batch * g.a_batch;
-  const TB* b = (const TB*)job.b + batch * g.b_batch;
-  const int64_t r0 = ti * NS_TILE, c0 = tj * NS_TILE;
-  int64_t k = 0, k1 = g.k;
-  if (MODE == NS_GRAM) {
-    k = split * g.k_per_split;
-    k1 = k + g.k_per_split < g.k ? k + g.k_per_split : g.k;
-  }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = (wave & 1) * 32, wc = (wave >> 1) * 32;
-  ns_f64x4 acc[2][2] = {};
-  double va[4], vb[4];
-  if (k < k1) {
-    ns_load(a, g.ars, g.aks, r0, g.rows, k, k1, va);
-    ns_load(b, g.brs, g.bks, c0, g.cols, k, k1, vb);
-  }
-  for (int step = 0; k < k1; k += NS_BK, ++step) {
-    double *la = sa[step & 1], *lb = sb[step & 1];
-    ns_put(la, g.ars, va);
-    ns_put(lb, g.brs, vb);
-    __syncthreads();
-    if (k + NS_BK < k1) {
-      ns_load(a, g.ars, g.aks, r0, g.rows, k + NS_BK, k1, va);
-      ns_load(b, g.brs, g.bks, c0, g.cols, k + NS_BK, k1, vb);
-    }
-#pragma unroll
-    for (int kk = 0; kk < NS_BK; kk += 4) {
-      const int at = (kk + (lane >> 4)) * (NS_TILE + 16) + (lane & 15);
-      double fa[2], fb[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fa[i] = la[at + wr + 16 * i];
-        fb[i] = lb[at + wc + 16 * i];
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(fa[i], fb[j], acc[i][j], 0, 0, 0);
-    }
-  }
-  // lane (l & 15, l >> 4), value e: row (l >> 4) + 4 e, column l & 15 of the fragment
-  double c1 = job.c1, c2 = job.c2;
-  if (g.alpha) {
-    const double al = g.alpha[batch];
-    for (int p = 0; p < job.pow1; ++p) c1 *= al;
-    for (int p = 0; p < job.pow2; ++p) c2 *= al;
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t r = r0 + wr + 16 * i + (lane >> 4) + 4 * e, c = c0 + wc + 16 * j + (lane & 15);
-        if (r >= g.rows || c >= g.cols) continue;
-        const double v = acc[i][j][e];
-        if (MODE == NS_GRAM) {
-          ((double*)job.out)[(batch * g.splits + split) * g.rows * g.cols + r * g.cols + c] = v;
-        } else if (MODE == NS_APPLY) {
-          ((TO*)job.out)[batch * g.out_batch + r * g.ors + c] = (TO)(float)(c2 * v);
-        } else if (!g.symmetric || c <= r) {
-          double* o = (double*)job.out + batch * g.out_batch;
-          double w = c2 * v;
-          if (job.add) w += c1 * job.add[batch * g.out_batch + r * g.cols + c];
-          if (r == c) w += job.c0;
-          o[r * g.cols + c] = w;
-          if (g.symmetric) o[c * g.cols + r] = w;
-        }
-      }
-}
 
 // ---- one step in one launch, for a short side of at most NS_PANEL_MAX ------------------------------------------------------------
 // All factors are polynomials of S, so a workgroup that holds the whole of S in its LDS can take 16 rows of everything through a step on
@@ -427,34 +297,231 @@ __global__ __launch_bounds__(256) void k_ns_sum(const double* __restrict__ part,
     out[batch * s * s + c * s + r] = v;
   }
 }
-// alpha = 1 / (|G| + eps)
-__global__ __launch_bounds__(64) void k_ns_alpha(const double* __restrict__ S, int64_t s, double eps, double* __restrict__ alpha) {
-  const double* p = S + (int64_t)blockIdx.x * s * s;
+// ---- short sides above NS_PANEL_MAX -------------------------------------------------------------------------------------------------
+// Here the products are large enough for the matrix pipe, and fp64 is 32 times slower than bf16 on it: the iteration runs as it is
+// defined, X <- X P with S = X^T X, T = S S, P = a I + b S + c T anew in every step (an error of S is not carried on, so no growth of it
+// beyond what the definition has in fp32).  Matrices are sums of bf16 planes, hi + lo (16 bits) for 16-bit results, hi + mid + lo (24
+// bits) for fp32 ones; a product takes the plane pairs above the last plane's rounding (3, or 6), on k_gemm.  X starts as G 2^e with 2^e
+// the power of two at 1 / (|G| + eps), which needs no rounding (bf16: one plane); the rest of the scale, f in [1, 2), enters the first P.
+// Two planes carry 2^-17 of a value (P and X are rounded to them, each step), three 2^-25: below the half step of the results' type.
+// S and T: lower tiles, the contraction in parts to fill the chip, added in order where S's and P's planes are made.
+
+struct NsScale {  // per batch element
+  float f, pad;
+};
+
+// partial sums of squares of a batch element: part[batch][NS_NORM_PARTS]
+#define NS_NORM_PARTS 64
+template <typename T>
+__global__ __launch_bounds__(256) void k_ns_norm(const T* __restrict__ g, int64_t count, double* __restrict__ part) {
+  __shared__ double red[4];
+  const T* p = g + (int64_t)blockIdx.y * count;
   double v = 0.0;
-  for (int64_t i = threadIdx.x; i < s; i += 64) v += p[i * s + i];
+#pragma unroll 8
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += NS_NORM_PARTS * 256) {
+    const double x = (double)(float)p[i];
+    v = fma(x, x, v);
+  }
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-  if (threadIdx.x == 0) alpha[blockIdx.x] = 1.0 / (sqrt(v) + eps);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) part[(int64_t)blockIdx.y * NS_NORM_PARTS + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+// v as NP bf16 terms
+template <int NP>
+__device__ __forceinline__ void ns_planes(float v, pp_bf16 (&p)[NP]) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    p[i] = (pp_bf16)v;
+    v -= (float)p[i];
+  }
+}
+
+// X = G 2^e in NP planes [m][ld], zeros behind the columns; f of the batch element
+template <typename T, int NP>
+__global__ __launch_bounds__(256) void k_ns_scale(const T* __restrict__ g, int64_t m, int64_t n, int64_t ld, const double* __restrict__ part,
+                                                  double eps, pp_bf16* __restrict__ planes, int64_t plane, NsScale* __restrict__ scale) {
+  const int64_t batch = blockIdx.y;
+  double v = part[batch * NS_NORM_PARTS + (threadIdx.x & 63)];
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  const double alpha = 1.0 / (sqrt(v) + eps);
+  double two = 1.0;
+  float f;
+  if (alpha > 0.0 && alpha < 1e300) {
+    int e;
+    f = 2.f * (float)frexp(alpha, &e);
+    two = ldexp(1.0, e - 1);
+  } else {
+    f = (float)alpha;  // 0, infinity or NaN: the result is NaN, as the definition's
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) scale[batch].f = f;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8, r = i / ld, c = i - r * ld;
+  if (r >= m) return;
+  gm_u32x4 out[NP];
+  pp_bf16* const o = (pp_bf16*)out;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    pp_bf16 p[NP];
+    ns_planes<NP>(c + k < n ? (float)((double)(float)g[batch * m * n + r * n + c + k] * two) : 0.f, p);
+#pragma unroll
+    for (int q = 0; q < NP; ++q) o[q * 8 + k] = p[q];
+  }
+#pragma unroll
+  for (int q = 0; q < NP; ++q) *(gm_u32x4*)(planes + q * plane + batch * m * ld + i) = out[q];
+}
+
+// epilogue of S and T: the part's fp32 sums
+struct NsPartEpilogue {
+  static constexpr bool COLUMN_SUMS = false;
+  struct Row {};
+  float* part;
+  int64_t s, ld;
+  int splits;
+  int64_t c;
+  float* o;
+  __device__ __forceinline__ void block(int64_t first_column, int split, int64_t batch) {
+    c = first_column;
+    o = part + (batch * splits + split) * s * ld + c;
+  }
+  __device__ __forceinline__ void load(int64_t, Row&) const {}
+  __device__ __forceinline__ void put(int64_t r, Row&, float (&v)[8]) {
+    if (r < s && c < ld) pp_store<float, 8>(o + r * ld, v);
+  }
+};
+// epilogue of X P: the next X's planes, zeros behind the columns, or after the last step the result
+template <typename T, int NP>
+struct NsXEpilogue {
+  static constexpr bool COLUMN_SUMS = false;
+  struct Row {};
+  pp_bf16* planes;
+  int64_t plane, m, n, ld;
+  T* out;  // nullable
+  int vec;
+  int64_t c, at;
+  __device__ __forceinline__ void block(int64_t first_column, int, int64_t batch) {
+    c = first_column;
+    at = batch;
+  }
+  __device__ __forceinline__ void load(int64_t, Row&) const {}
+  __device__ __forceinline__ void put(int64_t r, Row&, float (&v)[8]) {
+    if (r >= m || c >= n) return;
+    if (out) {
+      T* const o = out + (at * m + r) * n + c;
+      if (vec) {
+        pp_store<T, 8>(o, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < n) o[e] = (T)v[e];
+      }
+      return;
+    }
+    gm_u32x4 w[NP];
+    pp_bf16* const o = (pp_bf16*)w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      pp_bf16 p[NP];
+      ns_planes<NP>(c + e < n ? v[e] : 0.f, p);
+#pragma unroll
+      for (int q = 0; q < NP; ++q) o[q * 8 + e] = p[q];
+    }
+#pragma unroll
+    for (int q = 0; q < NP; ++q) *(gm_u32x4*)(planes + q * plane + (at * m + r) * ld + c) = w[q];
+  }
+};
+
+// A 32 x 32 tile on or below the diagonal and its mirror image: adds the parts, then
+//   S32 null: S -> planes, S kept in fp32 (to `keep`);   else: P = f (c0 I + c1 f^2 S + c2 f^4 T) -> planes, T the parts' sum
+template <int NP>
+__global__ __launch_bounds__(256) void k_ns_square(const float* __restrict__ part, int splits, int64_t s, int64_t ld, float* __restrict__ keep,
+                                                   const float* __restrict__ S32, const NsScale* __restrict__ scale, double c0, double c1,
+                                                   double c2, pp_bf16* __restrict__ planes, int64_t plane) {
+  __shared__ float tile[32][33];
+  int ti = (int)((sqrtf(8.f * (float)blockIdx.x + 1.f) - 1.f) * 0.5f);
+  while ((ti + 1) * (ti + 2) / 2 <= (int)blockIdx.x) ++ti;
+  while (ti * (ti + 1) / 2 > (int)blockIdx.x) --ti;
+  const int tj = (int)blockIdx.x - ti * (ti + 1) / 2;
+  const int64_t batch = blockIdx.y, size = s * ld;
+  const int x = threadIdx.x & 31;
+  const double f = scale ? (double)scale[batch].f : 1.0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int y = (threadIdx.x >> 5) + 8 * k;
+    const int64_t r = ti * 32 + y, c = tj * 32 + x;
+    float v = 0.f;
+    if (r < s && c < s) {
+      float sum = 0.f;
+#pragma unroll 4
+      for (int q = 0; q < splits; ++q) sum += part[(batch * splits + q) * size + r * ld + c];
+      if (S32) {
+        const double t = c2 * (f * f) * (f * f) * (double)sum + c1 * (f * f) * (double)S32[batch * size + r * ld + c] + (r == c ? c0 : 0.0);
+        v = (float)(f * t);
+      } else {
+        v = sum;
+        keep[batch * size + r * ld + c] = v;
+      }
+    }
+    tile[y][x] = v;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int mirror = 0; mirror < 2; ++mirror) {
+    if (mirror && ti == tj) break;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int y = (threadIdx.x >> 5) + 8 * k;
+      const int64_t r = (mirror ? tj : ti) * 32 + y, c = (mirror ? ti : tj) * 32 + x;
+      if (r >= s || c >= ld) continue;  // (columns s .. ld - 1 get the zeros of the tile)
+      pp_bf16 p[NP];
+      ns_planes<NP>(mirror || (ti == tj && x > y) ? tile[x][y] : tile[y][x], p);
+#pragma unroll
+      for (int q = 0; q < NP; ++q) planes[q * plane + batch * size + r * ld + c] = p[q];
+    }
+  }
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------
-static int64_t ns_lower_tiles(int64_t s) {
-  const int64_t t = (s + NS_TILE - 1) / NS_TILE;
-  return t * (t + 1) / 2;
+static int ns_parts(int64_t l) { return (int)((l + NS_LONG - 1) / NS_LONG); }
+static int64_t ns_lower(int64_t s, int64_t t) {
+  const int64_t k = (s + t - 1) / t;
+  return k * (k + 1) / 2;
 }
-// parts of the long side: about two workgroups per compute unit, at least 128 of it each
-static int ns_splits(int64_t batch, int64_t s, int64_t l) {
-  if (s <= NS_PANEL_MAX) return (int)((l + NS_LONG - 1) / NS_LONG);
-  int64_t q = 512 / (ns_lower_tiles(s) * batch);
-  if (q > (l + 127) / 128) q = (l + 127) / 128;
+// parts of a contraction of length k behind the lower 128 x 128 tiles of an s x s result: two workgroups per compute unit, a part is at
+// least 256 long
+static int ns_splits(int64_t batch, int64_t s, int64_t k) {
+  int64_t q = 512 / (ns_lower(s, 128) * batch);
+  if (q > (k + 255) / 256) q = (k + 255) / 256;
   return q < 1 ? 1 : (int)q;
+}
+static int64_t ns_round8(int64_t v) { return (v + 7) / 8 * 8; }
+
+struct NsLargeWs {
+  double* norm;
+  NsScale* scale;
+  float *part, *S32;
+  pp_bf16 *X[2], *S, *P;
+};
+static size_t ns_large_ws(PPArena* ws, int planes, int64_t batch, int64_t m, int64_t n, NsLargeWs* w) {
+  const int64_t s = m < n ? m : n, l = m < n ? n : m, ld = ns_round8(s), xs = batch * m * ns_round8(n), ss = batch * s * ld;
+  const int s0 = ns_splits(batch, s, l), s1 = ns_splits(batch, s, s);
+  const size_t sizes[8] = {(size_t)batch * NS_NORM_PARTS * 8, (size_t)batch * sizeof(NsScale), (size_t)(s0 > s1 ? s0 : s1) * ss * 4, (size_t)ss * 4,
+                           (size_t)xs * planes * 2, (size_t)xs * planes * 2, (size_t)ss * planes * 2, (size_t)ss * planes * 2};
+  size_t total = 0;
+  void* at[8];
+  for (int i = 0; i < 8; ++i) {
+    total += pp_align(sizes[i]);
+    if (ws) at[i] = ws->take<char>(sizes[i]);
+  }
+  if (ws) *w = NsLargeWs{(double*)at[0], (NsScale*)at[1], (float*)at[2], (float*)at[3], {(pp_bf16*)at[4], (pp_bf16*)at[5]}, (pp_bf16*)at[6], (pp_bf16*)at[7]};
+  return total;
 }
 
 extern "C" size_t pp_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n) {
   if (batch < 0 || m < 1 || n < 1 || m > 65536 * 64 || n > 65536 * 64) return 0;
   const int64_t s = m < n ? m : n, l = m < n ? n : m;
-  const size_t one = pp_align((size_t)batch * s * s * sizeof(double));
-  return pp_align((size_t)ns_splits(batch > 0 ? batch : 1, s, l) * batch * s * s * sizeof(double)) + 6 * one +
-         pp_align((size_t)batch * sizeof(double)) + 256;
+  if (s > NS_PANEL_MAX) return ns_large_ws(nullptr, 3, batch > 0 ? batch : 1, m, n, nullptr) + 256;
+  return pp_align((size_t)ns_parts(l) * batch * s * s * sizeof(double)) + 4 * pp_align((size_t)batch * s * s * sizeof(double)) + 256;
 }
 
 template <int SB>
@@ -511,96 +578,107 @@ static int ns_part_apply(const T* g, int64_t m, int64_t n, int64_t s, int vec, c
 #undef NS_CALL
 }
 
+// plane pairs of a product of operands of pa and pb planes, the smallest first: pairs whose product is below the last plane are left out
+static void ns_segments(GemmArgs& g, const pp_bf16* a, int64_t a_plane, int pa, const pp_bf16* b, int64_t b_plane, int pb, int planes) {
+  g.segments = 0;
+  for (int sum = planes - 1; sum >= 0; --sum)
+    for (int i = 0; i <= sum; ++i)
+      if (i < pa && sum - i < pb) {
+        g.a[g.segments] = a + i * a_plane;
+        g.b[g.segments++] = b + (sum - i) * b_plane;
+      }
+}
+template <bool AC, bool BC, int BM, int BN, int WM, int WN, typename Epi>
+static int ns_gemm(GemmArgs& g, const Epi& e, int64_t batch, hipStream_t st) {
+  const int64_t tiles = g.lower ? ns_lower(g.m, BM) : ((g.m + BM - 1) / BM) * ((g.n + BN - 1) / BN);
+  PP_REQUIRE(tiles <= 0x7FFFFFFF, "pp_newton_schulz: too many tiles");
+  if (g.splits < 1) g.splits = 1;
+  g.k_per_split = ((g.k + g.splits - 1) / g.splits + GM_BK - 1) / GM_BK * GM_BK;
+  hipLaunchKernelGGL((k_gemm<pp_bf16, AC, BC, BM, BN, WM, WN, Epi>), dim3((unsigned)tiles, g.splits, (unsigned)batch),
+                     dim3(BM / WM * (BN / WN) * 64), 0, st, g, e);
+  PP_LAUNCH_CHECK();
+  return PP_OK;
+}
+
+template <typename T, int NP>
+static int ns_large(const T* g, int64_t batch, int64_t m, int64_t n, int steps, double ca, double cb, double cc, double eps, T* out, PPArena& ws,
+                    hipStream_t st) {
+  const bool tall = m >= n;
+  const int64_t s = tall ? n : m, l = tall ? m : n, ld = ns_round8(s), ldx = ns_round8(n), xplane = batch * m * ldx, splane = batch * s * ld;
+  NsLargeWs w;
+  ns_large_ws(&ws, NP, batch, m, n, &w);
+  PP_REQUIRE(w.norm && w.scale && w.part && w.S32 && w.X[0] && w.X[1] && w.S && w.P, "pp_newton_schulz: workspace layout");
+  const unsigned nb = (unsigned)batch;
+  hipLaunchKernelGGL((k_ns_norm<T>), dim3(NS_NORM_PARTS, nb), dim3(256), 0, st, g, m * n, w.norm);
+  hipLaunchKernelGGL((k_ns_scale<T, NP>), dim3((unsigned)((m * ldx / 8 + 255) / 256), nb), dim3(256), 0, st, g, m, n, ldx, w.norm, eps, w.X[0], xplane,
+                     w.scale);
+  PP_LAUNCH_CHECK();
+  int rc;
+  for (int k = 0; k < steps; ++k) {
+    const pp_bf16* X = w.X[k & 1];
+    const int px = k == 0 && sizeof(T) == 2 && NP == 2 && __is_same(T, pp_bf16) ? 1 : NP;  // (bf16: G 2^e is one plane)
+    GemmArgs a{};
+    a.m = a.n = s; a.k = l; a.lda = a.ldb = ldx; a.a_batch = a.b_batch = m * ldx; a.lower = 1; a.splits = ns_splits(batch, s, l);
+    ns_segments(a, X, xplane, px, X, xplane, px, NP);
+    NsPartEpilogue pe{};
+    pe.part = w.part; pe.s = s; pe.ld = ld; pe.splits = a.splits;
+    rc = tall ? ns_gemm<true, true, 128, 128, 64, 64>(a, pe, batch, st) : ns_gemm<false, false, 128, 128, 64, 64>(a, pe, batch, st);
+    if (rc != PP_OK) return rc;
+    const unsigned sq = (unsigned)ns_lower(s, 32);
+    hipLaunchKernelGGL((k_ns_square<NP>), dim3(sq, nb), dim3(256), 0, st, w.part, a.splits, s, ld, w.S32, (const float*)nullptr,
+                       (const NsScale*)nullptr, 0.0, 0.0, 0.0, w.S, splane);
+    a = GemmArgs{};
+    a.m = a.n = a.k = s; a.lda = a.ldb = ld; a.a_batch = a.b_batch = s * ld; a.lower = 1; a.splits = ns_splits(batch, s, s);
+    ns_segments(a, w.S, splane, NP, w.S, splane, NP, NP);
+    pe.splits = a.splits;
+    if ((rc = ns_gemm<false, false, 128, 128, 64, 64>(a, pe, batch, st)) != PP_OK) return rc;
+    hipLaunchKernelGGL((k_ns_square<NP>), dim3(sq, nb), dim3(256), 0, st, w.part, a.splits, s, ld, (float*)nullptr, w.S32,
+                       k == 0 ? w.scale : (const NsScale*)nullptr, ca, cb, cc, w.P, splane);
+    PP_LAUNCH_CHECK();
+    NsXEpilogue<T, NP> xe{};
+    xe.planes = w.X[~k & 1]; xe.plane = xplane; xe.m = m; xe.n = n; xe.ld = ldx; xe.out = k == steps - 1 ? out : nullptr;
+    xe.vec = n % 8 == 0 && (uintptr_t)out % 16 == 0;
+    a = GemmArgs{};
+    a.m = m; a.n = n; a.k = s;
+    const bool large = ((m + 255) / 256) * ((n + 255) / 256) * batch >= 128;
+    if (tall) {
+      a.lda = ldx; a.a_batch = m * ldx; a.ldb = ld; a.b_batch = s * ld;
+      ns_segments(a, X, xplane, px, w.P, splane, NP, NP);
+      rc = large ? ns_gemm<false, false, 256, 256, 128, 64>(a, xe, batch, st) : ns_gemm<false, false, 128, 128, 64, 64>(a, xe, batch, st);
+    } else {
+      a.lda = ld; a.a_batch = s * ld; a.ldb = ldx; a.b_batch = m * ldx;
+      ns_segments(a, w.P, splane, NP, X, xplane, px, NP);
+      rc = large ? ns_gemm<false, true, 256, 256, 128, 64>(a, xe, batch, st) : ns_gemm<false, true, 128, 128, 64, 64>(a, xe, batch, st);
+    }
+    if (rc != PP_OK) return rc;
+  }
+  return PP_OK;
+}
+
 template <typename T>
 static int ns_run(const void* g, int64_t batch, int64_t m, int64_t n, int steps, double ca, double cb, double cc, double eps, void* out,
                   PPArena& ws, hipStream_t st) {
-  const bool tall = m >= n;
-  const int64_t s = tall ? n : m, l = tall ? m : n;
-  const int splits = ns_splits(batch, s, l);
+  const int64_t s = m < n ? m : n, l = m < n ? n : m;
+  if (s > NS_PANEL_MAX) return ns_large<T, sizeof(T) == 2 ? 2 : 3>((const T*)g, batch, m, n, steps, ca, cb, cc, eps, (T*)out, ws, st);
+  const int splits = ns_parts(l);
   double* part = ws.take<double>((size_t)splits * batch * s * s);
-  double* mats[6];
+  double* mats[4];
   for (double*& p : mats) p = ws.take<double>((size_t)batch * s * s);
-  double* alpha = ws.take<double>((size_t)batch);
-  PP_REQUIRE(part && mats[5] && alpha, "pp_newton_schulz: workspace layout");
-  const unsigned low = (unsigned)ns_lower_tiles(s), nb = (unsigned)batch;
-  const bool panels = s <= NS_PANEL_MAX;
+  PP_REQUIRE(part && mats[3], "pp_newton_schulz: workspace layout");
+  const unsigned nb = (unsigned)batch;
   const int vec = n % 4 == 0 && (uintptr_t)g % (4 * sizeof(T)) == 0;
-  if (panels) {
-    int rc = ns_part_gram<T>((const T*)g, m, n, s, splits, vec, part, nb, st);
-    if (rc != PP_OK) return rc;
-    hipLaunchKernelGGL(k_ns_sum, dim3((unsigned)((s * s + 31) / 32), nb), dim3(256), 0, st, part, splits, s, mats[0]);
-    PP_LAUNCH_CHECK();
-  } else {  // S of the matrix as it is
-    NsArgs a{};
-    a.job[0].a = a.job[0].b = g; a.job[0].out = part;
-    a.rows = a.cols = s; a.k = l;
-    a.ars = a.brs = tall ? 1 : n; a.aks = a.bks = tall ? n : 1;
-    a.a_batch = a.b_batch = m * n;
-    a.splits = splits; a.k_per_split = ((l + splits - 1) / splits + NS_BK - 1) / NS_BK * NS_BK; a.symmetric = 1;
-    hipLaunchKernelGGL((k_ns_tile<T, T, double, NS_GRAM>), dim3(low, splits, nb), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(k_ns_sum, dim3((unsigned)((s * s + 31) / 32), nb), dim3(256), 0, st, part, splits, s, mats[0]);
-    hipLaunchKernelGGL(k_ns_alpha, dim3(nb), dim3(64), 0, st, mats[0], s, eps, alpha);
-    PP_LAUNCH_CHECK();
-  }
-  double *S = mats[0], *P = mats[1], *U = mats[2], *N = mats[3], *Q = mats[4], *R = mats[5];
-  if (panels) {
-    NsStepArgs p{};
-    p.s = s; p.a = ca; p.b = cb; p.c = cc; p.eps = eps;
-    for (int k = 0; k < steps; ++k) {
-      p.S = k & 1 ? N : S; p.S2 = k == steps - 1 ? nullptr : (k & 1 ? S : N);
-      p.Q = k == 0 ? nullptr : (k & 1 ? Q : R); p.Q2 = k & 1 ? R : Q;
-      int rc = ns_step(p, nb, st);
-      if (rc != PP_OK) return rc;
-    }
-    return ns_part_apply<T>((const T*)g, m, n, s, vec, steps & 1 ? Q : R, (T*)out, nb, st);
-  }
-  NsArgs a{};
-  a.rows = a.cols = a.k = s; a.ars = a.brs = 1; a.aks = a.bks = s; a.ors = s;
-  a.a_batch = a.b_batch = a.out_batch = s * s; a.alpha = alpha; a.symmetric = 1;
-  auto chain = [&](int jobs) -> int {
-    hipLaunchKernelGGL((k_ns_tile<double, double, double, NS_CHAIN>), dim3(low, jobs, nb), dim3(256), 0, st, a);
-    PP_LAUNCH_CHECK();
-    return PP_OK;
-  };
-  int rc;
-  for (int k = 0; k < steps; ++k) {
-    const int p = k == 0 ? 2 : 0;  // S is scaled by alpha^2 from the second step on
-    a.job[0] = NsJob{S, S, P, S, ca, cb, cc, p, 2 * p};
-    if ((rc = chain(1)) != PP_OK) return rc;
-    const bool last = k == steps - 1;
-    int jobs = 0;
-    if (k > 0) {  // Q <- Q P
-      a.job[jobs++] = NsJob{Q, P, R, nullptr, 0.0, 0.0, 1.0, 0, 0};
-    }
-    if (!last) a.job[jobs++] = NsJob{S, P, U, nullptr, 0.0, 0.0, 1.0, 0, p};
-    if (jobs && (rc = chain(jobs)) != PP_OK) return rc;
-    if (k > 0) {
-      double* t = Q; Q = R; R = t;
-    } else {  // Q = P: the next step's P goes elsewhere
-      double* t = Q; Q = P; P = t;
-    }
-    if (!last) {  // S <- U P with this step's P (in Q after the first step)
-      a.job[0] = NsJob{U, k == 0 ? Q : P, N, nullptr, 0.0, 0.0, 1.0, 0, 0};
-      if ((rc = chain(1)) != PP_OK) return rc;
-      double* t = S; S = N; N = t;
-    }
-  }
-  NsArgs e{};
-  e.alpha = alpha; e.k = s; e.rows = m; e.cols = n; e.ors = n; e.out_batch = m * n;
-  e.job[0].c2 = 1.0; e.job[0].pow2 = 1; e.job[0].out = out;
-  const int64_t tiles = ((m + NS_TILE - 1) / NS_TILE) * ((n + NS_TILE - 1) / NS_TILE);
-  PP_REQUIRE(tiles <= 0x7FFFFFFF, "pp_newton_schulz: too many tiles");
-  if (tall) {
-    e.job[0].a = g; e.ars = n; e.aks = 1; e.a_batch = m * n;
-    e.job[0].b = Q; e.brs = 1; e.bks = s; e.b_batch = s * s;
-    hipLaunchKernelGGL((k_ns_tile<T, double, T, NS_APPLY>), dim3((unsigned)tiles, 1, nb), dim3(256), 0, st, e);
-  } else {
-    e.job[0].a = Q; e.ars = 1; e.aks = s; e.a_batch = s * s;
-    e.job[0].b = g; e.brs = 1; e.bks = n; e.b_batch = m * n;
-    hipLaunchKernelGGL((k_ns_tile<double, T, T, NS_APPLY>), dim3((unsigned)tiles, 1, nb), dim3(256), 0, st, e);
-  }
+  int rc = ns_part_gram<T>((const T*)g, m, n, s, splits, vec, part, nb, st);
+  if (rc != PP_OK) return rc;
+  hipLaunchKernelGGL(k_ns_sum, dim3((unsigned)((s * s + 31) / 32), nb), dim3(256), 0, st, part, splits, s, mats[0]);
   PP_LAUNCH_CHECK();
-  return PP_OK;
+  NsStepArgs p{};
+  p.s = s; p.a = ca; p.b = cb; p.c = cc; p.eps = eps;
+  for (int k = 0; k < steps; ++k) {  // S in mats[0], mats[1] in turn, Q in mats[2], mats[3]
+    p.S = mats[k & 1]; p.S2 = k == steps - 1 ? nullptr : mats[~k & 1];
+    p.Q = k == 0 ? nullptr : mats[2 + (~k & 1)]; p.Q2 = mats[2 + (k & 1)];
+    if ((rc = ns_step(p, nb, st)) != PP_OK) return rc;
+  }
+  return ns_part_apply<T>((const T*)g, m, n, s, vec, mats[2 + (~steps & 1)], (T*)out, nb, st);
 }
 
 extern "C" int pp_newton_schulz(const void* g, int32_t dtype, int64_t batch, int64_t m, int64_t n, int32_t steps, double ca, double cb,

@@ -3,7 +3,12 @@
 Error bound.  The steps run in fp64 on the Gram matrix S of the shorter side s.  An error of S grows by at most a^2 = 11.9 a step
 (in the directions where S is near 0; elsewhere the iteration contracts), a product of s terms rounds by s 2^-53 at most, and a step
 has four of them: 4 s 2^-53 (1 + 11.9 + .. + 11.9^(steps - 1)) < 4 s 2^-53 1.1 a^(2 steps - 2), taken relative to the largest value an
-entry can have (the largest singular value, 1.3).  The result is rounded to fp32 and to its type."""
+entry can have (the largest singular value, 1.3).  The result is rounded to fp32 and to its type.
+
+Shorter sides above 128 run the iteration in operands of two (16-bit types) or three bf16 planes, e = 2^-18 or 2^-26 of a value (each
+plane rounds to half a step of 8 bits).  In a step, X, P and S are rounded to planes and the products leave out pairs below e: less than
+9 e |P| |X|_F in all (S enters P with |b + 2 c S| < 5), and fp32 sums of 6 s products of random sign add sqrt(6 s) u |P| |X|_F.  What a
+step brings grows in the later ones by at most max |p'(sigma)| over the singular values they meet, p(x) = a x + b x^3 + c x^5."""
 import pytest
 import torch
 
@@ -15,17 +20,25 @@ A, B, C = ops.NEWTON_SCHULZ_COEFFICIENTS
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
-def iterate(g, steps=5, coefficients=(A, B, C), eps=1e-7):
-    """the definition, one matrix, 64 bits on the CPU"""
+def iterate(g, steps=5, coefficients=(A, B, C), eps=1e-7, planes=None):
+    """the definition, one matrix, 64 bits on the CPU; with `planes`, and the bound of the plane form's error (Frobenius norm)"""
     a, b, c = coefficients
     x = g.detach().double().cpu()
     x = x / (x.norm() + eps)
     tall = x.shape[0] > x.shape[1]
     x = x.t() if tall else x
+    e = {None: 0.0, 2: 2.0 ** -18, 3: 2.0 ** -26}[planes]
+    bound = 0.0
     for _ in range(steps):
         s = x @ x.t()
-        x = a * x + (b * s + c * (s @ s)) @ x
-    return x.t() if tall else x
+        p = a * torch.eye(len(s), dtype=torch.float64) + b * s + c * (s @ s)
+        if planes:
+            lam = torch.linalg.eigvalsh(s).clamp(min=0)
+            bound = bound * float((a + 3 * b * lam + 5 * c * lam * lam).abs().max())
+            bound += (9 * e + (6 * len(s)) ** 0.5 * 2.0 ** -24) * float(torch.linalg.matrix_norm(p, 2)) * float(x.norm())
+        x = p @ x
+    x = x.t() if tall else x
+    return (x, bound) if planes else x
 
 
 def check(g, steps=5, coefficients=(A, B, C), eps=1e-7):
@@ -34,6 +47,11 @@ def check(g, steps=5, coefficients=(A, B, C), eps=1e-7):
     U = HALF_STEP[g.dtype]
     s = min(g.shape[-2:])
     for o, x in zip(out.view(-1, *g.shape[-2:]), g.view(-1, *g.shape[-2:])):
+        if s > 128:
+            want, bound = iterate(x, steps, coefficients, eps, 3 if g.dtype == torch.float32 else 2)
+            off = float((o.double().cpu() - want).norm())
+            assert off <= bound + (U + 2.0 ** -24) * float(want.norm()) + TINY[g.dtype] * want.numel() ** 0.5, (tuple(g.shape), off, bound)
+            continue
         want = iterate(x, steps, coefficients, eps)
         room = (U + 2.0 ** -24) * want.abs() + 4 * s * 2.0 ** -53 * 1.1 * abs(coefficients[0]) ** (2 * steps - 2) * 1.3 + TINY[g.dtype]
         over = (o.double().cpu() - want).abs() - room
@@ -46,6 +64,43 @@ def matrices(batch, m, n, dtype, seed=0, scale=1e-3):
     k = max(1, min(m, n) // 8)
     strong = torch.randn((batch, m, k), generator=gen) / (1 + torch.arange(k)) @ torch.randn((batch, k, n), generator=gen)
     return ((strong + torch.randn((batch, m, n), generator=gen)) * scale).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,m,n", [(1, 129, 129), (2, 300, 260), (3, 140, 1000), (1, 1030, 520), (1, 512, 512), (2, 256, 2049), (1, 3000, 131)])
+def test_long_short_sides(batch, m, n, dtype):
+    check(matrices(batch, m, n, dtype, seed=m + n))
+    gen = torch.Generator().manual_seed(m)
+    check(torch.randn((1, m, n), generator=gen).to(dtype).cuda())  # singular values near each other: nothing grows
+
+
+def test_scales_of_large_matrices():
+    for scale in (1e-30, 1e-6, 1e6, 1e25):
+        check(matrices(2, 300, 200, torch.float32, scale=scale), eps=0.0)
+    check(matrices(1, 300, 200, torch.float16, scale=1.0))
+    for steps in (1, 2):
+        check(matrices(1, 200, 300, torch.bfloat16), steps=steps)
+    g = matrices(4, 200, 190, torch.float32)
+    clean = ops.newton_schulz(g)
+    h = g.clone()
+    h[0] = 0
+    h[1, 3, 4] = float("nan")
+    h[2, 60, 0] = float("inf")
+    out = ops.newton_schulz(h)
+    assert torch.equal(out[0], torch.zeros_like(out[0])) and torch.equal(out[3], clean[3])
+    assert torch.isnan(out[1]).all() and torch.isnan(out[2]).all()
+    want = ops.newton_schulz(g)
+    static = g.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.newton_schulz(static)
+    for k in range(3):
+        static.copy_(g * (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.newton_schulz(static)), k
+    assert torch.equal(want, clean)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
