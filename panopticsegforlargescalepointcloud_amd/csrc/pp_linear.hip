@@ -402,16 +402,19 @@ static int lin_go_wide(const LinArgs& a, int splits, hipStream_t s) {
   return PP_OK;
 }
 
-// rows of a workgroup's tile: large tiles where they fill the chip (256 x 256 tiles of half the chip's units, parts counted)
+// rows of a workgroup's tile.  Two 128 x 128 workgroups on a compute unit run the loop faster than one of 256 x 256 (contraction 4096,
+// 8192 x 1024 results: 66 against 117 us), but a tile costs its start and its epilogue: with contractions below 2048 and enough tiles for
+// the chip the large ones win (1024, 8192 x 4096: 86 against 115 us)
 template <typename T, bool AS, bool BS, int MODE>
-static int lin_tile_rows(const LinArgs& a, int splits) {
-  return lin_wide<T, AS, BS, MODE>(a) && lin_tiles(a.m, a.n, 256) * splits >= 128 ? 256 : 128;
+static int lin_tile_rows(const LinArgs& a) {
+  return lin_wide<T, AS, BS, MODE>(a) && MODE != LIN_PART && a.k < 2048 && lin_tiles(a.m, a.n, 256) >= 192 ? 256 : 128;
 }
 template <typename T, bool AS, bool BS, int MODE>
 static int lin_tile(const LinArgs& a, int splits, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
     if (lin_wide<T, AS, BS, MODE>(a)) {
-      if (lin_tile_rows<T, AS, BS, MODE>(a, splits) == 256) return lin_go_wide<T, AS, BS, MODE, 256, 256, 128, 64>(a, splits, s);
+      if constexpr (MODE != LIN_PART)
+        if (lin_tile_rows<T, AS, BS, MODE>(a) == 256) return lin_go_wide<T, AS, BS, MODE, 256, 256, 128, 64>(a, splits, s);
       return lin_go_wide<T, AS, BS, MODE, 128, 128, 64, 64>(a, splits, s);
     }
   }
@@ -420,12 +423,11 @@ static int lin_tile(const LinArgs& a, int splits, hipStream_t s) {
 }
 
 
-// parts of the weight gradient's contraction: about two workgroups of the tile kernel per compute unit (one of the wide kernel's), at
-// least 256 (512) rows each
+// parts of the weight gradient's contraction: about two workgroups per compute unit, at least 256 rows (wide kernel: 512) each
 static int lin_splits(int64_t n, int cin, int cout, bool wide) {
-  const int64_t tiles = wide ? lin_tiles(cout, cin, 256) : (int64_t)((cout + 127) / 128) * ((cin + (cin > 64 ? 127 : 63)) / (cin > 64 ? 128 : 64));
+  const int64_t tiles = (int64_t)((cout + 127) / 128) * ((cin + (cin > 64 ? 127 : 63)) / (cin > 64 ? 128 : 64));
   const int64_t rows = wide ? 512 : 256;
-  int64_t s = (wide ? 256 : 512) / tiles;
+  int64_t s = 512 / tiles;
   if (s > (n + rows - 1) / rows) s = (n + rows - 1) / rows;
   return s < 1 ? 1 : (int)s;
 }
@@ -509,7 +511,7 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
       a.extra = dy; a.out = z; a.ldo = ldz; a.n_out = (int)ldz;
       a.vo = cout % 8 == 0 && lin_aligned(dy, cout, 16, sizeof(T));
       a.part_bias = db ? part_bias : nullptr;
-      const int rows = lin_tile_rows<T, false, false, LIN_DZ>(a, 1);
+      const int rows = lin_tile_rows<T, false, false, LIN_DZ>(a);
       bias_parts = (n + rows - 1) / rows;
       if ((rc = lin_tile<T, false, false, LIN_DZ>(a, 1, s)) != PP_OK) return rc;
     }

@@ -304,7 +304,8 @@ __global__ __launch_bounds__(256) void k_ns_sum(const double* __restrict__ part,
 // bits) for fp32 ones; a product takes the plane pairs above the last plane's rounding (3, or 6), on k_gemm.  X starts as G 2^e with 2^e
 // the power of two at 1 / (|G| + eps), which needs no rounding (bf16: one plane); the rest of the scale, f in [1, 2), enters the first P.
 // Two planes carry 2^-17 of a value (P and X are rounded to them, each step), three 2^-25: below the half step of the results' type.
-// S and T: lower tiles, the contraction in parts to fill the chip, added in order where S's and P's planes are made.
+// S and T: lower tiles, the contraction in parts to fill the chip, added in order where S's and P's planes are made.  All products take
+// 128 x 128 tiles (X P at 2 x [1024, 4096]: 57 us, 84 us with 256 x 256 ones, which leave half of the chip without work).
 
 struct NsScale {  // per batch element
   float f, pad;
@@ -317,8 +318,18 @@ __global__ __launch_bounds__(256) void k_ns_norm(const T* __restrict__ g, int64_
   __shared__ double red[4];
   const T* p = g + (int64_t)blockIdx.y * count;
   double v = 0.0;
-#pragma unroll 8
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += NS_NORM_PARTS * 256) {
+  constexpr int W = 16 / (int)sizeof(T);
+  const bool vec = count % W == 0 && (uintptr_t)g % 16 == 0;
+  const int64_t vecs = vec ? count / W : 0;
+#pragma unroll 4
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < vecs; i += NS_NORM_PARTS * 256) {
+    float x[W];
+    pp_load<T, W>(p + i * W, x);
+#pragma unroll
+    for (int e = 0; e < W; ++e) v = fma((double)x[e], (double)x[e], v);
+  }
+#pragma unroll 4
+  for (int64_t i = vecs * W + (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += NS_NORM_PARTS * 256) {
     const double x = (double)(float)p[i];
     v = fma(x, x, v);
   }
@@ -640,15 +651,14 @@ static int ns_large(const T* g, int64_t batch, int64_t m, int64_t n, int steps, 
     xe.vec = n % 8 == 0 && (uintptr_t)out % 16 == 0;
     a = GemmArgs{};
     a.m = m; a.n = n; a.k = s;
-    const bool large = ((m + 255) / 256) * ((n + 255) / 256) * batch >= 128;
     if (tall) {
       a.lda = ldx; a.a_batch = m * ldx; a.ldb = ld; a.b_batch = s * ld;
       ns_segments(a, X, xplane, px, w.P, splane, NP, NP);
-      rc = large ? ns_gemm<false, false, 256, 256, 128, 64>(a, xe, batch, st) : ns_gemm<false, false, 128, 128, 64, 64>(a, xe, batch, st);
+      rc = ns_gemm<false, false, 128, 128, 64, 64>(a, xe, batch, st);
     } else {
       a.lda = ld; a.a_batch = s * ld; a.ldb = ldx; a.b_batch = m * ldx;
       ns_segments(a, w.P, splane, NP, X, xplane, px, NP);
-      rc = large ? ns_gemm<false, true, 256, 256, 128, 64>(a, xe, batch, st) : ns_gemm<false, true, 128, 128, 64, 64>(a, xe, batch, st);
+      rc = ns_gemm<false, true, 128, 128, 64, 64>(a, xe, batch, st);
     }
     if (rc != PP_OK) return rc;
   }
