@@ -158,7 +158,7 @@ def test_shapes(n, lengths, c, groups, dtype):
     check(n, lengths, c, groups, dtype, "silu", seed=n + c)
 
 
-@pytest.mark.parametrize("n,b", [(70_001, 3), (140_000, 1), (30_000, 2500), (66_000, 37)])
+@pytest.mark.parametrize("n,b", [(70_001, 3), (140_000, 1), (30_000, 2500), (66_000, 37), (700_000, 5)])
 def test_long_and_many(n, b):
     """elements longer than a chunk, chunks that hold many elements, some of them empty"""
     gen = torch.Generator().manual_seed(n)
@@ -166,6 +166,12 @@ def test_long_and_many(n, b):
     ends = cut + [n]
     lengths = [e - s for s, e in zip([0] + cut, ends)]
     check(n, lengths, 16, 4, torch.float32, "gelu", seed=b)
+
+
+@pytest.mark.parametrize("dtype,c,groups,shuffle", [(torch.bfloat16, 96, 32, False), (torch.float16, 40, 40, True), (torch.bfloat16, 72, 3, False)])
+def test_long_16_bit(dtype, c, groups, shuffle):
+    """more rows than workgroups find room at once; elements with more slots than the second pass adds itself"""
+    check(500_000, [499_000, 0, 900], c, groups, dtype, "silu", seed=c, shuffle=shuffle)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
