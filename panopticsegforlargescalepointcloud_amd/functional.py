@@ -7,18 +7,20 @@ from . import ops
 class _GroupNormActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, offsets, num_groups, weight, bias, eps, act, slope, order):
-        x = x.contiguous()
-        y, mean, rstd = ops.group_norm_fwd(x, offsets, num_groups, weight, bias, eps, act, slope, order)
-        ctx.save_for_backward(x, offsets, weight, bias, mean, rstd, order)
+        with ops.device_of(x):
+            y, stat = ops._group_norm_fwd(x, offsets, num_groups, weight, bias, eps, act, slope, order)
+        ctx.save_for_backward(x, offsets, weight, bias, stat, order)
         ctx.cfg = (num_groups, act, slope)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, offsets, weight, bias, mean, rstd, order = ctx.saved_tensors
+        x, offsets, weight, bias, stat, order = ctx.saved_tensors
         num_groups, act, slope = ctx.cfg
-        dx, dw, db = ops.group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act, slope, order)
+        at = stat.data_ptr()
+        with ops.device_of(x):
+            dx, dw, db = ops._group_norm_bwd(x, dy, offsets, num_groups, weight, bias, at, at + 2 * stat.numel(), act, slope, order)
         return dx, None, None, dw if weight is not None else None, db if bias is not None else None, None, None, None, None
 
 

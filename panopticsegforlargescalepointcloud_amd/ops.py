@@ -3,6 +3,7 @@
 PyTorch is plumbing here (allocation, streams); every op below is one or a few launches of the hand-written
 gfx950 kernels in csrc/.  All tensors must live on a HIP device; there is no CPU path.
 """
+import contextlib
 import ctypes as C
 import functools
 import os
@@ -1244,11 +1245,26 @@ def _on_device_of(fn):
     def call(x, *args, **kwargs):
         if not torch.is_tensor(x) or not x.is_cuda:
             raise _lib.PanopticHipError("%s: the input must be a HIP device tensor (there is no CPU fallback)" % fn.__name__)
-        if x.device.index == torch._C._cuda_getDevice():
+        if x.get_device() == torch._C._cuda_getDevice():
             return fn(x, *args, **kwargs)
         with torch.cuda.device(x.device):
             return fn(x, *args, **kwargs)
     return call
+
+
+_HERE = contextlib.nullcontext()
+
+
+def device_of(x):
+    """context in which the device of x is current; refuses tensors that are not on a HIP device"""
+    if not x.is_cuda:
+        raise _lib.PanopticHipError("the input must be a HIP device tensor (there is no CPU fallback)")
+    return _HERE if x.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(x.device)
+
+
+def _at(t):
+    """device address of a nullable tensor (the small calls of the row operators are paced by the host: plain integers)"""
+    return None if t is None else t.data_ptr()
 
 
 def _row_dtype(x, name):
@@ -1262,11 +1278,11 @@ def _beside(t, x, dtype, shape, name):
     """operand `t` (nullable) of a launch on x: same device, the given element type and shape; contiguous"""
     if t is None:
         return None
-    if t.device != x.device:
-        raise _lib.PanopticHipError("%s is on %s, the input on %s" % (name, t.device, x.device))
     if t.dtype != dtype:
         raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
-    if tuple(t.shape) != tuple(shape):
+    if not t.is_cuda or t.get_device() != x.get_device():
+        raise _lib.PanopticHipError("%s is on %s, the input on %s" % (name, t.device, x.device))
+    if t.shape != shape:  # (a torch.Size is a tuple)
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
     return t if t.is_contiguous() else t.contiguous()
 
@@ -1281,8 +1297,9 @@ def _group_norm_operands(x, offsets, num_groups, weight, bias, order):
         raise ValueError("group_norm: %d groups do not divide %d channels" % (num_groups, c))
     if offsets.dim() != 1 or offsets.shape[0] < 1:
         raise ValueError("group_norm: offsets must be [batch + 1], got %s" % (tuple(offsets.shape),))
-    return (_beside(offsets, x, torch.int64, offsets.shape, "offsets"), _beside(weight, x, torch.float32, (c,), "weight"),
-            _beside(bias, x, torch.float32, (c,), "bias"), _beside(order, x, torch.int64, (n,), "order"))
+    return (x if x.is_contiguous() else x.contiguous(), _beside(offsets, x, torch.int64, offsets.shape, "offsets"),
+            _beside(weight, x, torch.float32, (c,), "weight"), _beside(bias, x, torch.float32, (c,), "bias"),
+            _beside(order, x, torch.int64, (n,), "order"))
 
 
 @_on_device_of
@@ -1291,42 +1308,53 @@ def group_norm_fwd(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, act
     bfloat16 or float16; batch element s owns positions offsets[s] .. offsets[s+1] (int64 [batch + 1]), position p is row order[p]
     (int64 [n]) or row p; rows of no batch element come out as zeros.  weight / bias float32 [c] or None.
     Returns (y, mean, rstd), the statistics float32 [batch, num_groups]."""
+    y, stat = _group_norm_fwd(x, offsets, num_groups, weight, bias, eps, act, slope, order)
+    return y, stat[0], stat[1]
+
+
+def _group_norm_fwd(x, offsets, num_groups, weight, bias, eps, act, slope, order):
+    """(y, [mean, rstd]); x's device is current"""
     lib = _lib.load()
     code = _row_dtype(x, "x")
-    offsets, weight, bias, order = _group_norm_operands(x, offsets, num_groups, weight, bias, order)
-    x = x if x.is_contiguous() else x.contiguous()
+    x, offsets, weight, bias, order = _group_norm_operands(x, offsets, num_groups, weight, bias, order)
     n, c = x.shape
     b = offsets.shape[0] - 1
     y = torch.empty_like(x)
     stat = torch.empty((2, b, num_groups), dtype=torch.float32, device=x.device)
     wsb = lib.pp_group_norm_workspace(n, b, c, num_groups, 0)
     ws = _ws(wsb, x.device)
-    _lib.check(lib.pp_group_norm_fwd(_ptr(x), code, n, c, num_groups, _ptr(offsets), b, _ptr(order), _ptr(weight), _ptr(bias), float(eps),
-                                     int(act), float(slope), _ptr(y), _ptr(stat[0]), _ptr(stat[1]), _ptr(ws), ws.numel(), _stream()),
+    at = stat.data_ptr()
+    _lib.check(lib.pp_group_norm_fwd(x.data_ptr(), code, n, c, num_groups, offsets.data_ptr(), b, _at(order), _at(weight), _at(bias), eps, act,
+                                     slope, y.data_ptr(), at, at + 4 * b * num_groups, ws.data_ptr(), ws.numel(), _stream()),
                "pp_group_norm_fwd")
-    return y, stat[0], stat[1]
+    return y, stat
 
 
 @_on_device_of
 def group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act=0, slope=0.0, order=None):
     """Backward of group_norm_fwd with the statistics it returned: (dx, dweight, dbias), the last two float32 [c]."""
+    shape = (offsets.shape[0] - 1, num_groups)
+    mean = _beside(mean, x, torch.float32, shape, "mean")
+    rstd = _beside(rstd, x, torch.float32, shape, "rstd")
+    return _group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean.data_ptr(), rstd.data_ptr(), act, slope, order)
+
+
+def _group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act, slope, order):
+    """mean, rstd: device addresses of contiguous statistics; x's device is current"""
     lib = _lib.load()
     code = _row_dtype(x, "x")
-    offsets, weight, bias, order = _group_norm_operands(x, offsets, num_groups, weight, bias, order)
-    x = x if x.is_contiguous() else x.contiguous()
+    x, offsets, weight, bias, order = _group_norm_operands(x, offsets, num_groups, weight, bias, order)
     n, c = x.shape
     b = offsets.shape[0] - 1
     dy = _beside(dy, x, x.dtype, (n, c), "dy")
-    mean = _beside(mean, x, torch.float32, (b, num_groups), "mean")
-    rstd = _beside(rstd, x, torch.float32, (b, num_groups), "rstd")
     dx = torch.empty_like(x)
-    dwb = torch.empty((2, c), dtype=torch.float32, device=x.device)
+    dw, db = torch.empty((2, c), dtype=torch.float32, device=x.device).unbind(0)
     wsb = lib.pp_group_norm_workspace(n, b, c, num_groups, 1)
     ws = _ws(wsb, x.device)
-    _lib.check(lib.pp_group_norm_bwd(_ptr(x), _ptr(dy), code, n, c, num_groups, _ptr(offsets), b, _ptr(order), _ptr(weight), _ptr(bias),
-                                     _ptr(mean), _ptr(rstd), int(act), float(slope), _ptr(dx), _ptr(dwb[0]), _ptr(dwb[1]), _ptr(ws),
-                                     ws.numel(), _stream()), "pp_group_norm_bwd")
-    return dx, dwb[0], dwb[1]
+    _lib.check(lib.pp_group_norm_bwd(x.data_ptr(), dy.data_ptr(), code, n, c, num_groups, offsets.data_ptr(), b, _at(order), _at(weight),
+                                     _at(bias), mean, rstd, act, slope, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws.numel(),
+                                     _stream()), "pp_group_norm_bwd")
+    return dx, dw, db
 
 
 def _linear_act_operands(x, weight, bias):
@@ -1347,7 +1375,7 @@ def linear_act_fwd(x, weight, bias=None, act=0, slope=0.0, residual=None):
     cout = weight.shape[0]
     residual = _beside(residual, x, x.dtype, (n, cout), "residual")
     y = torch.empty((n, cout), dtype=x.dtype, device=x.device)
-    _lib.check(lib.pp_linear_act_fwd(_ptr(x), code, n, cin, _ptr(weight), cout, _ptr(bias), int(act), float(slope), _ptr(residual), _ptr(y),
+    _lib.check(lib.pp_linear_act_fwd(_at(x), code, n, cin, _at(weight), cout, _at(bias), act, slope, _at(residual), _at(y),
                                      _stream()), "pp_linear_act_fwd")
     return y
 
@@ -1365,10 +1393,10 @@ def linear_act_bwd(x, dy, weight, bias=None, act=0, slope=0.0, want_input=True, 
     dx = torch.empty_like(x) if want_input else None
     dw = torch.empty_like(weight) if want_weight else None
     db = torch.empty(cout, dtype=x.dtype, device=x.device) if want_bias else None
-    wsb = lib.pp_linear_act_bwd_workspace(code, n, cin, cout, int(act))
+    wsb = lib.pp_linear_act_bwd_workspace(code, n, cin, cout, act)
     ws = _ws(wsb, x.device)
-    _lib.check(lib.pp_linear_act_bwd(_ptr(x), _ptr(dy), code, n, cin, _ptr(weight), cout, _ptr(bias), int(act), float(slope), _ptr(dx),
-                                     _ptr(dw), _ptr(db), _ptr(ws), ws.numel(), _stream()), "pp_linear_act_bwd")
+    _lib.check(lib.pp_linear_act_bwd(_at(x), _at(dy), code, n, cin, _at(weight), cout, _at(bias), act, slope, _at(dx),
+                                     _at(dw), _at(db), _at(ws), ws.numel(), _stream()), "pp_linear_act_bwd")
     return dx, dw, db
 
 
@@ -1395,7 +1423,7 @@ def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7)
     out = torch.empty_like(g)
     wsb = lib.pp_newton_schulz_workspace(batch, m, n)
     ws = _ws(wsb, g.device)
-    _lib.check(lib.pp_newton_schulz(_ptr(g), code, batch, m, n, int(steps), float(a), float(b), float(c), float(eps), _ptr(out), _ptr(ws),
+    _lib.check(lib.pp_newton_schulz(_at(g), code, batch, m, n, int(steps), float(a), float(b), float(c), float(eps), _at(out), _at(ws),
                                     ws.numel(), _stream()), "pp_newton_schulz")
     return out
 
