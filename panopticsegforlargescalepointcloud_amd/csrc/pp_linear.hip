@@ -25,7 +25,6 @@ struct LinArgs {
   float slope;
   void* out;
   int n_out;             // columns written (LIN_DZ pads its rows with zeros up to here)
-  int vo;                // eight neighbouring columns may be stored (and `extra` read) in 16-byte pieces
   float *part, *part_bias;   // LIN_PART: part[splits][m][n]; LIN_DZ: part_bias[row tile][n] (nullable)
   int64_t k_per_split;
 };
@@ -107,6 +106,11 @@ struct LinStage {
             if (r < rows && k + h * W < k1) q = *(const gm_u32x4*)(p + h * W);
             __builtin_memcpy(&v[i][h * W], &q, 16);
           }
+        } else if (r < rows && (k + 8 <= k1 || r + 1 < rows)) {  // eight elements from any address, the next row's among them at the end
+          typename PPVec<T, 8>::type q;
+          __builtin_memcpy(&q, p, sizeof(q));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i][e] = k + e < k1 ? q[e] : (T)0.f;
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[i][e] = r < rows && k + e < k1 ? p[e] : (T)0.f;
@@ -120,6 +124,11 @@ struct LinStage {
             unsigned long long q = 0ull;
             if (k + e < k1 && c < rows) q = *(const unsigned long long*)p;
             __builtin_memcpy(&v[i][e * COLS], &q, 8);
+          } else if (k + e < k1 && c < rows && (c + COLS <= rows || k + e + 1 < k1)) {  // (columns behind `rows`: results that nobody stores)
+            typename PPVec<T, COLS>::type q;
+            __builtin_memcpy(&q, p, sizeof(q));
+#pragma unroll
+            for (int j = 0; j < COLS; ++j) v[i][e * COLS + j] = q[j];
           } else {
 #pragma unroll
             for (int j = 0; j < COLS; ++j) v[i][e * COLS + j] = k + e < k1 && c + j < rows ? p[j] : (T)0.f;
@@ -185,8 +194,10 @@ struct LinEpilogue {
       for (int e = 0; e < 8; ++e) w.x[e] = 0.f;
       if (!a.extra || r >= a.m) return;
       const T* p = (const T*)a.extra + r * a.n + c;
-      if (a.vo) {
-        if (valid > 0) pp_load<T, 8>(p, w.x);
+      if (a.n % 8 == 0) {  // (uniform)
+        if (valid > 0) pp_load_any<T, 8>(p, w.x);
+      } else if (valid == 8) {
+        pp_load_any<T, 8>(p, w.x);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -220,8 +231,10 @@ struct LinEpilogue {
   }
   template <typename O>
   __device__ __forceinline__ void store(O* __restrict__ o, const float (&v)[8], int count) const {
-    if (a.vo) {
-      if (count > 0) pp_store<O, 8>(o, v);
+    if ((MODE == LIN_PART ? a.n : a.n_out) % 8 == 0) {  // (uniform)
+      if (count > 0) pp_store_any<O, 8>(o, v);
+    } else if (count == 8) {
+      pp_store_any<O, 8>(o, v);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -487,7 +500,6 @@ static int lin_forward(const void* x, int64_t n, int cin, const void* w, int cou
                        const void* residual, void* y, hipStream_t s) {
   LinArgs a = lin_base<T>(x, n, cin, w, cout, bias, act, slope);
   a.extra = residual; a.out = y; a.ldo = cout; a.n_out = cout;
-  a.vo = cout % 8 == 0 && lin_aligned(y, cout, 16, sizeof(T)) && lin_aligned(residual, cout, 16, sizeof(T));
   return lin_tile<T, false, false, LIN_FWD>(a, 1, s);
 }
 
@@ -509,8 +521,7 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
     if (n) {
       LinArgs a = lin_base<T>(x, n, cin, w, cout, bias, act, slope);
       a.extra = dy; a.out = z; a.ldo = ldz; a.n_out = (int)ldz;
-      a.vo = cout % 8 == 0 && lin_aligned(dy, cout, 16, sizeof(T));
-      a.part_bias = db ? part_bias : nullptr;
+        a.part_bias = db ? part_bias : nullptr;
       const int rows = lin_tile_rows<T, false, false, LIN_DZ>(a);
       bias_parts = (n + rows - 1) / rows;
       if ((rc = lin_tile<T, false, false, LIN_DZ>(a, 1, s)) != PP_OK) return rc;
@@ -525,7 +536,6 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
     LinArgs a{};
     a.a = dz; a.lda = ldz; a.b = w; a.ldb = cin; a.m = n; a.n = cin; a.k = cout; a.out = dx; a.ldo = cin; a.n_out = cin;
     a.va = lin_aligned(dz, ldz, 16, sizeof(T)); a.vb = lin_aligned(w, cin, 8, sizeof(T));
-    a.vo = cin % 8 == 0 && lin_aligned(dx, cin, 16, sizeof(T));
     if ((rc = lin_tile<T, false, true, LIN_STORE>(a, 1, s)) != PP_OK) return rc;
   }
   if (dw) {
@@ -533,7 +543,6 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
     a.a = dz; a.lda = ldz; a.b = x; a.ldb = cin; a.m = cout; a.n = cin; a.k = n;
     a.va = lin_aligned(dz, ldz, 8, sizeof(T)); a.vb = lin_aligned(x, cin, 8, sizeof(T));
     a.part = part; a.n_out = cin;
-    a.vo = cin % 8 == 0;  // (the parts are fp32 and start on 256 bytes)
     const int splits = lin_wide<T, true, true, LIN_PART>(a) ? p1 : p0;
     a.k_per_split = ((n + splits - 1) / splits + 63) / 64 * 64;
     if ((rc = lin_tile<T, true, true, LIN_PART>(a, splits, s)) != PP_OK) return rc;

@@ -60,6 +60,22 @@ __device__ __forceinline__ float pp_phi(float z) {
 }
 __device__ __forceinline__ float pp_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + pp_exp(-z)); }
 
+// the same at any element's address: the hardware takes 16-byte accesses that start anywhere
+template <typename T, int N>
+__device__ __forceinline__ void pp_load_any(const T* __restrict__ p, float (&v)[N]) {
+  typename PPVec<T, N>::type q;
+  __builtin_memcpy(&q, p, sizeof(q));
+#pragma unroll
+  for (int u = 0; u < N; ++u) v[u] = (float)q[u];
+}
+template <typename T, int N>
+__device__ __forceinline__ void pp_store_any(T* __restrict__ p, const float (&v)[N]) {
+  typename PPVec<T, N>::type q;
+#pragma unroll
+  for (int u = 0; u < N; ++u) q[u] = (T)v[u];
+  __builtin_memcpy(p, &q, sizeof(q));
+}
+
 // y = act(z).  `act` is uniform over a launch: the branch costs one scalar compare per vector of elements
 __device__ __forceinline__ float pp_act1(float z, int act, float slope) {
   switch (act) {

@@ -32,7 +32,7 @@ def test_group_norm_workspace():
     assert lib.pp_group_norm_workspace(-1, 1, 8, 2, 0) == 0
     for n in (0, 1, 65536, 65537, 1 << 33):
         for b in (0, 1, 5000):
-            chunks = min(1024, -(-n // 32))  # a slot per chunk and element that meet, two fp64 sums per group; backward two per channel and chunk
+            chunks = -(-n // max(32, -(-n // 1024)))  # a slot per chunk and element that meet, two fp64 sums per group; backward two per channel and chunk
             assert lib.pp_group_norm_workspace(n, b, 64, 8, 0) >= (chunks + b) * 8 * 16
             assert lib.pp_group_norm_workspace(n, b, 64, 8, 1) >= (chunks + b) * 8 * 16 + chunks * 64 * 16 + b * 8 * 8
 
