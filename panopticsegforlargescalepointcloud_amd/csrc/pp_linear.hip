@@ -106,7 +106,7 @@ struct LinStage {
             if (r < rows && k + h * W < k1) q = *(const gm_u32x4*)(p + h * W);
             __builtin_memcpy(&v[i][h * W], &q, 16);
           }
-        } else if (r < rows && (k + 8 <= k1 || r + 1 < rows)) {  // eight elements from any address, the next row's among them at the end
+        } else if (r < rows && (k + 8 <= k1 || (rows - r) * ld - k >= 8)) {  // eight elements from any address, later rows' among them at the end
           typename PPVec<T, 8>::type q;
           __builtin_memcpy(&q, p, sizeof(q));
 #pragma unroll
@@ -124,7 +124,7 @@ struct LinStage {
             unsigned long long q = 0ull;
             if (k + e < k1 && c < rows) q = *(const unsigned long long*)p;
             __builtin_memcpy(&v[i][e * COLS], &q, 8);
-          } else if (k + e < k1 && c < rows && (c + COLS <= rows || k + e + 1 < k1)) {  // (columns behind `rows`: results that nobody stores)
+          } else if (k + e < k1 && c < rows && (k1 - k - e) * ld - c >= COLS) {  // (columns behind `rows`: results that nobody stores)
             typename PPVec<T, COLS>::type q;
             __builtin_memcpy(&q, p, sizeof(q));
 #pragma unroll

@@ -84,6 +84,14 @@ def test_shapes(n, cin, cout, dtype):
     check(n, cin, cout, dtype, "silu")
 
 
+@pytest.mark.parametrize("n", [1, 2, 3, 130])
+@pytest.mark.parametrize("cin,cout", [(1, 1), (2, 3), (3, 2), (5, 7), (7, 5), (1, 7), (7, 1)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_shorter_than_a_vector(n, cin, cout, dtype):
+    """Rows of fewer than eight elements: what a load takes beside its own row still lies inside the tensor."""
+    check(n, cin, cout, dtype, "silu")
+
+
 @pytest.mark.parametrize("n,cin,cout", [(1, 5, 9), (131, 64, 64), (300, 75, 133), (640, 192, 96), (1025, 40, 260), (5000, 16, 24),
                                         (12_000, 130, 70), (700, 200, 392), (1030, 512, 264), (16_500, 128, 512), (70_000, 256, 512),
                                         (520, 264, 1160)])
