@@ -324,6 +324,235 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
   }
 }
 
+// ---- narrow layers over many rows, 16 bits --------------------------------------------------------------------------------------------------------
+// Up to 160 channels either side the weights fit the LDS, in the order of their fragments, and a wave needs nothing but 16 rows at a time:
+// they go from memory into the registers of the MFMA operand (lane (l & 15, l >> 4): row l & 15, eight neighbouring channels), the next 16
+// are asked for before these are multiplied, no barrier, no LDS traffic but the weights'.  The result has row l & 15 in a lane and four
+// neighbouring columns of every 16, and goes to memory from there.
+// Backward the two layers of the chain meet in the registers: dz is made where z comes out, and the columns 32 t + 4 q + (0 .. 3) and 16 + that
+// of a lane are, as they lie, its eight elements of the operand of dx = dz W over a contraction step of 32 -- in an order of their own, which
+// the fragments of W^T are laid out in.  dz is written for the weight gradient only.
+// Bound: memory (64 -> 64: 16 rows are 4 KB, 580 cycles of a compute unit's share of the bandwidth; 16 MFMAs of 16 cycles on one of four SIMDs,
+// 8 KB of fragments from the LDS; GELU takes another 300 cycles of a SIMD).  1.25 M x 64 -> 64 bf16, GELU and a residual: 144 us, 3.3 TB/s.
+// KB, NB: at least the 32-channel steps of cin and cout; kb, nb: these.
+#define LIN_STREAM_WAVES 8
+struct LinStreamArgs {
+  const void *x, *w, *bias, *extra;  // extra: the residual forward, dy backward; [n, cout]
+  int64_t n, ldz;
+  int cin, cout, kb, nb, act;
+  float slope;
+  void *y, *dx, *dz;                 // y forward; backward dx and dz (nullable both; [n, ldz])
+  float* part_bias;                  // backward [grid][cout], nullable
+};
+
+// `count` elements (0 .. N) at any address; where more than they may be read (`spare`), in one access
+template <typename T, int N>
+__device__ __forceinline__ typename PPVec<T, N>::type lin_take(const T* __restrict__ p, int count, bool spare) {
+  typename PPVec<T, N>::type q;
+#pragma unroll
+  for (int e = 0; e < N; ++e) q[e] = (T)0.f;
+  if (count >= N || (count > 0 && spare)) {
+    __builtin_memcpy(&q, p, sizeof(q));
+#pragma unroll
+    for (int e = 0; e < N; ++e) q[e] = e < count ? q[e] : (T)0.f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < count) q[e] = p[e];
+  }
+  return q;
+}
+template <typename T>
+__device__ __forceinline__ void lin_put4(T* __restrict__ p, const float (&v)[4], int count) {
+  if (count >= 4) {
+    pp_store_any<T, 4>(p, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < count) p[e] = (T)v[e];
+  }
+}
+template <typename T>
+__device__ __forceinline__ LinChunk<T> lin_chunk(typename PPVec<T, 8>::type q) {
+  T v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = q[e];
+  LinChunk<T> c;
+  lin_pack(v, c);
+  return c;
+}
+
+template <typename T, int KB, int NB, bool BACKWARD>
+__global__ __launch_bounds__(64 * LIN_STREAM_WAVES, 2) void k_linear_stream(LinStreamArgs a) {
+  static_assert(sizeof(T) == 2, "one plane");
+  extern __shared__ gm_u32x4 frag[];  // W: [kb][2 nb][64]; backward W^T: [nb][2 kb][64]; bias fp32 [32 nb]
+  typedef typename PPVec<T, 8>::type Vec8;
+  typedef typename PPVec<T, 4>::type Vec4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, q = lane >> 4;
+  const int NT = 2 * a.nb, KT = 2 * a.kb;
+  gm_u32x4* const back = frag + (size_t)a.kb * NT * 64;
+  float* const bias = (float*)(back + (BACKWARD ? (size_t)a.nb * KT * 64 : 0));
+  const T* const w = (const T*)a.w;
+  for (int i = threadIdx.x; i < a.kb * NT * 64; i += blockDim.x) {
+    const int l = i & 63, t = i >> 6, r = t % NT * 16 + (l & 15), k = t / NT * 32 + 8 * (l >> 4);
+    const LinChunk<T> c = lin_chunk<T>(lin_take<T, 8>(w + (int64_t)r * a.cin + k, r < a.cout ? a.cin - k : 0, (a.cout - r) * a.cin - k >= 8));
+    frag[i] = c.p[0];
+  }
+  if (BACKWARD && a.dx)
+    for (int i = threadIdx.x; i < a.nb * KT * 64; i += blockDim.x) {
+      const int l = i & 63, t = i >> 6, m = t % KT * 16 + (l & 15), k = t / KT * 32 + 4 * (l >> 4);
+      Vec8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int o = k + (e < 4 ? e : 12 + e);
+        v[e] = o < a.cout && m < a.cin ? w[(int64_t)o * a.cin + m] : (T)0.f;
+      }
+      const LinChunk<T> c = lin_chunk<T>(v);
+      back[i] = c.p[0];
+    }
+  for (int i = threadIdx.x; i < 32 * a.nb; i += blockDim.x) bias[i] = a.bias && i < a.cout ? (float)((const T*)a.bias)[i] : 0.f;
+  __syncthreads();
+  const int64_t tiles = (a.n + 15) / 16, stride = (int64_t)gridDim.x * LIN_STREAM_WAVES;
+  const bool want_z = !BACKWARD || a.act != PP_ACT_NONE;
+  Vec8 xn[KB];
+  Vec4 en[2 * NB];
+  float zs[BACKWARD ? 2 * NB : 1][4] = {};
+  auto ask = [&](int64_t tile) {
+    const int64_t r = tile * 16 + j;
+    const bool in = r < a.n;
+    const int64_t rows = a.n - r < 8 ? a.n - r : 8;  // (enough to tell whether a vector ends in the tensor)
+    if (want_z) {
+#pragma unroll
+      for (int s = 0; s < KB; ++s)
+        if (s < a.kb) {
+          const int k = 32 * s + 8 * q;
+          xn[s] = lin_take<T, 8>((const T*)a.x + r * a.cin + k, in ? a.cin - k : 0, rows * a.cin - k >= 8);
+        }
+    }
+    if (a.extra) {
+#pragma unroll
+      for (int t = 0; t < 2 * NB; ++t)
+        if (t < NT) {
+          const int c = 16 * t + 4 * q;
+          en[t] = lin_take<T, 4>((const T*)a.extra + r * a.cout + c, in ? a.cout - c : 0, rows * a.cout - c >= 4);
+        }
+    }
+  };
+  int64_t tile = (int64_t)blockIdx.x * LIN_STREAM_WAVES + wave;
+  if (tile < tiles) ask(tile);
+  for (; tile < tiles; tile += stride) {
+    const int64_t r = tile * 16 + j;
+    gm_f32x4 acc[2 * NB];
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t) acc[t] = (gm_f32x4){0.f, 0.f, 0.f, 0.f};
+    Vec4 ex[2 * NB];
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t) ex[t] = en[t];
+    LinChunk<T> xc[KB];
+    if (want_z) {
+#pragma unroll
+      for (int s = 0; s < KB; ++s)
+        if (s < a.kb) xc[s] = lin_chunk<T>(xn[s]);
+    }
+    if (tile + stride < tiles) ask(tile + stride);
+    if (want_z) {
+#pragma unroll
+      for (int s = 0; s < KB; ++s)
+        if (s < a.kb) {
+#pragma unroll
+          for (int t = 0; t < 2 * NB; ++t)
+            if (t < NT) {
+              LinChunk<T> f;
+              f.p[0] = frag[(s * NT + t) * 64 + lane];
+              acc[t] = lin_mma(f, xc[s], acc[t]);
+            }
+        }
+    }
+    if constexpr (!BACKWARD) {
+#pragma unroll
+      for (int t = 0; t < 2 * NB; ++t)
+        if (t < NT) {
+          const int c = 16 * t + 4 * q;
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[t][e] + bias[c + e];
+          pp_act(v, a.act, a.slope);
+          if (a.extra) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += (float)ex[t][e];
+          }
+          lin_put4<T>((T*)a.y + r * a.cout + c, v, r < a.n ? a.cout - c : 0);
+        }
+    } else {
+      LinChunk<T> dc[NB];
+#pragma unroll
+      for (int u = 0; u < NB; ++u)
+        if (u < a.nb) {
+          Vec8 d;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int t = 2 * u + h, c = 16 * t + 4 * q;
+            float z[4], g[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              z[e] = acc[t][e] + bias[c + e];
+              g[e] = (float)ex[t][e];  // (0 behind the last row and column, whatever z is)
+            }
+            pp_dact(g, z, a.act, a.slope);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              g[e] = r < a.n && c + e < a.cout ? g[e] : 0.f;
+              zs[t][e] += g[e];
+              d[4 * h + e] = (T)g[e];
+            }
+            if (a.dz) lin_put4<T>((T*)a.dz + r * a.ldz + c, g, r < a.n ? (int)a.ldz - c : 0);
+          }
+          dc[u] = lin_chunk<T>(d);
+        }
+      if (a.dx) {
+#pragma unroll
+        for (int t = 0; t < 2 * KB; ++t)
+          if (t < KT) {
+            gm_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < NB; ++u)
+              if (u < a.nb) {
+                LinChunk<T> f;
+                f.p[0] = back[(u * KT + t) * 64 + lane];
+                s = lin_mma(f, dc[u], s);
+              }
+            const int c = 16 * t + 4 * q;
+            const float v[4] = {s[0], s[1], s[2], s[3]};
+            lin_put4<T>((T*)a.dx + r * a.cin + c, v, r < a.n ? a.cin - c : 0);
+          }
+      }
+    }
+  }
+  if constexpr (BACKWARD) {
+    if (a.part_bias) {  // a column's rows in a wave, then the waves, in order
+      float* const red = (float*)frag;
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < 2 * NB; ++t)
+        if (t < NT) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = zs[t][e];
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
+            if (j == 0) red[wave * NT * 16 + 16 * t + 4 * q + e] = v;
+          }
+        }
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.cout; c += blockDim.x) {
+        float v = 0.f;
+        for (int k = 0; k < LIN_STREAM_WAVES; ++k) v += red[k * NT * 16 + c];
+        a.part_bias[(int64_t)blockIdx.x * a.cout + c] = v;
+      }
+    }
+  }
+}
+
 // out[i] = sum of part[q][i] over the q of this group (blockIdx.y of gridDim.y), S slices of a block's threads over q, added in order
 template <typename T>
 __global__ __launch_bounds__(256) void k_linear_sum(const float* __restrict__ part, int64_t parts, int64_t n, int S, T* __restrict__ out) {
@@ -446,12 +675,19 @@ static int lin_splits(int64_t n, int cin, int cout, bool wide) {
 }
 #define LIN_SUM_GROUPS 32
 #define LIN_COLUMN_PARTS 64
+#define LIN_STREAM_GRID_MAX 256
 static int64_t lin_ldz(int cout) { return (cout + 7) / 8 * 8; }
+
+// rows of the bias gradient's parts: row tiles (or column parts without an activation), or the narrow kernel's workgroups; room to add them
+static size_t lin_bias_rows(int64_t n, int act) {
+  const size_t tiles = act == PP_ACT_NONE ? LIN_COLUMN_PARTS : (size_t)((n + 127) / 128);
+  return (tiles > LIN_STREAM_GRID_MAX ? tiles : LIN_STREAM_GRID_MAX) + LIN_SUM_GROUPS;
+}
 
 extern "C" size_t pp_linear_act_bwd_workspace(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_t act) {
   if (n < 0 || cin < 1 || cout < 1) return 0;
   const size_t p0 = (size_t)lin_splits(n, cin, cout, false), p1 = (size_t)lin_splits(n, cin, cout, true), parts = p0 > p1 ? p0 : p1;
-  const size_t bias = act == PP_ACT_NONE ? LIN_COLUMN_PARTS : (size_t)((n + 127) / 128) + LIN_SUM_GROUPS;
+  const size_t bias = lin_bias_rows(n, act);
   return pp_align(parts * cout * cin * 4) + pp_align(bias * cout * 4) +
          (act == PP_ACT_NONE ? 0 : pp_align((size_t)n * lin_ldz(cout) * pp_dtype_bytes(dtype))) + 256;
 }
@@ -478,6 +714,49 @@ static int lin_sum(float* part, int64_t parts, int64_t n, T* out, hipStream_t s)
   return PP_OK;
 }
 
+// LDS of the narrow kernel, 0 where the tiles serve: fp32 (its three planes leave room for one workgroup of a compute unit: 300 k x 64 -> 64
+// forward 57 us against 45), a few rows (16 x 160 -> 160 12.3 : 9.3), and widths that fill the tiles.  Measured in bf16, narrow kernel against tiles --
+// forward, GELU and a residual: 1024 x 96 -> 96 8.8 us against 12.7, 300 k x 33 -> 33 32 : 45, 1 M x 96 -> 96 238 : 282, 1 M x 64 -> 64 118 : 134, but 300 k x 96 -> 64
+// 53 : 41, 300 k x 128 -> 128 93 : 77; backward with the activation: 300 k x 96 -> 96 168 : 217, 300 k x 128 -> 64 155 : 157, 300 k x
+// 128 -> 128 293 : 263; backward without one (the tiles need no z there): 300 k x 64 -> 64 105 : 143, but 8192 x 160 -> 160 56 : 47.
+#define LIN_STREAM_ROWS 64
+template <typename T>
+static size_t lin_stream_lds(int64_t n, int cin, int cout, int act, bool backward) {
+  if (sizeof(T) != 2 || cin > 160 || cout > 160 || n < LIN_STREAM_ROWS) return 0;
+  if (cin % 8 == 0 && cout % 8 == 0) {
+    if (!backward && cout % 64 == 0 && (cin > 64 || cout > 64)) return 0;
+    if (backward && act != PP_ACT_NONE && cin % 128 == 0 && cout % 128 == 0) return 0;
+  }
+  if (backward && act == PP_ACT_NONE && n < 65536) return 0;
+  const size_t kb = (cin + 31) / 32, nb = (cout + 31) / 32;
+  return kb * nb * 2048 * (backward ? 2 : 1) + nb * 128;  // (103 KB at most)
+}
+// workgroups: what finds room on the chip at once (two of a compute unit forward, the registers leave one backward)
+static int64_t lin_stream_grid(int64_t n, bool backward) {
+  const int64_t most = backward ? LIN_STREAM_GRID_MAX : 2 * LIN_STREAM_GRID_MAX, tiles = (n + 16 * LIN_STREAM_WAVES - 1) / (16 * LIN_STREAM_WAVES);
+  return tiles < most ? tiles : most;
+}
+template <typename T, int KB, int NB, bool BACKWARD>
+static int lin_stream_go(const LinStreamArgs& a, size_t lds, hipStream_t s) {
+  PP_HIP(hipFuncSetAttribute((const void*)k_linear_stream<T, KB, NB, BACKWARD>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  hipLaunchKernelGGL((k_linear_stream<T, KB, NB, BACKWARD>), dim3((unsigned)lin_stream_grid(a.n, BACKWARD)), dim3(64 * LIN_STREAM_WAVES), lds, s, a);
+  PP_LAUNCH_CHECK();
+  return PP_OK;
+}
+template <typename T, bool BACKWARD>
+static int lin_stream(LinStreamArgs& a, size_t lds, hipStream_t s) {
+  a.kb = (a.cin + 31) / 32;
+  a.nb = (a.cout + 31) / 32;
+#define LIN_BY_NB(KB)                                                    \
+  return a.nb <= 2   ? lin_stream_go<T, KB, 2, BACKWARD>(a, lds, s)      \
+         : a.nb == 3 ? lin_stream_go<T, KB, 3, BACKWARD>(a, lds, s)      \
+                     : lin_stream_go<T, KB, 5, BACKWARD>(a, lds, s);
+  if (a.kb <= 2) LIN_BY_NB(2)
+  if (a.kb == 3) LIN_BY_NB(3)
+  LIN_BY_NB(5)
+#undef LIN_BY_NB
+}
+
 static int lin_check(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_t act) {
   PP_REQUIRE(pp_rows_dtype_ok(dtype), "pp_linear_act: unknown element type");
   PP_REQUIRE(pp_rows_act_ok(act), "pp_linear_act: unknown activation");
@@ -498,6 +777,12 @@ static LinArgs lin_base(const void* x, int64_t n, int cin, const void* w, int co
 template <typename T>
 static int lin_forward(const void* x, int64_t n, int cin, const void* w, int cout, const void* bias, int act, float slope,
                        const void* residual, void* y, hipStream_t s) {
+  if constexpr (sizeof(T) == 2)
+    if (const size_t lds = lin_stream_lds<T>(n, cin, cout, act, false)) {
+      LinStreamArgs a{};
+      a.x = x; a.w = w; a.bias = bias; a.extra = residual; a.n = n; a.cin = cin; a.cout = cout; a.act = act; a.slope = slope; a.y = y;
+      return lin_stream<T, false>(a, lds, s);
+    }
   LinArgs a = lin_base<T>(x, n, cin, w, cout, bias, act, slope);
   a.extra = residual; a.out = y; a.ldo = cout; a.n_out = cout;
   return lin_tile<T, false, false, LIN_FWD>(a, 1, s);
@@ -508,12 +793,27 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
                         void* dx, void* dw, void* db, PPArena& ws, hipStream_t s) {
   const int p0 = lin_splits(n, cin, cout, false), p1 = lin_splits(n, cin, cout, true);
   float* part = ws.take<float>((size_t)(p0 > p1 ? p0 : p1) * cout * cin);
-  float* part_bias = ws.take<float>((act == PP_ACT_NONE ? LIN_COLUMN_PARTS : (size_t)((n + 127) / 128) + LIN_SUM_GROUPS) * cout);
+  float* part_bias = ws.take<float>(lin_bias_rows(n, act) * cout);
   PP_REQUIRE(part && part_bias, "pp_linear_act_bwd: workspace layout");
   const T* dz = (const T*)dy;
   int64_t ldz = cout, bias_parts = 0;
   int rc;
-  if (act != PP_ACT_NONE) {
+  const size_t stream = lin_stream_lds<T>(n, cin, cout, act, true);
+  if (stream) {
+    LinStreamArgs a{};
+    a.x = x; a.w = w; a.bias = bias; a.extra = dy; a.n = n; a.cin = cin; a.cout = cout; a.act = act; a.slope = slope; a.dx = dx;
+    if (act != PP_ACT_NONE && dw) {
+      ldz = a.ldz = lin_ldz(cout);
+      a.dz = ws.take<T>((size_t)n * ldz);
+      PP_REQUIRE(a.dz, "pp_linear_act_bwd: workspace layout");
+      dz = (const T*)a.dz;
+    }
+    a.part_bias = db ? part_bias : nullptr;
+    bias_parts = lin_stream_grid(n, true);
+    if constexpr (sizeof(T) == 2)
+      if (dx || db || a.dz)
+        if ((rc = lin_stream<T, true>(a, stream, s)) != PP_OK) return rc;
+  } else if (act != PP_ACT_NONE) {
     ldz = lin_ldz(cout);
     T* z = ws.take<T>((size_t)n * ldz);
     PP_REQUIRE(z || n == 0, "pp_linear_act_bwd: workspace layout");
@@ -521,7 +821,7 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
     if (n) {
       LinArgs a = lin_base<T>(x, n, cin, w, cout, bias, act, slope);
       a.extra = dy; a.out = z; a.ldo = ldz; a.n_out = (int)ldz;
-        a.part_bias = db ? part_bias : nullptr;
+      a.part_bias = db ? part_bias : nullptr;
       const int rows = lin_tile_rows<T, false, false, LIN_DZ>(a);
       bias_parts = (n + rows - 1) / rows;
       if ((rc = lin_tile<T, false, false, LIN_DZ>(a, 1, s)) != PP_OK) return rc;
@@ -532,7 +832,7 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
                        (n + bias_parts - 1) / bias_parts, part_bias);
     PP_LAUNCH_CHECK();
   }
-  if (dx && n) {
+  if (dx && n && !stream) {
     LinArgs a{};
     a.a = dz; a.lda = ldz; a.b = w; a.ldb = cin; a.m = n; a.n = cin; a.k = cout; a.out = dx; a.ldo = cin; a.n_out = cin;
     a.va = lin_aligned(dz, ldz, 16, sizeof(T)); a.vb = lin_aligned(w, cin, 8, sizeof(T));

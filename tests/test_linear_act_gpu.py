@@ -113,6 +113,40 @@ def test_whole_numbers_are_exact(n, cin, cout, dtype):
     assert torch.equal(dx.cpu(), stored(dy @ w)) and torch.equal(dw.cpu(), stored(dy.t() @ x)) and torch.equal(db.cpu(), stored(dy.sum(0)))
 
 
+@pytest.mark.parametrize("n,cin,cout", [(64, 1, 1), (8193, 3, 5), (9001, 31, 33), (65_537, 64, 64), (8200, 96, 96), (70_001, 75, 133), (65_536, 128, 128), (12_345, 75, 133), (8192, 160, 160),
+                                        (8211, 129, 40), (8299, 40, 129), (20_000, 128, 128), (9000, 7, 160), (9000, 160, 7), (8192, 97, 96)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_narrow_layers_over_many_rows(n, cin, cout, dtype):
+    check(n, cin, cout, dtype, "gelu")
+    check(n, cin, cout, dtype, "none", bias=False, residual=False)
+    g = torch.Generator().manual_seed(n)
+    draw = lambda *s: torch.randint(-3, 4, s, generator=g).double()  # noqa: E731
+    x, w, b, res, dy = draw(n, cin), draw(cout, cin), draw(cout), draw(n, cout), draw(n, cout)
+    up, stored = (lambda t: t.to(dtype).cuda()), (lambda t: t.float().to(dtype).cpu())  # noqa: E731
+    z = x @ w.t() + b
+    assert torch.equal(ops.linear_act_fwd(up(x), up(w), up(b), 1, 0.0, up(res)).cpu(), stored(z.clamp(min=0) + res))
+    dz = dy * (z > 0)
+    for act, d in ((1, dz), (0, dy)):
+        dx, dw, db = ops.linear_act_bwd(up(x), up(dy), up(w), up(b), act)
+        assert torch.equal(dx.cpu(), stored(d @ w)) and torch.equal(dw.cpu(), stored(d.t() @ x)) and torch.equal(db.cpu(), stored(d.sum(0)))
+        for want in ((True, False, False), (False, True, False), (False, False, True)):
+            got = ops.linear_act_bwd(up(x), up(dy), up(w), up(b), act, want_input=want[0], want_weight=want[1], want_bias=want[2])
+            assert all((p is None) != k and (not k or torch.equal(p, q)) for p, q, k in zip(got, (dx, dw, db), want))
+
+
+def test_narrow_layers_keep_non_finite_rows_apart_and_repeat():
+    x, w, b, res, dy = tensors(9000, 75, 133, torch.bfloat16, 11)
+    clean = ops.linear_act_bwd(x, dy, w, b, 3)
+    again = ops.linear_act_bwd(x, dy, w, b, 3)
+    assert all(torch.equal(p, q) for p, q in zip(clean, again))
+    bad = x.clone()
+    bad[7, 3], bad[8999, 74] = float("nan"), float("inf")
+    y, dx = ops.linear_act_fwd(bad, w, b, 3, 0.0, res), ops.linear_act_bwd(bad, dy, w, b, 3)[0]
+    keep = torch.ones(9000, dtype=torch.bool, device="cuda")
+    keep[7] = keep[8999] = False
+    assert torch.equal(y[keep], ops.linear_act_fwd(x, w, b, 3, 0.0, res)[keep]) and torch.equal(dx[keep], clean[0][keep])
+
+
 def test_fp32_keeps_all_bits_of_its_operands():
     """one product per result: fp32 operands of 24 significant bits against a power of two come back unchanged"""
     x = torch.randn(200, 64, device="cuda")
