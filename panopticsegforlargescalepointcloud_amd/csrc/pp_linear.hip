@@ -332,8 +332,9 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
 // Backward the two layers of the chain meet in the registers: dz is made where z comes out, and the columns 32 t + 4 q + (0 .. 3) and 16 + that
 // of a lane are, as they lie, its eight elements of the operand of dx = dz W over a contraction step of 32 -- in an order of their own, which
 // the fragments of W^T are laid out in.  dz is written for the weight gradient only.
-// Bound: memory (64 -> 64: 16 rows are 4 KB, 580 cycles of a compute unit's share of the bandwidth; 16 MFMAs of 16 cycles on one of four SIMDs,
-// 8 KB of fragments from the LDS; GELU takes another 300 cycles of a SIMD).  1.25 M x 64 -> 64 bf16, GELU and a residual: 144 us, 3.3 TB/s.
+// Bound: memory where the activation leaves it (64 -> 64: 16 rows are 4 KB, 580 cycles of a compute unit's share of the bandwidth, against 16
+// MFMAs of 16 cycles and 400 cycles of GELU on one of four SIMDs): no load of the loop is masked but the row's last eight elements, no store
+// but the last columns', and only the tensor's very end is read one by one -- masks of every load took 1.38 times as long at 160 -> 160.
 // KB, NB: at least the 32-channel steps of cin and cout; kb, nb: these.
 #define LIN_STREAM_WAVES 8
 struct LinStreamArgs {
@@ -345,31 +346,27 @@ struct LinStreamArgs {
   float* part_bias;                  // backward [grid][cout], nullable
 };
 
-// `count` elements (0 .. N) at any address; where more than they may be read (`spare`), in one access
+// N elements of a tensor of `total` from any place in it, in one access but at its very end (zeros behind it)
 template <typename T, int N>
-__device__ __forceinline__ typename PPVec<T, N>::type lin_take(const T* __restrict__ p, int count, bool spare) {
+__device__ __forceinline__ typename PPVec<T, N>::type lin_take(const T* __restrict__ base, int64_t at, int64_t total) {
   typename PPVec<T, N>::type q;
-#pragma unroll
-  for (int e = 0; e < N; ++e) q[e] = (T)0.f;
-  if (count >= N || (count > 0 && spare)) {
-    __builtin_memcpy(&q, p, sizeof(q));
-#pragma unroll
-    for (int e = 0; e < N; ++e) q[e] = e < count ? q[e] : (T)0.f;
+  if (at + N <= total) {
+    __builtin_memcpy(&q, base + at, sizeof(q));
   } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (e < count) q[e] = p[e];
+    for (int e = 0; e < N; ++e) q[e] = at + e < total ? base[at + e] : (T)0.f;
   }
   return q;
 }
+// four of a row's 16 columns from `at` on, of which `count` (the same in every lane) exist
 template <typename T>
-__device__ __forceinline__ void lin_put4(T* __restrict__ p, const float (&v)[4], int count) {
-  if (count >= 4) {
+__device__ __forceinline__ void lin_put4(T* __restrict__ p, const float (&v)[4], int count, int at) {
+  if (count >= 16 || at + 4 <= count) {
     pp_store_any<T, 4>(p, v);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (e < count) p[e] = (T)v[e];
+      if (at + e < count) p[e] = (T)v[e];
   }
 }
 template <typename T>
@@ -393,10 +390,40 @@ __global__ __launch_bounds__(64 * LIN_STREAM_WAVES, 2) void k_linear_stream(LinS
   gm_u32x4* const back = frag + (size_t)a.kb * NT * 64;
   float* const bias = (float*)(back + (BACKWARD ? (size_t)a.nb * KT * 64 : 0));
   const T* const w = (const T*)a.w;
+  const int64_t tiles = (a.n + 15) / 16, stride = (int64_t)gridDim.x * LIN_STREAM_WAVES;
+  const bool want_z = !BACKWARD || a.act != PP_ACT_NONE;
+  Vec8 xn[KB];
+  Vec4 en[2 * NB];
+  float zs[BACKWARD ? 2 * NB : 1][4] = {};
+  const int64_t x_end = a.n * a.cin, e_end = a.n * a.cout;
+  gm_u32x4 tail;  // what of the last step's eight elements lies in the row
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int left = a.cin - 32 * (a.kb - 1) - 8 * q - 2 * e;
+    tail[e] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+  }
+  // (a row behind the last reads the last one and stores nothing; columns behind the last are dropped)
+  auto ask = [&](int64_t tile) {
+    const int64_t r = tile * 16 + j < a.n ? tile * 16 + j : a.n - 1;
+    if (want_z) {
+#pragma unroll
+      for (int s = 0; s < KB; ++s)
+        if (s < a.kb) xn[s] = lin_take<T, 8>((const T*)a.x, r * a.cin + 32 * s + 8 * q, x_end);
+    }
+    if (a.extra) {
+#pragma unroll
+      for (int t = 0; t < 2 * NB; ++t)
+        if (t < NT) en[t] = lin_take<T, 4>((const T*)a.extra, r * a.cout + 16 * t + 4 * q, e_end);
+    }
+  };
+  int64_t tile = (int64_t)blockIdx.x * LIN_STREAM_WAVES + wave;
+  if (!BACKWARD && tile < tiles) ask(tile);
   for (int i = threadIdx.x; i < a.kb * NT * 64; i += blockDim.x) {
     const int l = i & 63, t = i >> 6, r = t % NT * 16 + (l & 15), k = t / NT * 32 + 8 * (l >> 4);
-    const LinChunk<T> c = lin_chunk<T>(lin_take<T, 8>(w + (int64_t)r * a.cin + k, r < a.cout ? a.cin - k : 0, (a.cout - r) * a.cin - k >= 8));
-    frag[i] = c.p[0];
+    Vec8 v = lin_take<T, 8>(w, r < a.cout ? r * a.cin + k : a.cout * a.cin, a.cout * a.cin);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = k + e < a.cin ? v[e] : (T)0.f;
+    frag[i] = lin_chunk<T>(v).p[0];
   }
   if (BACKWARD && a.dx)
     for (int i = threadIdx.x; i < a.nb * KT * 64; i += blockDim.x) {
@@ -407,39 +434,11 @@ __global__ __launch_bounds__(64 * LIN_STREAM_WAVES, 2) void k_linear_stream(LinS
         const int o = k + (e < 4 ? e : 12 + e);
         v[e] = o < a.cout && m < a.cin ? w[(int64_t)o * a.cin + m] : (T)0.f;
       }
-      const LinChunk<T> c = lin_chunk<T>(v);
-      back[i] = c.p[0];
+      back[i] = lin_chunk<T>(v).p[0];
     }
   for (int i = threadIdx.x; i < 32 * a.nb; i += blockDim.x) bias[i] = a.bias && i < a.cout ? (float)((const T*)a.bias)[i] : 0.f;
   __syncthreads();
-  const int64_t tiles = (a.n + 15) / 16, stride = (int64_t)gridDim.x * LIN_STREAM_WAVES;
-  const bool want_z = !BACKWARD || a.act != PP_ACT_NONE;
-  Vec8 xn[KB];
-  Vec4 en[2 * NB];
-  float zs[BACKWARD ? 2 * NB : 1][4] = {};
-  auto ask = [&](int64_t tile) {
-    const int64_t r = tile * 16 + j;
-    const bool in = r < a.n;
-    const int64_t rows = a.n - r < 8 ? a.n - r : 8;  // (enough to tell whether a vector ends in the tensor)
-    if (want_z) {
-#pragma unroll
-      for (int s = 0; s < KB; ++s)
-        if (s < a.kb) {
-          const int k = 32 * s + 8 * q;
-          xn[s] = lin_take<T, 8>((const T*)a.x + r * a.cin + k, in ? a.cin - k : 0, rows * a.cin - k >= 8);
-        }
-    }
-    if (a.extra) {
-#pragma unroll
-      for (int t = 0; t < 2 * NB; ++t)
-        if (t < NT) {
-          const int c = 16 * t + 4 * q;
-          en[t] = lin_take<T, 4>((const T*)a.extra + r * a.cout + c, in ? a.cout - c : 0, rows * a.cout - c >= 4);
-        }
-    }
-  };
-  int64_t tile = (int64_t)blockIdx.x * LIN_STREAM_WAVES + wave;
-  if (tile < tiles) ask(tile);
+  if (BACKWARD && tile < tiles) ask(tile);
   for (; tile < tiles; tile += stride) {
     const int64_t r = tile * 16 + j;
     gm_f32x4 acc[2 * NB];
@@ -452,7 +451,10 @@ __global__ __launch_bounds__(64 * LIN_STREAM_WAVES, 2) void k_linear_stream(LinS
     if (want_z) {
 #pragma unroll
       for (int s = 0; s < KB; ++s)
-        if (s < a.kb) xc[s] = lin_chunk<T>(xn[s]);
+        if (s < a.kb) {
+          xc[s] = lin_chunk<T>(xn[s]);
+          if (s == a.kb - 1) xc[s].p[0] &= tail;
+        }
     }
     if (tile + stride < tiles) ask(tile + stride);
     if (want_z) {
@@ -481,7 +483,7 @@ __global__ __launch_bounds__(64 * LIN_STREAM_WAVES, 2) void k_linear_stream(LinS
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] += (float)ex[t][e];
           }
-          lin_put4<T>((T*)a.y + r * a.cout + c, v, r < a.n ? a.cout - c : 0);
+          if (r < a.n) lin_put4<T>((T*)a.y + r * a.cout + c, v, a.cout - 16 * t, 4 * q);
         }
     } else {
       LinChunk<T> dc[NB];
@@ -505,7 +507,7 @@ __global__ __launch_bounds__(64 * LIN_STREAM_WAVES, 2) void k_linear_stream(LinS
               zs[t][e] += g[e];
               d[4 * h + e] = (T)g[e];
             }
-            if (a.dz) lin_put4<T>((T*)a.dz + r * a.ldz + c, g, r < a.n ? (int)a.ldz - c : 0);
+            if (a.dz && r < a.n) lin_put4<T>((T*)a.dz + r * a.ldz + c, g, (int)a.ldz - 16 * t, 4 * q);
           }
           dc[u] = lin_chunk<T>(d);
         }
@@ -523,7 +525,7 @@ __global__ __launch_bounds__(64 * LIN_STREAM_WAVES, 2) void k_linear_stream(LinS
               }
             const int c = 16 * t + 4 * q;
             const float v[4] = {s[0], s[1], s[2], s[3]};
-            lin_put4<T>((T*)a.dx + r * a.cin + c, v, r < a.n ? a.cin - c : 0);
+            if (r < a.n) lin_put4<T>((T*)a.dx + r * a.cin + c, v, a.cin - 16 * t, 4 * q);
           }
       }
     }
@@ -715,17 +717,19 @@ static int lin_sum(float* part, int64_t parts, int64_t n, T* out, hipStream_t s)
 }
 
 // LDS of the narrow kernel, 0 where the tiles serve: fp32 (its three planes leave room for one workgroup of a compute unit: 300 k x 64 -> 64
-// forward 57 us against 45), a few rows (16 x 160 -> 160 12.3 : 9.3), and widths that fill the tiles.  Measured in bf16, narrow kernel against tiles --
-// forward, GELU and a residual: 1024 x 96 -> 96 8.8 us against 12.7, 300 k x 33 -> 33 32 : 45, 1 M x 96 -> 96 238 : 282, 1 M x 64 -> 64 118 : 134, but 300 k x 96 -> 64
-// 53 : 41, 300 k x 128 -> 128 93 : 77; backward with the activation: 300 k x 96 -> 96 168 : 217, 300 k x 128 -> 64 155 : 157, 300 k x
-// 128 -> 128 293 : 263; backward without one (the tiles need no z there): 300 k x 64 -> 64 105 : 143, but 8192 x 160 -> 160 56 : 47.
+// forward 57 us against 45), fewer than 64 rows (16 x 160 -> 160 forward 12.3 : 9.3), and aligned widths that fill the tiles' columns --
+// forward, where the rows are wide against the results (fp16 300 k x 128 -> 64 48 us against 38; 96 -> 64 31 : 38, 96 -> 128 56 : 67), or
+// where the tiles fill the chip and the waves here have no second 16 rows to read ahead (65536 x 128 -> 128 25 : 17; 8192 rows 11.4 : 11.3,
+// 300 k 65 : 68); backward without an activation and with few rows, where the tiles need no z and more workgroups share the weights (8192 x
+// 64 -> 128 36 : 30, 65536 57 : 59).  Else this one: 300 k x 160 -> 160 89 : 156 forward, 434 : 608 backward with the activation; 75 -> 133 74 : 167
+// and 255 : 415; 1024 x 96 -> 96 bf16 forward 8.0 : 12.7; 1 k .. 65 k x 160 -> 160 backward 0.95 .. 1.24 of the tiles' speed.
 #define LIN_STREAM_ROWS 64
 template <typename T>
 static size_t lin_stream_lds(int64_t n, int cin, int cout, int act, bool backward) {
   if (sizeof(T) != 2 || cin > 160 || cout > 160 || n < LIN_STREAM_ROWS) return 0;
-  if (cin % 8 == 0 && cout % 8 == 0) {
-    if (!backward && cout % 64 == 0 && (cin > 64 || cout > 64)) return 0;
-    if (backward && act != PP_ACT_NONE && cin % 128 == 0 && cout % 128 == 0) return 0;
+  if (!backward && cin % 8 == 0 && cout % 64 == 0) {
+    if (cin > 96 && cout <= 64) return 0;
+    if ((cin > 64 || cout > 64) && n >= 32768 && n < 131072) return 0;
   }
   if (backward && act == PP_ACT_NONE && n < 65536) return 0;
   const size_t kb = (cin + 31) / 32, nb = (cout + 31) / 32;
