@@ -409,9 +409,9 @@ int pp_group_norm_bwd(const void* x, const void* dy, int32_t dtype, int64_t n, i
  * Linear layer of any width with bias, activation and residual in its epilogue, and its gradients   (beside pp_linear_rows: <= 32
  * channels, fp32)
  * x [n,cin], weight [cout,cin], bias [cout] (nullable), residual [n,cout] (nullable), y [n,cout], all of element type `dtype`.
- * fwd: y = act(x weight^T + bias) + residual, fp32 accumulation, one rounding.
- * bwd: dz = dy act'(x weight^T + bias) (recomputed; rounded to the element type), dx = dz weight, dweight = dz^T x, dbias = column
- *      sums of dz; each of dx, dweight, dbias nullable.  The residual's gradient is dy itself.  Results repeat bit for bit.
+ * Up to 2^31 - 1 rows, 2^20 channels.  fwd: y = act(x weight^T + bias) + residual, fp32 accumulation, one rounding.
+ * bwd: dz = dy act'(x weight^T + bias) (recomputed), dbias = column sums of it; then rounded to the element type: dx = dz weight,
+ *      dweight = dz^T x; each of dx, dweight, dbias nullable.  The residual's gradient is dy itself.  Results repeat bit for bit.
  * ---------------------------------------------------------------------------------------------- */
 int pp_linear_act_fwd(const void* x, int32_t dtype, int64_t n, int32_t cin, const void* weight, int32_t cout, const void* bias,
                       int32_t act, float slope, const void* residual, void* y, pp_stream_t stream);

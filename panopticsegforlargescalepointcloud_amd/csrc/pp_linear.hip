@@ -735,7 +735,7 @@ static size_t lin_stream_lds(int64_t n, int cin, int cout, int act, bool backwar
   const size_t kb = (cin + 31) / 32, nb = (cout + 31) / 32;
   return kb * nb * 2048 * (backward ? 2 : 1) + nb * 128;  // (103 KB at most)
 }
-// workgroups: what finds room on the chip at once (two of a compute unit forward, the registers leave one backward)
+// workgroups: what finds room on the chip at once (two of a compute unit forward, up to 96 channels; the registers leave one backward)
 static int64_t lin_stream_grid(int64_t n, bool backward) {
   const int64_t most = backward ? LIN_STREAM_GRID_MAX : 2 * LIN_STREAM_GRID_MAX, tiles = (n + 16 * LIN_STREAM_WAVES - 1) / (16 * LIN_STREAM_WAVES);
   return tiles < most ? tiles : most;
@@ -765,7 +765,7 @@ static int lin_check(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_
   PP_REQUIRE(pp_rows_dtype_ok(dtype), "pp_linear_act: unknown element type");
   PP_REQUIRE(pp_rows_act_ok(act), "pp_linear_act: unknown activation");
   PP_REQUIRE(cin >= 1 && cin <= (1 << 20) && cout >= 1 && cout <= (1 << 20), "pp_linear_act: channels out of range");
-  PP_REQUIRE(n >= 0 && n <= ((int64_t)1 << 36), "pp_linear_act: rows out of range");
+  PP_REQUIRE(n >= 0 && n < ((int64_t)1 << 31), "pp_linear_act: rows out of range");  // (a launch has less than 2^32 threads)
   return PP_OK;
 }
 

@@ -1366,7 +1366,7 @@ def _linear_act_operands(x, weight, bias):
 @_on_device_of
 def linear_act_fwd(x, weight, bias=None, act=0, slope=0.0, residual=None):
     """y = act(x W^T + bias) + residual in one launch (csrc/pp_linear.hip): x [n, cin], weight [cout, cin], bias [cout], residual
-    [n, cout], all of one type (float32, bfloat16, float16); any width and any number of rows."""
+    [n, cout], all of one type (float32, bfloat16, float16); any width, up to 2^31 - 1 rows."""
     lib = _lib.load()
     code = _row_dtype(x, "x")
     weight, bias = _linear_act_operands(x, weight, bias)

@@ -58,7 +58,7 @@ def linear(**kw):
 
 
 @pytest.mark.parametrize("kw", [{"dtype": 3}, {"act": 5}, {"cin": 0}, {"cout": 0}, {"cout": (1 << 20) + 1}, {"n": -1}, {"w": None},
-                                {"x": None}, {"y": None}])
+                                {"x": None}, {"y": None}, {"n": 1 << 31}])
 def test_linear_act_entry_refuses(kw):
     assert linear(**kw) == INVALID
 
