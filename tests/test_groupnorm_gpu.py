@@ -299,6 +299,34 @@ def test_bad_offsets_and_orders_touch_nothing_outside():
     assert torch.isfinite(y[keep]).all()
 
 
+@pytest.mark.parametrize("dtype,shuffled", [(torch.bfloat16, False), (torch.float32, True)])
+def test_offsets_past_32_bits(dtype, shuffled):
+    """More than 2^31 elements: batch elements with the same rows have the same results, wherever they lie."""
+    blocks, c = 4200, 128
+    g = torch.Generator().manual_seed(3)
+    x, dy = torch.randn((4096, c), generator=g).to(dtype).cuda(), torch.randn((4096, c), generator=g).to(dtype).cuda()
+    w, b = torch.rand(c, generator=g).cuda() + 0.5, torch.randn(c, generator=g).cuda()
+    off = torch.arange(blocks + 1, device="cuda") * 4096
+    order = torch.arange(blocks * 4096, device="cuda").flip(0).contiguous() if shuffled else None  # (elements from the end, rows backwards)
+    big, big_dy = x.repeat(blocks, 1), dy.repeat(blocks, 1)
+    assert big.numel() > 2 ** 31
+    y, mean, rstd = ops.group_norm_fwd(big, off, 8, w, b, 1e-5, 3, 0.0, order)
+    one, m1, r1 = ops.group_norm_fwd(x, off[:2], 8, w, b, 1e-5, 3)
+    # sums in 64 bits: the statistics differ by a rounding to fp32 at most, which moves a result by a few more
+    assert float((mean - m1).abs().max()) <= 2 ** -23 and float((rstd / r1 - 1).abs().max()) <= 2 ** -22
+    tol = dict(rtol=2 * torch.finfo(dtype).eps, atol=2 ** -18)
+    torch.testing.assert_close(y.view(blocks, 4096, c)[0], one, **tol)
+    dx, dw, db = ops.group_norm_bwd(big, big_dy, off, 8, w, b, mean, rstd, 3, 0.0, order)
+    dx1, dw1, db1 = ops.group_norm_bwd(x, dy, off[:2], 8, w, b, m1, r1, 3)
+    torch.testing.assert_close(dx.view(blocks, 4096, c)[0], dx1, **tol)
+    for part in (y, dx):
+        part = part.view(blocks, 4096, c)
+        for i in range(1, blocks, 600):
+            torch.testing.assert_close(part[i:i + 600], part[:1].expand(min(600, blocks - i), -1, -1), **tol)
+    for got, want in ((dw, dw1), (db, db1)):
+        assert float((got.double() / blocks - want.double()).abs().max()) <= 2 ** -20 * float(want.abs().max())
+
+
 def test_refusals():
     x = torch.randn((10, 12), device="cuda")
     off = torch.tensor([0, 10], device="cuda")

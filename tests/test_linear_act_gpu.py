@@ -252,6 +252,30 @@ def test_repeats_stream_and_graph():
         assert all(torch.equal(p, q) for p, q in zip(by, ops.linear_act_bwd(sx, sdy, w, b, 3))), k
 
 
+@pytest.mark.parametrize("dtype,blocks,cin,cout", [(torch.bfloat16, 4200, 128, 8), (torch.float16, 4200, 8, 128), (torch.bfloat16, 4200, 128, 128),
+                                                  (torch.float32, 4200, 128, 8), (torch.bfloat16, 530, 1024, 256)])
+def test_offsets_past_32_bits(dtype, blocks, cin, cout):
+    """More than 2^31 elements: 4096 rows of small whole numbers again and again give the same results again and again.  Every sum is a
+    whole number below 2^24 (weight gradient: blocks times one block's, which is below 2^10), so fp32 holds it whatever the order."""
+    g = torch.Generator().manual_seed(blocks + cin)
+    draw = lambda *s: torch.randint(-1, 2, s, generator=g).double()  # noqa: E731
+    x, w, b, dy = draw(4096, cin), draw(cout, cin), draw(cout), draw(4096, cout)
+    up = lambda t: t.to(dtype).cuda()  # noqa: E731
+    same = lambda t, want: bool((t.view(blocks, 4096, -1) == up(want)).all())  # noqa: E731
+    many = lambda t: up(t).repeat(blocks, 1)  # noqa: E731
+    assert max(cin, cout) * 4096 * blocks > 2 ** 31
+    z = x @ w.t() + b
+    big, big_dy = many(x), many(dy)
+    assert same(ops.linear_act_fwd(big, up(w), up(b), 1), z.clamp(min=0))
+    for act, dz in ((1, dy * (z > 0)), (0, dy)):
+        dw_one = dz.t() @ x
+        assert dw_one.abs().max() < 2 ** 10 and dz.sum(0).abs().max() < 2 ** 10
+        dx, dw, db = ops.linear_act_bwd(big, big_dy, up(w), up(b), act)
+        assert same(dx, dz @ w)
+        assert torch.equal(dw, up((dw_one * blocks).float())) and torch.equal(db, up((dz.sum(0) * blocks).float()))
+        del dx
+
+
 def test_refusals():
     x, w, b, res, dy = tensors(10, 12, 8, torch.float32, 6)
     for args, err in (((x, w[:, :11].contiguous()), ValueError), ((x.view(-1), w), ValueError), ((x, w.half()), TypeError),

@@ -172,6 +172,31 @@ def test_batch_strides_repeats_stream_and_graph():
         assert torch.equal(out, ops.newton_schulz(static)), k
 
 
+@pytest.mark.parametrize("dtype,batch,m,n", [(torch.bfloat16, 6, 4_000_000, 96), (torch.bfloat16, 3, 160, 4_194_304)])
+def test_offsets_past_32_bits(dtype, batch, m, n):
+    """More than 2^31 elements: the same matrix at the start and at the end of a batch; diagonals of one value below each other, so
+    that the result is a multiple of it."""
+    s, l = min(m, n), max(m, n)
+    one = torch.zeros((l, s), dtype=dtype, device="cuda")
+    rows = torch.arange(l // s * s, device="cuda")
+    one[rows, rows % s] = 0.5
+    g = (one if m > n else one.t()).repeat(batch, 1, 1)
+    assert g.numel() > 2 ** 30 and (batch - 1) * m * n * g.element_size() > 2 ** 31
+    out = ops.newton_schulz(g)
+    assert all(torch.equal(out[0], out[i]) for i in range(1, batch))
+    # columns of one length, orthogonal: all singular values are one number t = 1 / sqrt(s) of the norm, and so are they in the result
+    t = s ** -0.5
+    for _ in range(5):
+        a, b, c = ops.NEWTON_SCHULZ_COEFFICIENTS
+        t = a * t + b * t ** 3 + c * t ** 5
+    value = t / (l // s) ** 0.5  # every column has l // s entries
+    have = out[0] if m > n else out[0].t()
+    # bf16's half step; two planes of 8 bits leave 2^-16 of an operand, three operands a step, of which the later steps make no more than
+    # |t f'(t) / f(t)| <= 4 times as much: below 2^-8 in all
+    assert float((have[rows, rows % s].double() / value - 1).abs().max()) <= 2 ** -7
+    assert int(have.count_nonzero()) == rows.numel()
+
+
 def test_refusals():
     g = torch.randn(8, 8, device="cuda")
     for bad, err in ((torch.zeros(8, device="cuda"), ValueError), (torch.zeros(2, 2, 2, 2, device="cuda"), ValueError),
