@@ -106,34 +106,53 @@ struct LinStage {
             if (r < rows && k + h * W < k1) q = *(const gm_u32x4*)(p + h * W);
             __builtin_memcpy(&v[i][h * W], &q, 16);
           }
-        } else if (r < rows && (k + 8 <= k1 || (rows - r) * ld - k >= 8)) {  // eight elements from any address, later rows' among them at the end
-          typename PPVec<T, 8>::type q;
-          __builtin_memcpy(&q, p, sizeof(q));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[i][e] = k + e < k1 ? q[e] : (T)0.f;
         } else {
+          // eight elements from any address, later rows' among them at the end (taken out below, when all loads are on their way)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[i][e] = r < rows && k + e < k1 ? p[e] : (T)0.f;
+          for (int e = 0; e < 8; ++e) v[i][e] = (T)0.f;
+          if (r < rows && (rows - r) * ld - k >= 8) {
+            __builtin_memcpy(&v[i][0], p, 8 * sizeof(T));
+          } else if (r < rows) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (k + e < k1) v[i][e] = p[e];
+          }
         }
       } else {
         const int64_t c = row0 + (unit % (ROWS / COLS)) * COLS, k = k0 + unit / (ROWS / COLS) * 8;
+        const T* p = src + k * ld + c;
+        if (vec) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const T* p = src + (k + e) * ld + c;
-          if (vec) {
+          for (int e = 0; e < 8; ++e) {
             unsigned long long q = 0ull;
-            if (k + e < k1 && c < rows) q = *(const unsigned long long*)p;
+            if (k + e < k1 && c < rows) q = *(const unsigned long long*)(p + e * ld);
             __builtin_memcpy(&v[i][e * COLS], &q, 8);
-          } else if (k + e < k1 && c < rows && (k1 - k - e) * ld - c >= COLS) {  // (columns behind `rows`: results that nobody stores)
-            typename PPVec<T, COLS>::type q;
-            __builtin_memcpy(&q, p, sizeof(q));
+          }
+        } else {
+          // (columns behind `rows`: results that nobody stores.)  One branch around the eight loads: a branch to each, and they wait for
+          // one another (weight gradient of 50 k rows, 75 and 133 wide, fp16: 36 us, 19.6 us now)
 #pragma unroll
-            for (int j = 0; j < COLS; ++j) v[i][e * COLS + j] = q[j];
-          } else {
+          for (int e = 0; e < 8 * COLS; ++e) v[i][e] = (T)0.f;
+          if (c < rows && (k1 - k - 7) * ld - c >= COLS) {
 #pragma unroll
-            for (int j = 0; j < COLS; ++j) v[i][e * COLS + j] = k + e < k1 && c + j < rows ? p[j] : (T)0.f;
+            for (int e = 0; e < 8; ++e) __builtin_memcpy(&v[i][e * COLS], p + e * ld, COLS * sizeof(T));
+          } else if (c < rows) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+              for (int j = 0; j < COLS; ++j)
+                if (k + e < k1 && c + j < rows) v[i][e * COLS + j] = p[e * ld + j];
           }
         }
+      }
+    }
+    if (!STRIDED && !vec) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int unit = threadIdx.x + 256 * i;
+        const int64_t k = k0 + (unit % CH) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = k + e < k1 ? v[i][e] : (T)0.f;
       }
     }
   }
@@ -720,9 +739,9 @@ static int lin_sum(float* part, int64_t parts, int64_t n, T* out, hipStream_t s)
 // forward 57 us against 45), fewer than 64 rows (16 x 160 -> 160 forward 12.3 : 9.3), and aligned widths that fill the tiles' columns --
 // forward, where the rows are wide against the results (fp16 300 k x 128 -> 64 48 us against 38; 96 -> 64 31 : 38, 96 -> 128 56 : 67), or
 // where the tiles fill the chip and the waves here have no second 16 rows to read ahead (65536 x 128 -> 128 25 : 17; 8192 rows 11.4 : 11.3,
-// 300 k 65 : 68); backward without an activation and with few rows, where the tiles need no z and more workgroups share the weights (8192 x
-// 64 -> 128 36 : 30, 65536 57 : 59).  Else this one: 300 k x 160 -> 160 89 : 156 forward, 434 : 608 backward with the activation; 75 -> 133 74 : 167
-// and 255 : 415; 1024 x 96 -> 96 bf16 forward 8.0 : 12.7; 1 k .. 65 k x 160 -> 160 backward 0.95 .. 1.24 of the tiles' speed.
+// 300 k 65 : 68); backward with few rows, where more workgroups share the tiles, and no z is needed (8192 x 64 -> 128 36 : 30, 65536 57 : 59) or
+// the weights are large (8192 x 160 -> 160 48 : 42, 65536 82 : 92).  Else this one: 300 k x 160 -> 160 87 : 128 forward, 246 : 345 backward with
+// the activation; 75 -> 133 74 : 155 and 183 : 300; 1024 x 96 -> 96 forward 7.1 : 10.1, backward 29 : 32 (160 -> 160 forward 11.9 : 11.0).
 #define LIN_STREAM_ROWS 64
 template <typename T>
 static size_t lin_stream_lds(int64_t n, int cin, int cout, int act, bool backward) {
@@ -731,7 +750,7 @@ static size_t lin_stream_lds(int64_t n, int cin, int cout, int act, bool backwar
     if (cin > 96 && cout <= 64) return 0;
     if ((cin > 64 || cout > 64) && n >= 32768 && n < 131072) return 0;
   }
-  if (backward && act == PP_ACT_NONE && n < 65536) return 0;
+  if (backward && n < 65536 && (act == PP_ACT_NONE || (cin > 128 && cout > 128))) return 0;
   const size_t kb = (cin + 31) / 32, nb = (cout + 31) / 32;
   return kb * nb * 2048 * (backward ? 2 : 1) + nb * 128;  // (103 KB at most)
 }
