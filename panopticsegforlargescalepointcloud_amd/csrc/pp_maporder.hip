@@ -306,13 +306,11 @@ __global__ __launch_bounds__(NT) void k_window_sort_big(const uint32_t* __restri
   }
 }
 
-// 4096 is NOT served (round 6).  k_window_sort<4096> -- the one instantiation with 512 threads = 8 waves per workgroup, 72 VGPRs and
-// 24.3 KiB of LDS -- returns orders whose rows leave their window (16-bit row indices overwritten by keys: a scatter position
-// beyond the window) in 20 - 34 of 40 launches when k_kernel_map_bi or k_map_permute_big runs on ANOTHER stream at the same time, and
-// never alone, never beside the other sorts, the coarsening kernels or a fill, while 1024 / 2048 / 8192 / 16384 / 32768 pass 40 of 40
-// under the same load (profiles/sort_race_probe.py -> profiles/r06_sort_race_probe.txt; rocgdb put the bench's memory faults of the
-// window sweeps of rounds 4 and 6 into the k_map_permute_win<4096> launch that consumed such an order).  The ISA was read barrier by
-// barrier without finding a missing one; until the cause is known the size is refused instead of being left as a trap.
+// 4096 is NOT served.  k_window_sort<4096> -- the one instantiation with 512 threads = 8 waves per workgroup, 72 VGPRs and 24.3 KiB of
+// LDS -- returned orders whose rows left their window (16-bit row indices overwritten by keys) while k_kernel_map_bi or
+// k_map_permute_big ran on another stream, and the k_map_permute_win<4096> launch that took such an order read out of range.  Never
+// alone, and no other window did.  The cause is not known (reading it barrier by barrier shows no missing one), so the size is refused
+// and stays off the GPU.
 static bool map_window_ok(int w) { return w >= 1024 && w <= 32768 && (w & (w - 1)) == 0 && w != 4096; }
 extern "C" int32_t pp_map_window(void) { return g_window; }
 extern "C" int pp_map_set_window(int32_t window) {
