@@ -1,0 +1,65 @@
+"""The row operators (group norm, linear layer, Newton-Schulz) where values, sizes or calls are at the edge of what they take, against
+64 bits.  u = 2^-24; HALF_STEP is half a step of the stored type."""
+import math
+
+import pytest
+import torch
+
+from panopticsegforlargescalepointcloud_amd import ops
+from test_groupnorm_gpu import HALF_STEP, TINY, act64, dact64
+
+pytestmark = pytest.mark.gpu
+
+u = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def far_values(dtype):
+    return torch.tensor([-5.5, -6.0, -6.5, -7.0, -8.0, -9.5, -11.0, -12.5, -15.0, -20.0, -1e4, torch.finfo(dtype).min, 6.5, 20.0, 1e4]).to(dtype)
+
+
+def check_gelu(z, y, dz, dtype):
+    """Phi(z) behind -6 is kept to 1 % (0.7 % by its fit, and the hardware's exponential), z^2 / 2 is rounded once (z^2 u of the density),
+    and what is below 2^-126 may be 0; in front of it 16 u as everywhere"""
+    z, y, dz = z.double().cpu(), y.double().cpu(), dz.double().cpu()
+    U, tiny = HALF_STEP[dtype], TINY[dtype]
+    want, slope = act64(z, "gelu"), dact64(z, "gelu")
+    density = torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    near_zero = 2.0 ** -126 * (z > -40) * (1 + z.abs())  # farther out nothing but 0 will do
+    rel = torch.where(z < -6, 0.01, 0.0) * want.abs() + torch.where(z < -6, 0.0, 16 * u) * z.abs()
+    assert bool(((y - want).abs() <= rel + U * (want.abs() + rel) + tiny * (z > -40) + near_zero).all()), (y, want)
+    phi = 0.5 * torch.erfc(-z / math.sqrt(2.0))
+    rel = torch.where(z < -6, 0.01, 0.0) * phi + torch.where(z < -6, 0.0, 16 * u) + (8 + 2 * z * z) * u * (z.abs() * density)
+    rel = torch.where(z.abs() < 40, rel, 16 * u * (z > 0))
+    assert bool(((dz - slope).abs() <= rel + U * (slope.abs() + rel) + tiny * (z > -40) + near_zero).all()), (dz, slope)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("copies", [1, 40])  # few rows, and enough for the kernel that streams them
+def test_gelu_goes_to_zero_in_the_far_tail_linear(dtype, copies):
+    z = far_values(dtype).repeat(copies).cuda().view(-1, 1)
+    one = torch.ones((1, 1), dtype=dtype, device="cuda")
+    y = ops.linear_act_fwd(z, one, None, 4)
+    dx = ops.linear_act_bwd(z, torch.ones_like(z), one, None, 4)[0]
+    check_gelu(z, y, dx, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [3, 3000])
+def test_gelu_goes_to_zero_in_the_far_tail_group_norm(dtype, rows):
+    """weight 0: z is the bias, whatever the rows are; the bias gradient of one gradient of 1 is act'(z)"""
+    z = far_values(torch.float32)
+    c = z.numel()
+    x = torch.randn((rows, c), device="cuda").to(dtype)
+    off = torch.tensor([0, rows], device="cuda")
+    w, b = torch.zeros(c, device="cuda"), z.cuda()
+    y, mean, rstd = ops.group_norm_fwd(x, off, 1, w, b, 1e-5, 4)
+    dy = torch.zeros_like(x)
+    dy[rows // 2] = 1
+    db = ops.group_norm_bwd(x, dy, off, 1, w, b, mean, rstd, 4)[2]
+    assert bool((y == y[:1]).all())
+    keep = z.abs() <= torch.finfo(dtype).max
+    check_gelu(z[keep], y[0].cpu()[keep].float(), db.cpu()[keep], dtype)
+    far = torch.tensor([-math.inf, math.inf, 0.0], device="cuda").repeat(c // 3)
+    y = ops.group_norm_fwd(x, off, 1, w, far, 1e-5, 4)[0].float()
+    assert bool(torch.isnan(y[:, 0]).all()) and bool((y[:, 1] == math.inf).all()) and bool((y[:, 2] == 0).all())
