@@ -211,8 +211,8 @@ __device__ __forceinline__ void gn_rows_sum(const GnArgs& a, const GnChunk<T, OR
               s0[k][u] += v;
               s1[k][u] = fma(v, v, s1[k][u]);
             } else {
-              const float xh = (xr[i][k][u] - mu[k][u]) * rs[k][u];
-              const double dz = (double)(dr[i][k][u] * pp_dact1(fmaf(xh, af.w[k][u], af.b[k][u]), a.act, a.slope));
+              const float d = xr[i][k][u] - mu[k][u], xh = d * rs[k][u];
+              const double dz = (double)(dr[i][k][u] * pp_dact1(fmaf(d, rs[k][u] * af.w[k][u], af.b[k][u]), a.act, a.slope));
               s0[k][u] += dz;
               s1[k][u] = fma(dz, (double)xh, s1[k][u]);
             }
@@ -274,14 +274,16 @@ __device__ __forceinline__ void gn_moments(double s0, double s1, double m, doubl
   *rstd = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + eps));  // (a NaN stays one)
 }
 
-// y or dx of the rows [p, e) of one batch element.  Forward z = x ka + kb with ka = rstd w, kb = b - mean rstd w, each rounded once from
-// fp64: as exact as x - mean first (whose mean is rounded), in half the registers; backward ka, kb = mean(h), mean(h xh)
+// y or dx of the rows [p, e) of one batch element.  z = (x - mean) (rstd w) + b both ways, the same three operations, so that the two agree
+// about the side of a kink.  x - mean comes first: it is exact where x is near the mean (one-row elements, constant channels: z = b), where
+// x (rstd w) + (b - mean rstd w) would leave |x| rstd 2^-24, with rstd up to 1 / sqrt(eps).  Backward ka, kb = mean(h), mean(h xh)
 template <typename T, int VEC, int NC, bool FORWARD, bool ORDER, typename Lane>
 __device__ __forceinline__ void gn_rows_apply(const GnArgs& a, const GnChunk<T, ORDER>& chunk, const Lane& ln, const GnAffine<VEC, NC>& af, int p, int e,
                                               const float (&mu)[NC][VEC], const float (&rs)[NC][VEC], const float (&ka)[NC][VEC],
                                               const float (&kb)[NC][VEC]) {
   if (!ln.on) return;
-  constexpr int U = NC == 1 ? 4 : 1;
+  // rows in flight: forward three, what 64 registers hold with mean, rstd w and b (2.5 M x 96 bf16, gelu: 375 us a pass, 392 with four)
+  constexpr int U = NC > 1 ? 1 : FORWARD ? 3 : 4;
   GnRows<ORDER, U> rows(a, chunk, p + ln.rin, e, ln.rps);
   while (rows.more()) {
     GnRaw<T, VEC> xr[U][NC], dr[U][NC];
@@ -303,14 +305,15 @@ __device__ __forceinline__ void gn_rows_apply(const GnArgs& a, const GnChunk<T, 
           float o[VEC];
           if (FORWARD) {
 #pragma unroll
-            for (int u = 0; u < VEC; ++u) o[u] = fmaf(xr[i][k][u], ka[k][u], kb[k][u]);
+            for (int u = 0; u < VEC; ++u) o[u] = fmaf(xr[i][k][u] - mu[k][u], ka[k][u], af.b[k][u]);
             pp_act(o, a.act, a.slope);
           } else {
             float xh[VEC], z[VEC];
 #pragma unroll
             for (int u = 0; u < VEC; ++u) {
-              xh[u] = (xr[i][k][u] - mu[k][u]) * rs[k][u];
-              z[u] = fmaf(xh[u], af.w[k][u], af.b[k][u]);
+              const float d = xr[i][k][u] - mu[k][u];
+              xh[u] = d * rs[k][u];
+              z[u] = fmaf(d, rs[k][u] * af.w[k][u], af.b[k][u]);
               o[u] = dr[i][k][u] * af.w[k][u];
             }
             pp_dact(o, z, a.act, a.slope);
@@ -559,11 +562,7 @@ __global__ __launch_bounds__(256, NC > 1 ? 1 : INLINE ? 4 : FORWARD ? 8 : 5) voi
 #pragma unroll
       for (int k = 0; k < NC; ++k)
 #pragma unroll
-        for (int u = 0; u < VEC; ++u) {
-          const double f = (double)rs[k][u] * (double)af.w[k][u];
-          ka[k][u] = (float)f;
-          kb[k][u] = (float)((double)af.b[k][u] - (double)mu[k][u] * f);
-        }
+        for (int u = 0; u < VEC; ++u) ka[k][u] = rs[k][u] * af.w[k][u];
     }
     gn_rows_apply<T, VEC, NC, FORWARD, ORDER>(a, chunk, ln, af, p, e, mu, rs, ka, kb);
   }

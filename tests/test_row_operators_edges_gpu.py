@@ -63,3 +63,40 @@ def test_gelu_goes_to_zero_in_the_far_tail_group_norm(dtype, rows):
     far = torch.tensor([-math.inf, math.inf, 0.0], device="cuda").repeat(c // 3)
     y = ops.group_norm_fwd(x, off, 1, w, far, 1e-5, 4)[0].float()
     assert bool(torch.isnan(y[:, 0]).all()) and bool((y[:, 1] == math.inf).all()) and bool((y[:, 2] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["none", "relu", "silu"])
+def test_rows_equal_to_their_mean_come_out_as_the_bias(dtype, kind):
+    """one-row elements under instance norm, and constant channels: x is its mean, so z is the bias whatever the size of x"""
+    act = ops.activation_id(kind)
+    size = torch.tensor([0.3, 10.3, 1000.1, 30000.0], device="cuda")
+    for c, rows in ((8, 1), (7, 1), (64, 300), (300, 40), (12, 70_000)):
+        sign = torch.where(torch.arange(c, device="cuda") % 3 == 0, -1.0, 1.0)
+        x = (size.repeat(-(-c // 4))[:c] * sign).repeat(3 * rows, 1).to(dtype)
+        off = torch.tensor([0, rows, rows, 3 * rows], device="cuda")
+        w, b = 1 + torch.rand(c, device="cuda"), torch.randn(c, device="cuda")
+        y, mean, rstd = ops.group_norm_fwd(x, off, c, w, b, 1e-5, act)
+        assert bool((y == y[:1]).all())
+        want = act64(b.double(), kind)
+        assert bool(((y[0].double() - want).abs() <= HALF_STEP[dtype] * want.abs() + (16 * u if kind == "silu" else 0) * b.double().abs()).all())
+        y, mean, rstd = ops.group_norm_fwd(x, off, c, w, None, 1e-5, act)
+        assert int(y.count_nonzero()) == 0
+        assert int(ops.group_norm_bwd(x, torch.ones_like(x), off, c, w, None, mean, rstd, 1)[2].count_nonzero()) == 0  # relu at 0: slope 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c,groups", [(32, 8), (7, 7), (300, 300)])
+@pytest.mark.parametrize("lengths", [[20_000], [1, 2, 3, 500, 9494, 10_000]])
+def test_forward_and_backward_agree_about_the_side_of_a_kink(dtype, c, groups, lengths):
+    """with gradients of one the bias gradient of relu counts the values whose z is positive: those that are in the result"""
+    n = sum(lengths)
+    gen = torch.Generator(device="cuda").manual_seed(c + n)
+    x = (200 + 3 * torch.randn((n, c), generator=gen, device="cuda")).to(dtype)
+    off = torch.tensor([0] + lengths, device="cuda").cumsum(0)
+    w = 1 + torch.rand(c, generator=gen, device="cuda")
+    for b in (None, 1e-6 * torch.randn(c, generator=gen, device="cuda")):
+        _, mean, rstd = ops.group_norm_fwd(x, off, groups, w, b, 1e-5, 1)
+        db = ops.group_norm_bwd(x, torch.ones_like(x), off, groups, w, b, mean, rstd, 1)[2]
+        positive = ops.group_norm_fwd(x.float(), off, groups, w, b, 1e-5, 1)[0] > 0  # (16-bit values are fp32 values)
+        assert torch.equal(db.double(), positive.sum(0).double())
