@@ -16,6 +16,7 @@
 
 #define GN_MAX_CHUNKS 1024
 #define GN_MAX_C 1024
+#define GN_FINISH_BLOCKS (1 << 22)
 
 struct GnArgs {
   const void *x, *dy;
@@ -446,7 +447,8 @@ __device__ __forceinline__ void gn_parameters(const GnArgs& a, int block, double
   if (j == 1 && a.dweight) a.dweight[ch] = (float)v0;
 }
 
-// Between the passes: one wave per (element, group) adds its slots; backward, the workgroups behind them make the parameters' gradients
+// Between the passes: one wave per (element, group) adds its slots, in turns where there are more than GN_FINISH_BLOCKS workgroups' worth (a
+// launch has less than 2^32 threads); backward, the workgroups behind them make the parameters' gradients
 template <bool FORWARD>
 __global__ __launch_bounds__(256) void k_gn_finish(GnArgs a, int64_t group_blocks) {
   if (!FORWARD && (int64_t)blockIdx.x >= group_blocks) {
@@ -455,27 +457,27 @@ __global__ __launch_bounds__(256) void k_gn_finish(GnArgs a, int64_t group_block
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= a.b * a.g) return;
-  const int64_t s = w / a.g;
-  const int g = (int)(w - s * a.g);
-  int64_t j0, j1;
-  double m, v0 = 0.0, v1 = 0.0;
-  const bool any = gn_slots(a, s, &j0, &j1, &m);
-  if (any)
-    for (int64_t j = j0 + lane; j <= j1; j += 64) {
-      v0 += a.slots[((j + s) * a.g + g) * 2];
-      v1 += a.slots[((j + s) * a.g + g) * 2 + 1];
+  for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); w < a.b * a.g; w += group_blocks * 4) {
+    const int64_t s = w / a.g;
+    const int g = (int)(w - s * a.g);
+    int64_t j0, j1;
+    double m, v0 = 0.0, v1 = 0.0;
+    const bool any = gn_slots(a, s, &j0, &j1, &m);
+    if (any)
+      for (int64_t j = j0 + lane; j <= j1; j += 64) {
+        v0 += a.slots[((j + s) * a.g + g) * 2];
+        v1 += a.slots[((j + s) * a.g + g) * 2 + 1];
+      }
+    for (int d = 32; d > 0; d >>= 1) {
+      v0 += __shfl_xor(v0, d);
+      v1 += __shfl_xor(v1, d);
     }
-  for (int d = 32; d > 0; d >>= 1) {
-    v0 += __shfl_xor(v0, d);
-    v1 += __shfl_xor(v1, d);
+    if (lane != 0) continue;
+    float first = 0.f, second = 0.f;
+    if (any) gn_stat<FORWARD>(a, v0, v1, m, &first, &second);
+    (FORWARD ? a.mean : a.coef)[FORWARD ? w : 2 * w] = first;
+    (FORWARD ? a.rstd : a.coef)[FORWARD ? w : 2 * w + 1] = second;
   }
-  if (lane != 0) return;
-  float first = 0.f, second = 0.f;
-  if (any) gn_stat<FORWARD>(a, v0, v1, m, &first, &second);
-  (FORWARD ? a.mean : a.coef)[FORWARD ? w : 2 * w] = first;
-  (FORWARD ? a.rstd : a.coef)[FORWARD ? w : 2 * w + 1] = second;
 }
 
 // The same inside the second pass: the workgroup's threads over slots and groups, -> stat[g][2] in the LDS, and to mean and rstd by the
@@ -615,7 +617,7 @@ static int gn_launch(GnArgs& a, hipStream_t s) {
       gn_sums<T, VEC, NC, FORWARD, ORDER>(a, s);
     PP_LAUNCH_CHECK();
   }
-  const int64_t gb = (a.b * a.g + 3) / 4, pb = FORWARD ? 0 : (a.c + 3) / 4;
+  const int64_t gw = (a.b * a.g + 3) / 4, gb = gw < GN_FINISH_BLOCKS ? gw : GN_FINISH_BLOCKS, pb = FORWARD ? 0 : (a.c + 3) / 4;
   if (in) {
     const int64_t more = FORWARD ? (a.b + 255) / 256 : pb;
     hipLaunchKernelGGL((k_gn_chunk_apply<T, VEC, NC, FORWARD, ORDER, true>), dim3((unsigned)(a.blocks + more)), dim3(256),

@@ -100,3 +100,40 @@ def test_forward_and_backward_agree_about_the_side_of_a_kink(dtype, c, groups, l
         db = ops.group_norm_bwd(x, torch.ones_like(x), off, groups, w, b, mean, rstd, 1)[2]
         positive = ops.group_norm_fwd(x.float(), off, groups, w, b, 1e-5, 1)[0] > 0  # (16-bit values are fp32 values)
         assert torch.equal(db.double(), positive.sum(0).double())
+
+
+def test_more_statistics_than_a_launch_has_threads_for():
+    """65600 batch elements x 1024 groups = 2^26 statistics and more, of elements of one and two rows.  Instance norm of two rows: the
+    values are d and -d around their mean, so xh = +- d / sqrt(d^2 + eps)"""
+    b, c = 65_600, 1024
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    lengths = torch.ones(b, dtype=torch.int64, device="cuda")
+    lengths[::40] = 2
+    lengths[7::40] = 0
+    off = torch.zeros(b + 1, dtype=torch.int64, device="cuda")
+    off[1:] = lengths.cumsum(0)
+    n = int(off[-1])
+    x = torch.randn((n, c), generator=gen, device="cuda")
+    w, bias = 1 + torch.rand(c, generator=gen, device="cuda"), torch.randn(c, generator=gen, device="cuda")
+    assert b * c >= 2 ** 26
+    y, mean, rstd = ops.group_norm_fwd(x, off, c, w, bias, 1e-5)
+    first = off[:-1][lengths == 2]
+    pair = torch.zeros(n, dtype=torch.bool, device="cuda")
+    pair[first] = pair[first + 1] = True
+    assert torch.equal(y[~pair], bias.expand(n, c)[~pair]) and int(rstd[7::40].count_nonzero()) == 0
+    p, q = x[first].double(), x[first + 1].double()
+    d, m = (p - q) / 2, (p + q) / 2
+    r = 1 / torch.sqrt(d * d + 1e-5)
+    ez = w.double() * 4 * u * (r * (p.abs() + m.abs()) + 1) + 2 * u * (w.double() + bias.abs().double())
+    assert bool(((y[first].double() - (d * r * w + bias)).abs() <= ez + u * 4).all())
+    assert bool(((mean[lengths == 2].double() - m).abs() <= 2 * u * m.abs() + 1e-30).all()) and bool(((rstd[lengths == 2].double() - r).abs() <= 2 * u * r).all())
+    # one row: every value is its own mean, so its gradient is 0; two rows: dx = r (1 - xh^2) (dy1 - dy2) / 2 w
+    dy = torch.randn((n, c), generator=gen, device="cuda")
+    dx, dw, db = ops.group_norm_bwd(x, dy, off, c, w, bias, mean, rstd)
+    assert int(dx[~pair].count_nonzero()) == 0
+    xh, h1, h2 = d * r, dy[first].double() * w, dy[first + 1].double() * w
+    exh = 4 * u * (r * (p.abs() + m.abs()) + 1)
+    want = r * (1 - xh * xh) * (h1 - h2) / 2
+    size = h1.abs() + h2.abs()
+    assert bool(((dx[first].double() - want).abs() <= r * (20 * u * size + 4 * exh * size)).all())
+    assert bool(((db.double() - dy.double().sum(0)).abs() <= 2 * u * dy.double().abs().sum(0)).all())
