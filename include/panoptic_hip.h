@@ -393,7 +393,8 @@ int pp_bn_train_bwd(const float* x, const float* dy, const float* y_relu, int64_
  * positions offsets[s] .. offsets[s+1] - 1 (device int64 [b+1], ascending); position p is row order[p] (device int64 [n], each row
  * once; NULL: row p).  Rows of no batch element get zeros.  weight, bias float32 [c], nullable.  mean, rstd float32 [b,groups] are
  * kept for the backward (0 for a batch element without rows).
- * fwd: y = act((x - mean) * rstd * weight + bias), biased variance.   bwd: dx, dweight, dbias (nullable) of the same.
+ * fwd: y = act((x - mean) * rstd * weight + bias), biased variance.   bwd: dx, dweight, dbias of the same; each nullable, and what
+ * only it needs is left out (without dx the second pass over the rows).
  * Sums are float64, no atomics: results repeat bit for bit.
  * ---------------------------------------------------------------------------------------------- */
 size_t pp_group_norm_workspace(int64_t n, int64_t b, int32_t c, int32_t groups, int32_t backward);

@@ -32,7 +32,7 @@ struct GnArgs {
   float slope;
   float *mean, *rstd;   // [b, g]; written forward, read backward
   double* slots;        // [slot][g][2]: sums of x, x^2 forward, of h, h xh backward
-  double* totals;       // backward [chunk][2][c]: sums of dz, dz xh
+  double* totals;       // backward [chunk][2][c]: sums of dz, dz xh; null: nobody wants the parameters' gradients
   float* coef;          // backward [b, g][2]: mean(h), mean(h xh), where k_gn_finish makes them
   float *dweight, *dbias;
   int64_t rows_per_chunk, rows_per_block;  // positions of a workgroup of the first, and of the second pass
@@ -378,6 +378,7 @@ __global__ __launch_bounds__(256, NC == 1 ? 4 : 1) void k_gn_chunk_sums(GnArgs a
     __syncthreads();
   }
   if constexpr (!FORWARD) {
+    if (!a.totals) return;
     if (ln.on)
 #pragma unroll
       for (int k = 0; k < NC; ++k)
@@ -605,7 +606,7 @@ static int gn_launch(GnArgs& a, hipStream_t s) {
   a.rows_per_chunk = gn_rows_per_chunk(a.n);
   a.chunks = gn_chunks(a.n);
   a.rows_per_block = gn_rows_per_block(a.n, (int64_t)a.c * sizeof(T));
-  a.blocks = (int)((a.n + a.rows_per_block - 1) / a.rows_per_block);
+  a.blocks = a.out ? (int)((a.n + a.rows_per_block - 1) / a.rows_per_block) : 0;  // (backward without dx: no second pass)
   const bool in = a.b > 0 && a.blocks <= GN_MAX_CHUNKS && (a.chunks / a.b + 2) * a.g * (int64_t)(2 * sizeof(double)) <= GN_INLINE;
   if (a.chunks) {
     // eight channels of 16 bits at a time where the loads bound, as in long forward sums (2.5 M x 96: 119 us, 160 us with four); elsewhere
@@ -617,9 +618,10 @@ static int gn_launch(GnArgs& a, hipStream_t s) {
       gn_sums<T, VEC, NC, FORWARD, ORDER>(a, s);
     PP_LAUNCH_CHECK();
   }
-  const int64_t gw = (a.b * a.g + 3) / 4, gb = gw < GN_FINISH_BLOCKS ? gw : GN_FINISH_BLOCKS, pb = FORWARD ? 0 : (a.c + 3) / 4;
+  const int64_t gw = (a.b * a.g + 3) / 4, gb = gw < GN_FINISH_BLOCKS ? gw : GN_FINISH_BLOCKS, pb = FORWARD || !a.totals ? 0 : (a.c + 3) / 4;
   if (in) {
     const int64_t more = FORWARD ? (a.b + 255) / 256 : pb;
+    if (a.blocks + more == 0) return PP_OK;
     hipLaunchKernelGGL((k_gn_chunk_apply<T, VEC, NC, FORWARD, ORDER, true>), dim3((unsigned)(a.blocks + more)), dim3(256),
                        512 * sizeof(double) + (size_t)a.g * 2 * sizeof(float), s, a);
     PP_LAUNCH_CHECK();
@@ -689,8 +691,9 @@ extern "C" int pp_group_norm_bwd(const void* x, const void* dy, int32_t dtype, i
                                  void* ws, size_t ws_bytes, pp_stream_t stream) {
   int rc = gn_check(dtype, n, c, groups, offsets, b, act);
   if (rc != PP_OK) return rc;
-  PP_REQUIRE((n == 0 || (x && dy && dx)) && (b == 0 || (mean && rstd)) && ws, "pp_group_norm_bwd: null pointer");
+  PP_REQUIRE((n == 0 || (x && dy)) && (b == 0 || (mean && rstd)) && ws, "pp_group_norm_bwd: null pointer");
   PP_REQUIRE((uintptr_t)ws % 16 == 0, "pp_group_norm_bwd: the workspace must be 16-byte aligned");
+  if (!dx && !dweight && !dbias) return PP_OK;
   if (ws_bytes < pp_group_norm_workspace(n, b, c, groups, 1)) {
     pp_set_error("pp_group_norm_bwd: workspace too small");
     return PP_ERR_WORKSPACE;
@@ -705,5 +708,6 @@ extern "C" int pp_group_norm_bwd(const void* x, const void* dy, int32_t dtype, i
   a.totals = arena.take<double>((size_t)(gn_chunks(n) + 1) * 2 * c);
   a.coef = arena.take<float>((size_t)b * groups * 2);
   PP_REQUIRE(a.slots && a.totals && a.coef, "pp_group_norm_bwd: workspace layout");
+  if (!dweight && !dbias) a.totals = nullptr;
   return gn_dispatch<false>(a, dtype, pp_s(stream));
 }

@@ -18,10 +18,14 @@ class _GroupNormActFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, offsets, weight, bias, stat, order = ctx.saved_tensors
         num_groups, act, slope = ctx.cfg
-        at = stat.data_ptr()
-        with ops.device_of(x):
-            dx, dw, db = ops._group_norm_bwd(x, dy, offsets, num_groups, weight, bias, at, at + 2 * stat.numel(), act, slope, order)
-        return dx, None, None, dw if weight is not None else None, db if bias is not None else None, None, None, None, None
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if need[0] or need[3] or need[4]:
+            at = stat.data_ptr()
+            with ops.device_of(x):
+                dx, dw, db = ops._group_norm_bwd(x, dy, offsets, num_groups, weight, bias, at, at + 2 * stat.numel(), act, slope, order,
+                                                 need[0], need[3], need[4])
+        return dx, None, None, dw, db, None, None, None, None
 
 
 def group_norm_act(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, activation="none", slope=0.2, order=None):

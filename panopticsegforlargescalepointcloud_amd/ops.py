@@ -1331,15 +1331,19 @@ def _group_norm_fwd(x, offsets, num_groups, weight, bias, eps, act, slope, order
 
 
 @_on_device_of
-def group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act=0, slope=0.0, order=None):
-    """Backward of group_norm_fwd with the statistics it returned: (dx, dweight, dbias), the last two float32 [c]."""
+def group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act=0, slope=0.0, order=None, want_input=True,
+                   want_weight=True, want_bias=True):
+    """Backward of group_norm_fwd with the statistics it returned: (dx, dweight, dbias), the last two float32 [c]; None for what is
+    not wanted."""
     shape = (offsets.shape[0] - 1, num_groups)
     mean = _beside(mean, x, torch.float32, shape, "mean")
     rstd = _beside(rstd, x, torch.float32, shape, "rstd")
-    return _group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean.data_ptr(), rstd.data_ptr(), act, slope, order)
+    return _group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean.data_ptr(), rstd.data_ptr(), act, slope, order, want_input,
+                           want_weight, want_bias)
 
 
-def _group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act, slope, order):
+def _group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act, slope, order, want_input=True, want_weight=True,
+                    want_bias=True):
     """mean, rstd: device addresses of contiguous statistics; x's device is current"""
     lib = _lib.load()
     code = _row_dtype(x, "x")
@@ -1347,12 +1351,13 @@ def _group_norm_bwd(x, dy, offsets, num_groups, weight, bias, mean, rstd, act, s
     n, c = x.shape
     b = offsets.shape[0] - 1
     dy = _beside(dy, x, x.dtype, (n, c), "dy")
-    dx = torch.empty_like(x)
+    dx = torch.empty_like(x) if want_input else None
     dw, db = torch.empty((2, c), dtype=torch.float32, device=x.device).unbind(0)
+    dw, db = dw if want_weight else None, db if want_bias else None
     wsb = lib.pp_group_norm_workspace(n, b, c, num_groups, 1)
     ws = _ws(wsb, x.device)
     _lib.check(lib.pp_group_norm_bwd(x.data_ptr(), dy.data_ptr(), code, n, c, num_groups, offsets.data_ptr(), b, _at(order), _at(weight),
-                                     _at(bias), mean, rstd, act, slope, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws.numel(),
+                                     _at(bias), mean, rstd, act, slope, _at(dx), _at(dw), _at(db), ws.data_ptr(), ws.numel(),
                                      _stream()), "pp_group_norm_bwd")
     return dx, dw, db
 
