@@ -612,20 +612,21 @@ __global__ __launch_bounds__(256) void k_linear_sum4(const float* __restrict__ p
   for (int e = 0; e < 4; ++e) out[i + e] = (T)(float)s[e];
 }
 
-// column sums of a part of the rows of [n, c]: part[blockIdx.y][c]; 64 columns a block, four rows side by side
+// column sums of a part of the rows of [n, c]: part[blockIdx.y][c]; 64 columns a block, four rows side by side.  In fp64: a thread's rows grow
+// with n, and sums of one sign in fp32 would lose n 2^-25 / 1024 of them (dy of 0.1, 10 M rows: 3.7e-4)
 template <typename T>
 __global__ __launch_bounds__(256) void k_linear_columns(const T* __restrict__ x, int64_t n, int c, int64_t rows_per_part, float* __restrict__ part) {
-  __shared__ float red[256];
+  __shared__ double red[256];
   const int col = blockIdx.x * 64 + (threadIdx.x & 63), rl = threadIdx.x >> 6;
   const int64_t r0 = blockIdx.y * rows_per_part, r1 = r0 + rows_per_part < n ? r0 + rows_per_part : n;
-  float s = 0.f;
+  double s = 0.0;
   if (col < c) {
 #pragma unroll 8
-    for (int64_t r = r0 + rl; r < r1; r += 4) s += (float)x[r * c + col];
+    for (int64_t r = r0 + rl; r < r1; r += 4) s += (double)(float)x[r * c + col];
   }
   red[threadIdx.x] = s;
   __syncthreads();
-  if (rl == 0 && col < c) part[(int64_t)blockIdx.y * c + col] = red[threadIdx.x] + red[threadIdx.x + 64] + red[threadIdx.x + 128] + red[threadIdx.x + 192];
+  if (rl == 0 && col < c) part[(int64_t)blockIdx.y * c + col] = (float)(red[threadIdx.x] + red[threadIdx.x + 64] + red[threadIdx.x + 128] + red[threadIdx.x + 192]);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------
@@ -695,14 +696,25 @@ static int lin_splits(int64_t n, int cin, int cout, bool wide) {
   return s < 1 ? 1 : (int)s;
 }
 #define LIN_SUM_GROUPS 32
-#define LIN_COLUMN_PARTS 64
+#define LIN_COLUMN_PARTS 512  // at most; a part has at least LIN_COLUMN_ROWS rows
+#define LIN_COLUMN_ROWS 1024
 #define LIN_STREAM_GRID_MAX 256
 static int64_t lin_ldz(int cout) { return (cout + 7) / 8 * 8; }
 
+// workgroups of the narrow kernel: what finds room on the chip at once (two of a compute unit forward, up to 96 channels; the registers leave
+// one backward).  Backward a lane adds its column's gradients over its tiles in fp32: at most LIN_STREAM_CHAIN of them, so that the sum is off
+// by 2^-15 of its terms' at most whatever n is
+#define LIN_STREAM_CHAIN 1024
+static int64_t lin_stream_grid(int64_t n, bool backward) {
+  const int64_t tiles = (n + 16 * LIN_STREAM_WAVES - 1) / (16 * LIN_STREAM_WAVES), long_n = (tiles + LIN_STREAM_CHAIN - 1) / LIN_STREAM_CHAIN;
+  const int64_t most = !backward ? 2 * LIN_STREAM_GRID_MAX : long_n > LIN_STREAM_GRID_MAX ? long_n : LIN_STREAM_GRID_MAX;
+  return tiles < most ? tiles : most;
+}
+
 // rows of the bias gradient's parts: row tiles (or column parts without an activation), or the narrow kernel's workgroups; room to add them
 static size_t lin_bias_rows(int64_t n, int act) {
-  const size_t tiles = act == PP_ACT_NONE ? LIN_COLUMN_PARTS : (size_t)((n + 127) / 128);
-  return (tiles > LIN_STREAM_GRID_MAX ? tiles : LIN_STREAM_GRID_MAX) + LIN_SUM_GROUPS;
+  const size_t tiles = act == PP_ACT_NONE ? LIN_COLUMN_PARTS : (size_t)((n + 127) / 128), stream = (size_t)lin_stream_grid(n, true);
+  return (tiles > stream ? tiles : stream) + LIN_SUM_GROUPS;
 }
 
 extern "C" size_t pp_linear_act_bwd_workspace(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_t act) {
@@ -753,11 +765,6 @@ static size_t lin_stream_lds(int64_t n, int cin, int cout, int act, bool backwar
   if (backward && n < 65536 && (act == PP_ACT_NONE || (cin > 128 && cout > 128))) return 0;
   const size_t kb = (cin + 31) / 32, nb = (cout + 31) / 32;
   return kb * nb * 2048 * (backward ? 2 : 1) + nb * 128;  // (103 KB at most)
-}
-// workgroups: what finds room on the chip at once (two of a compute unit forward, up to 96 channels; the registers leave one backward)
-static int64_t lin_stream_grid(int64_t n, bool backward) {
-  const int64_t most = backward ? LIN_STREAM_GRID_MAX : 2 * LIN_STREAM_GRID_MAX, tiles = (n + 16 * LIN_STREAM_WAVES - 1) / (16 * LIN_STREAM_WAVES);
-  return tiles < most ? tiles : most;
 }
 template <typename T, int KB, int NB, bool BACKWARD>
 static int lin_stream_go(const LinStreamArgs& a, size_t lds, hipStream_t s) {
@@ -850,7 +857,8 @@ static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const
       if ((rc = lin_tile<T, false, false, LIN_DZ>(a, 1, s)) != PP_OK) return rc;
     }
   } else if (db && n) {
-    bias_parts = n < 16 * LIN_COLUMN_PARTS ? 1 : LIN_COLUMN_PARTS;
+    bias_parts = (n + LIN_COLUMN_ROWS - 1) / LIN_COLUMN_ROWS;
+    if (bias_parts > LIN_COLUMN_PARTS) bias_parts = LIN_COLUMN_PARTS;
     hipLaunchKernelGGL((k_linear_columns<T>), dim3((unsigned)((cout + 63) / 64), (unsigned)bias_parts), dim3(256), 0, s, (const T*)dy, n, cout,
                        (n + bias_parts - 1) / bias_parts, part_bias);
     PP_LAUNCH_CHECK();

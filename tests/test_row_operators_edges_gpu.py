@@ -165,3 +165,24 @@ def test_group_norm_makes_the_gradients_that_are_wanted(dtype, lengths, c, group
         if frozen != 7:
             y.backward(dy)
         assert all(leaf.grad is None if frozen >> i & 1 else torch.equal(leaf.grad, f) for i, (leaf, f) in enumerate(zip(leaves, full))), frozen
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,cin,cout", [(1_250_000, 8, 8), (5_000_000, 8, 16), (1_250_001, 4, 200), (70_003, 16, 70)])
+@pytest.mark.parametrize("kind", ["none", "silu"])
+def test_bias_gradients_of_one_sign_over_many_rows(dtype, n, cin, cout, kind):
+    """dy near 0.1 everywhere.  Sums of positive terms: a chain of k fp32 additions is off by k u / 2 of the sum at most (its partial sums grow
+    evenly); no chain is longer than 1024 whatever n is, and what is added to it in fp64 rounds twice.  act' is off by 16 u."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn((n, cin), generator=gen, device="cuda").to(dtype)
+    w = torch.zeros((cout, cin), device="cuda", dtype=dtype)  # z is the bias
+    b = torch.linspace(0.5, 3, cout, device="cuda").to(dtype)
+    room = (64 if dtype == torch.float32 else 512 + 16) * u
+    for scale in (1.0, 1 / 64):
+        dy = (scale * (0.1 + 0.001 * torch.arange(cout, device="cuda"))).to(dtype).expand(n, cout).contiguous()
+        db = ops.linear_act_bwd(x, dy, w, b, ops.activation_id(kind), want_input=False, want_weight=False)[2]
+        want = dy[0].double() * dact64(b.double(), kind) * n
+        over = want > torch.finfo(dtype).max * (1 + HALF_STEP[dtype])  # (the sum itself is none of the type's numbers)
+        assert bool((db[over] == math.inf).all())
+        off = (db.double() / want - 1).abs()[~over]
+        assert bool((off <= room + HALF_STEP[dtype] * (1 + room)).all()), off.max()
