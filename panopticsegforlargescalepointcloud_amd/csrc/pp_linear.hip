@@ -5,8 +5,8 @@
 // down its columns is transposed on the way, in registers), 16 bytes at a time, XOR-swizzled so that the fragment reads of 16 rows
 // spread over all banks; the next step's loads are in flight while this step's fragments are multiplied.
 // fp32 operands are split exactly into three bf16 terms (8 + 8 + 8 bits) when they are staged, and a product is the six bf16 products
-// above 2^-24 of it, accumulated in fp32: an fp32-accurate evaluation at 2.7 times the rate of the fp32 matrix instructions.  A
-// non-finite value makes the results it enters NaN.  bf16 and fp16 operands are multiplied as they are, accumulated in fp32.
+// above 2^-24 of it, accumulated in fp32: an fp32-accurate evaluation at 2.7 times the rate of the fp32 matrix instructions.
+// Infinities and NaN do what they do in a plain sum (LinEpilogue::exact).  bf16 and fp16 operands are multiplied as they are, accumulated in fp32.
 // Nothing is kept for the backward pass but x: z is recomputed from it (the layers are bound by memory, a stored z would cost a write
 // and a read of its own, and its rounding would enter the gradients).  dz is rounded to the element type once, as the matrix
 // instructions take it.  The weight gradient's rows are cut into parts, whose sums are added in a fixed order: results repeat.
@@ -224,8 +224,38 @@ struct LinEpilogue {
       }
     }
   }
+  // fp32: where a term is infinite, NaN or so large that its first plane overflows, its planes make the products NaN.  Such results are
+  // made again from the operands as they are, one multiplication and addition at a time (in fp64: a sum that fp32 holds is not lost
+  // half way).  Nothing else is: the check is one comparison per value of the epilogue
+  __device__ __forceinline__ void exact(int64_t r, float (&v)[8]) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += v[e];
+    if (sum == sum) return;
+    constexpr bool AS = MODE == LIN_PART, BS = MODE == LIN_PART || MODE == LIN_STORE;
+    const float *A = (const float*)a.a, *B = (const float*)a.b;
+    const int64_t k0 = MODE == LIN_PART ? split * a.k_per_split : 0, k1 = MODE == LIN_PART && k0 + a.k_per_split < a.k ? k0 + a.k_per_split : a.k;
+    double s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = 0.0;
+#pragma unroll 1
+    for (int64_t k = k0; k < k1; ++k) {
+      const double x = (double)A[AS ? k * a.lda + r : r * a.lda + k];
+      bool all_nan = true;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < valid) {
+          s[e] = fma(x, (double)B[BS ? k * a.ldb + c + e : (c + e) * a.ldb + k], s[e]);
+          all_nan &= s[e] != s[e];
+        }
+      if (all_nan) break;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < valid ? (v[e] == v[e] ? v[e] : (float)s[e]) : 0.f;
+  }
   __device__ __forceinline__ void put(int64_t r, Row& w, float (&v)[8]) {
     if (r >= a.m) return;
+    if constexpr (sizeof(T) == 4) exact(r, v);
     if constexpr (FUSED) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += b[e];

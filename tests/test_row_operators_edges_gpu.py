@@ -186,3 +186,51 @@ def test_bias_gradients_of_one_sign_over_many_rows(dtype, n, cin, cout, kind):
         assert bool((db[over] == math.inf).all())
         off = (db.double() / want - 1).abs()[~over]
         assert bool((off <= room + HALF_STEP[dtype] * (1 + room)).all()), off.max()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,cin,cout", [(5, 8, 6), (300, 75, 133), (300, 64, 64), (400, 200, 392), (70_000, 40, 24)])
+def test_infinities_do_what_they_do_in_a_sum(dtype, n, cin, cout):
+    """rows, weights and gradients with infinities and the largest finite numbers: where the sum of 64 bits is infinite or NaN the result is,
+    and where act makes a number of it, it is that number"""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    draw = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    x, w, b, dy = draw(n, cin).to(dtype), (0.1 + draw(cout, cin).abs()).to(dtype), draw(cout).to(dtype), draw(n, cout).to(dtype)
+    x[0], x[n // 2, 3], x[n // 2, 5], x[n - 1, 0], x[2, 1] = -math.inf, math.inf, -math.inf, math.inf, math.nan
+    w[2, 4] = 0.0
+    x[3, 4] = math.inf  # times 0
+    finite = torch.isfinite(x).all(1)
+    plain_y = ops.linear_act_fwd(torch.where(finite[:, None], x, 0), w, b)
+    plain = ops.linear_act_bwd(torch.where(finite[:, None], x, 0), dy, w, b, 1)
+    z = x.double() @ w.double().t() + b.double()
+    for kind in ("none", "relu", "leaky_relu"):
+        y = ops.linear_act_fwd(x, w, b, ops.activation_id(kind), 0.2).double()
+        want = torch.where(torch.isnan(z), z, z.clamp(min=0) if kind == "relu" else torch.where(z > 0, z, 0.2 * z) if kind == "leaky_relu" else z)
+        special = ~finite
+        assert torch.equal(torch.isnan(y[special]), torch.isnan(want[special])), kind
+        keep = ~torch.isnan(want) & special[:, None]
+        assert torch.equal(y[keep], want[keep].to(dtype).double()), kind  # infinities, and relu's zeros
+    assert torch.equal(ops.linear_act_fwd(x, w, b)[finite], plain_y[finite])
+    # relu of a row of -inf or +inf: slopes 0 and 1, so dx is finite; the row's part of dW is 0 * inf = NaN or inf
+    dx, dw, db = ops.linear_act_bwd(x, dy, w, b, 1)
+    assert torch.equal(dx[finite], plain[0][finite]) and int(dx[0].count_nonzero()) == 0 and bool(torch.isfinite(dx[n - 1]).all())
+    assert bool(torch.isnan(dw).all()) and bool(torch.isfinite(db).all())  # (row 0: 0 * -inf in every entry)
+    d = dy.clone()
+    d[1, 2] = math.inf
+    clean = torch.where(finite[:, None], x, 0)
+    dx, dw, _ = ops.linear_act_bwd(clean, d, w, b, 0)
+    assert torch.equal(torch.isnan(dx[1]), w[2] == 0) and bool((dx[1][w[2] > 0] == math.inf).all())
+    want = math.inf * clean[1].double()
+    assert torch.equal(torch.isnan(dw[2].double()), torch.isnan(want)) and torch.equal(dw[2].double()[want.abs() == math.inf], want[want.abs() == math.inf])
+    same = torch.arange(cout, device="cuda") != 2
+    assert torch.equal(dw[same], ops.linear_act_bwd(clean, dy, w, b, 0)[1][same])
+
+
+def test_largest_numbers_of_fp32():
+    """values above the largest bfloat16, and partial sums that pass the range but come back"""
+    top = torch.finfo(torch.float32).max
+    x = torch.tensor([[top, 1.0, 0.0], [-top, 0.0, 2.0], [top, top, 0.0], [3.4e38, 0.0, 1e38]], device="cuda")
+    w = torch.tensor([[0.5, 0.0, 0.0], [1.0, 0.0, 0.0], [-0.25, -0.125, 1.0], [0.0, 2.0, 3.0]], device="cuda")
+    y = ops.linear_act_fwd(x, w).double()
+    want = (x.double() @ w.double().t())
+    assert torch.equal(y, want.float().double()), (y, want)
