@@ -4,8 +4,8 @@
 // in steps of BK: every operand is brought to the LDS as rows of consecutive contraction elements (an operand whose contraction runs
 // down its columns is transposed on the way, in registers), 16 bytes at a time, XOR-swizzled so that the fragment reads of 16 rows
 // spread over all banks; the next step's loads are in flight while this step's fragments are multiplied.
-// fp32 operands are split exactly into three bf16 terms (8 + 8 + 8 bits) when they are staged, and a product is the six bf16 products
-// above 2^-24 of it, accumulated in fp32: an fp32-accurate evaluation at 2.7 times the rate of the fp32 matrix instructions.
+// fp32 operands are split exactly into three bf16 terms (8 + 8 + 8 bits) when they are staged, and a product is the six largest of its
+// nine bf16 products (the others are at most 2^-23 of it), accumulated in fp32: an fp32-accurate evaluation at 2.7 times the rate of the fp32 matrix instructions.
 // Infinities and NaN do what they do in a plain sum (LinEpilogue::exact).  bf16 and fp16 operands are multiplied as they are, accumulated in fp32.
 // Nothing is kept for the backward pass but x: z is recomputed from it (the layers are bound by memory, a stored z would cost a write
 // and a read of its own, and its rounding would enter the gradients).  dz is rounded to the element type once, as the matrix
@@ -39,20 +39,22 @@ template <> struct LinType<float> {
 // eight elements of the contraction, in the form they have in the LDS: PLANES x 16 bytes
 template <typename T> struct LinChunk { gm_u32x4 p[LinType<T>::PLANES]; };
 
+// hi, mid and lo, each the nearest bf16 to what is left: hi + mid + lo is v exactly (24 bits in 8 and two signs), |mid| <= 2^-8 |v| and
+// |lo| <= 2^-16 |v| of either sign, so that the products left out, mid lo + lo mid + lo lo, are at most 2^-23 of v w and cancel in long
+// sums (cut off instead of rounded the terms all have v's sign: up to 2^-21, always towards 0).  The same number of instructions: the
+// conversion makes two values at once.  hi overflows above the largest bf16: see LinEpilogue::exact
+typedef float lin_f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 lin_bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void lin_pack(const float (&v)[8], LinChunk<float>& c) {
-  unsigned h[8], m[8], l[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {  // truncation: hi + mid + lo is v exactly, and no rounding can overflow
-    h[i] = __float_as_uint(v[i]) & 0xFFFF0000u;
-    const float r = v[i] - __uint_as_float(h[i]);
-    m[i] = __float_as_uint(r) & 0xFFFF0000u;
-    l[i] = __float_as_uint(r - __uint_as_float(m[i]));
-  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    c.p[0][i] = __builtin_amdgcn_perm(h[2 * i + 1], h[2 * i], 0x07060302u);
-    c.p[1][i] = __builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x07060302u);
-    c.p[2][i] = __builtin_amdgcn_perm(l[2 * i + 1], l[2 * i], 0x07060302u);
+    lin_f32x2 r = {v[2 * i], v[2 * i + 1]};
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const unsigned q = __builtin_bit_cast(unsigned, __builtin_convertvector(r, lin_bf16x2));
+      c.p[p][i] = q;
+      if (p < 2) r = (lin_f32x2){r[0] - __uint_as_float(q << 16), r[1] - __uint_as_float(q & 0xFFFF0000u)};
+    }
   }
 }
 __device__ __forceinline__ void lin_pack(const pp_bf16 (&v)[8], LinChunk<pp_bf16>& c) { __builtin_memcpy(&c.p[0], v, 16); }

@@ -234,3 +234,17 @@ def test_largest_numbers_of_fp32():
     y = ops.linear_act_fwd(x, w).double()
     want = (x.double() @ w.double().t())
     assert torch.equal(y, want.float().double()), (y, want)
+
+
+def test_fp32_products_leave_out_little_and_on_both_sides():
+    """one product per result: three bf16 terms of each operand, the middle one at most 2^-8 and the last 2^-16 of it, so the three products that
+    are left out are at most (2 2^-24 + 2^-32) = 2.01 u of it; the addition of the largest rounds once more, by a whole step (2 u) at most"""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x, w = (1 + torch.rand((2000, 1), generator=gen, device="cuda")), (1 + torch.rand((1000, 1), generator=gen, device="cuda"))
+    off = ops.linear_act_fwd(x, w).double() / (x.double() @ w.double().t()) - 1
+    assert float(off.abs().max()) <= 4.01 * u, float(off.abs().max() / u)
+    # sums of positive terms: a step of 32 terms is six additions, each off by a whole step (2 u) at most of partial sums that grow evenly, and
+    # at most one more inside it
+    x, w = (0.5 + torch.rand((300, 512), generator=gen, device="cuda")), (0.5 + torch.rand((200, 512), generator=gen, device="cuda"))
+    off = ops.linear_act_fwd(x, w).double() / (x.double() @ w.double().t()) - 1
+    assert float(off.abs().max()) <= (2.01 + 512 / 32 * 6 * 2) * u
