@@ -719,18 +719,24 @@ static int lin_tile(const LinArgs& a, int splits, hipStream_t s) {
 }
 
 
-// parts of the weight gradient's contraction: about two workgroups per compute unit, at least 256 rows (wide kernel: 512) each
-static int lin_splits(int64_t n, int cin, int cout, bool wide) {
+// parts of the weight gradient's contraction: about two workgroups per compute unit, at least 256 rows (wide kernel: 512) each, and at most
+// as many as a chain of fp32 additions stands: 2048 in fp32 (64 steps of six: terms of one sign lose 384 2^-24 of their sum at most; they
+// lost 9e-5 of 10 M rows in 512 parts), 65536 in 16 bits (2048 steps: 2048 2^-24, a quarter of fp16's half step)
+static int lin_splits(int64_t n, int cin, int cout, bool wide, size_t bytes) {
   const int64_t tiles = (int64_t)((cout + 127) / 128) * ((cin + (cin > 64 ? 127 : 63)) / (cin > 64 ? 128 : 64));
-  const int64_t rows = wide ? 512 : 256;
+  const int64_t rows = wide ? 512 : 256, most = bytes == 4 ? 2048 : 65536;
   int64_t s = 512 / tiles;
   if (s > (n + rows - 1) / rows) s = (n + rows - 1) / rows;
-  return s < 1 ? 1 : (int)s;
+  if (s < (n + most - 1) / most) s = (n + most - 1) / most;
+  return s < 1 ? 1 : s > 65535 ? 65535 : (int)s;  // (the launch's third dimension)
 }
 #define LIN_SUM_GROUPS 32
 #define LIN_COLUMN_PARTS 512  // at most; a part has at least LIN_COLUMN_ROWS rows
 #define LIN_COLUMN_ROWS 1024
 #define LIN_STREAM_GRID_MAX 256
+// more parts than this are added in LIN_SUM_GROUPS groups first, whose sums lie behind them
+#define LIN_SUM_DIRECT 512
+static size_t lin_sum_rows(int64_t parts) { return (size_t)(parts > LIN_SUM_DIRECT ? parts + LIN_SUM_GROUPS : parts); }
 static int64_t lin_ldz(int cout) { return (cout + 7) / 8 * 8; }
 
 // workgroups of the narrow kernel: what finds room on the chip at once (two of a compute unit forward, up to 96 channels; the registers leave
@@ -751,13 +757,14 @@ static size_t lin_bias_rows(int64_t n, int act) {
 
 extern "C" size_t pp_linear_act_bwd_workspace(int32_t dtype, int64_t n, int32_t cin, int32_t cout, int32_t act) {
   if (n < 0 || cin < 1 || cout < 1) return 0;
-  const size_t p0 = (size_t)lin_splits(n, cin, cout, false), p1 = (size_t)lin_splits(n, cin, cout, true), parts = p0 > p1 ? p0 : p1;
+  const int p0 = lin_splits(n, cin, cout, false, pp_dtype_bytes(dtype)), p1 = lin_splits(n, cin, cout, true, pp_dtype_bytes(dtype));
+  const size_t parts = lin_sum_rows(p0 > p1 ? p0 : p1);
   const size_t bias = lin_bias_rows(n, act);
   return pp_align(parts * cout * cin * 4) + pp_align(bias * cout * 4) +
          (act == PP_ACT_NONE ? 0 : pp_align((size_t)n * lin_ldz(cout) * pp_dtype_bytes(dtype))) + 256;
 }
 
-// sums of `parts` rows of n values; more than a few hundred rows go through LIN_SUM_GROUPS partial rows behind them
+// sums of `parts` rows of n values (room: lin_sum_rows)
 template <typename T>
 static int lin_sum(float* part, int64_t parts, int64_t n, T* out, hipStream_t s) {
   if (parts <= 16 && n % 4 == 0 && n >= 65536) {
@@ -765,7 +772,7 @@ static int lin_sum(float* part, int64_t parts, int64_t n, T* out, hipStream_t s)
     PP_LAUNCH_CHECK();
     return PP_OK;
   }
-  if (parts > 512) {
+  if (parts > LIN_SUM_DIRECT) {
     float* const mid = part + parts * n;
     hipLaunchKernelGGL((k_linear_sum<float>), dim3((unsigned)((n + 15) / 16), LIN_SUM_GROUPS), dim3(256), 0, s, part, parts, n, 16, mid);
     part = mid;
@@ -853,8 +860,8 @@ static int lin_forward(const void* x, int64_t n, int cin, const void* w, int cou
 template <typename T>
 static int lin_backward(const void* x, const void* dy, int64_t n, int cin, const void* w, int cout, const void* bias, int act, float slope,
                         void* dx, void* dw, void* db, PPArena& ws, hipStream_t s) {
-  const int p0 = lin_splits(n, cin, cout, false), p1 = lin_splits(n, cin, cout, true);
-  float* part = ws.take<float>((size_t)(p0 > p1 ? p0 : p1) * cout * cin);
+  const int p0 = lin_splits(n, cin, cout, false, sizeof(T)), p1 = lin_splits(n, cin, cout, true, sizeof(T));
+  float* part = ws.take<float>(lin_sum_rows(p0 > p1 ? p0 : p1) * cout * cin);
   float* part_bias = ws.take<float>(lin_bias_rows(n, act) * cout);
   PP_REQUIRE(part && part_bias, "pp_linear_act_bwd: workspace layout");
   const T* dz = (const T*)dy;

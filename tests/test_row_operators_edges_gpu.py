@@ -248,3 +248,15 @@ def test_fp32_products_leave_out_little_and_on_both_sides():
     x, w = (0.5 + torch.rand((300, 512), generator=gen, device="cuda")), (0.5 + torch.rand((200, 512), generator=gen, device="cuda"))
     off = ops.linear_act_fwd(x, w).double() / (x.double() @ w.double().t()) - 1
     assert float(off.abs().max()) <= (2.01 + 512 / 32 * 6 * 2) * u
+
+
+@pytest.mark.parametrize("n,cin,cout", [(10_000_000, 64, 32), (3_000_001, 130, 260), (300_000, 20, 600)])
+def test_weight_gradients_of_one_sign_over_many_rows(n, cin, cout):
+    """fp32, every product the same.  At most 2048 rows are one chain of fp32 additions, 64 steps of six: each is off by a whole step (2 u) at most
+    of partial sums that grow evenly.  The split leaves out 2.01 u, and the parts are rounded, added in fp64 and rounded"""
+    x, dy = torch.full((n, cin), 0.1, device="cuda"), torch.full((n, cout), 0.3, device="cuda")
+    w = torch.zeros((cout, cin), device="cuda")
+    dw = ops.linear_act_bwd(x, dy, w, None, 0, want_input=False, want_bias=False)[1]
+    off = dw.double() / (x[0, 0].double() * dy[0, 0].double() * n) - 1
+    assert float(off.abs().max()) <= (64 * 6 + 2.01 + 4) * u, float(off.abs().max() / u)
+    assert int((dw != dw[0, 0]).sum()) == 0
