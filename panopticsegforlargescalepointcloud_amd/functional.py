@@ -1,7 +1,14 @@
 """Differentiable row operators on [rows, channels] features: thin autograd nodes over ops.* (csrc/pp_groupnorm.hip, pp_linear.hip)."""
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
+
+
+def _refuse_tangents(name, *tensors):
+    """the operators have no forward-mode derivative: a tangent is refused, not dropped (the level is -1 outside forward_ad.dual_level)"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("%s has no forward-mode derivative" % name)
 
 
 class _GroupNormActFn(torch.autograd.Function):
@@ -36,6 +43,7 @@ def group_norm_act(x, offsets, num_groups, weight=None, bias=None, eps=1e-5, act
     get zero gradients.  activation: none, relu, leaky_relu (with `slope`), silu or gelu (exact).  num_groups = c: instance norm.
     Beside FastBatchNorm1d: the result for a row does not depend on the other batch elements, in training and in inference."""
     act = ops.activation_id(activation)
+    _refuse_tangents("group_norm_act", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _GroupNormActFn.apply(x, offsets, num_groups, weight, bias, eps, act, slope, order)
@@ -67,6 +75,7 @@ def linear_act(x, weight, bias=None, activation="none", slope=0.2, residual=None
     layout of torch.nn.Linear), bias [cout] or None, residual [n, cout] or None, all of one type (float32, bfloat16, float16).
     activation: none, relu, leaky_relu (with `slope`), silu or gelu (exact); it acts before the residual is added, as in ResBlock."""
     act = ops.activation_id(activation)
+    _refuse_tangents("linear_act", x, weight, bias, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return _LinearActFn.apply(x, weight, bias, act, slope, residual)
     return ops.linear_act_fwd(x, weight, bias, act, slope, residual)

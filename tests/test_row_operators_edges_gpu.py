@@ -260,3 +260,18 @@ def test_weight_gradients_of_one_sign_over_many_rows(n, cin, cout):
     off = dw.double() / (x[0, 0].double() * dy[0, 0].double() * n) - 1
     assert float(off.abs().max()) <= (64 * 6 + 2.01 + 4) * u, float(off.abs().max() / u)
     assert int((dw != dw[0, 0]).sum()) == 0
+
+
+def test_tangents_are_refused_not_dropped():
+    x, t = torch.randn(6, 8, device="cuda"), torch.randn(6, 8, device="cuda")
+    w, off = torch.randn(8, 8, device="cuda"), torch.tensor([0, 6], device="cuda")
+    scale = torch.ones(8, device="cuda")
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        dual = torch.autograd.forward_ad.make_dual(x, t)
+        for call in (lambda: modules.linear_act(dual, w), lambda: modules.linear_act(x, torch.autograd.forward_ad.make_dual(w, w)),
+                     lambda: modules.linear_act(x, w, None, residual=dual), lambda: modules.group_norm_act(dual, off, 2),
+                     lambda: modules.group_norm_act(x, off, 2, torch.autograd.forward_ad.make_dual(scale, scale))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert torch.equal(modules.linear_act(x, w), ops.linear_act_fwd(x, w))
+    assert torch.equal(modules.group_norm_act(x, off, 2), ops.group_norm_fwd(x, off, 2)[0])
