@@ -71,11 +71,26 @@ class _LinearActFn(torch.autograd.Function):
 
 
 def linear_act(x, weight, bias=None, activation="none", slope=0.2, residual=None):
-    """y = act(x W^T + bias) + residual as one launch, differentiable in all four operands.  x [n, cin], weight [cout, cin] (the
-    layout of torch.nn.Linear), bias [cout] or None, residual [n, cout] or None, all of one type (float32, bfloat16, float16).
+    """y = act(x W^T + bias) + residual as one launch, differentiable in all four operands.  x [..., cin], weight [cout, cin] (the
+    layout of torch.nn.Linear), bias [cout] or None, residual [..., cout] or None, all of one type (float32, bfloat16, float16); under
+    torch.autocast they are brought to its type, as torch.nn.functional.linear's are.
     activation: none, relu, leaky_relu (with `slope`), silu or gelu (exact); it acts before the residual is added, as in ResBlock."""
     act = ops.activation_id(activation)
     _refuse_tangents("linear_act", x, weight, bias, residual)
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
+        x, weight, bias, residual = (t if t is None or t.dtype == torch.float64 else t.to(dtype) for t in (x, weight, bias, residual))
+    if x.dim() != 2:
+        if x.dim() == 0 or (residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0])):
+            raise ValueError("linear_act: input %s, weight %s and residual %s do not fit" % (
+                tuple(x.shape), tuple(weight.shape), None if residual is None else tuple(residual.shape)))
+        rows = x.reshape(x.shape[:-1].numel(), x.shape[-1])
+        more = None if residual is None else residual.reshape(rows.shape[0], weight.shape[0])
+        return _linear_act(rows, weight, bias, act, slope, more).view(*x.shape[:-1], weight.shape[0])
+    return _linear_act(x, weight, bias, act, slope, residual)
+
+
+def _linear_act(x, weight, bias, act, slope, residual):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return _LinearActFn.apply(x, weight, bias, act, slope, residual)
     return ops.linear_act_fwd(x, weight, bias, act, slope, residual)

@@ -262,6 +262,43 @@ def test_weight_gradients_of_one_sign_over_many_rows(n, cin, cout):
     assert int((dw != dw[0, 0]).sum()) == 0
 
 
+def test_linear_layers_take_what_their_parent_takes():
+    """any leading dimensions, and mixed types under autocast (the results of linear layers have its type)"""
+    torch.manual_seed(1)
+    layer = modules.LinearAct(24, 40, activation="silu").cuda()
+    for shape in ((24,), (5, 24), (3, 7, 24), (2, 3, 4, 24), (0, 24), (4, 0, 24)):
+        x = torch.randn(shape, device="cuda", requires_grad=True)
+        res = torch.randn(*shape[:-1], 40, device="cuda", requires_grad=True)
+        y = layer(x, res)
+        assert y.shape == (*shape[:-1], 40)
+        rows = ops.linear_act_fwd(x.detach().reshape(-1, 24), layer.weight.detach(), layer.bias.detach(), 3, 0.0, res.detach().reshape(-1, 40))
+        assert torch.equal(y.detach().reshape(-1, 40), rows)
+        dy = torch.randn_like(y)
+        gx, gr = torch.autograd.grad(y, (x, res), dy)
+        want = ops.linear_act_bwd(x.detach().reshape(-1, 24), dy.reshape(-1, 40), layer.weight.detach(), layer.bias.detach(), 3)[0]
+        assert torch.equal(gx.reshape(-1, 24), want) and torch.equal(gr, dy)
+    strided = torch.randn(6, 24, 5, device="cuda").transpose(1, 2)
+    assert torch.equal(layer(strided), layer(strided.contiguous()))
+    for bad in ((torch.randn((), device="cuda"), None), (torch.randn(3, 7, 23, device="cuda"), None),
+                (torch.randn(3, 7, 24, device="cuda"), torch.randn(7, 3, 40, device="cuda"))):
+        with pytest.raises(ValueError):
+            layer(*bad)
+    for dtype in (torch.bfloat16, torch.float16):
+        x = torch.randn(300, 24, device="cuda", requires_grad=True)
+        with torch.autocast("cuda", dtype=dtype):
+            y = layer(x)
+            inner = layer(x.to(dtype), torch.zeros(300, 40, device="cuda"))
+        assert y.dtype == inner.dtype == dtype
+        low = lambda t: t.detach().to(dtype)  # noqa: E731
+        assert torch.equal(y, ops.linear_act_fwd(low(x), low(layer.weight), low(layer.bias), 3)) and torch.equal(inner, y)
+        dy = torch.randn_like(y)
+        grads = torch.autograd.grad(y, (x, layer.weight, layer.bias), dy)
+        want = ops.linear_act_bwd(low(x), dy, low(layer.weight), low(layer.bias), 3)
+        assert all(g.dtype == torch.float32 and torch.equal(g, w.float()) for g, w in zip(grads, want))
+        with pytest.raises(TypeError):
+            layer(x.to(dtype))  # without autocast: types are not mixed
+
+
 def test_tangents_are_refused_not_dropped():
     x, t = torch.randn(6, 8, device="cuda"), torch.randn(6, 8, device="cuda")
     w, off = torch.randn(8, 8, device="cuda"), torch.tensor([0, 6], device="cuda")
