@@ -427,7 +427,8 @@ int pp_linear_act_bwd(const void* x, const void* dy, int32_t dtype, int64_t n, i
  * X <- a X + (b A + c A^2) X with A = X X^T on the shorter side (at most 8192).  Computed on the Gram matrix of the shorter side in
  * float64; results repeat bit for bit.
  * ---------------------------------------------------------------------------------------------- */
-size_t pp_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n);
+size_t pp_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n);  /* for any type and number of steps */
+size_t pp_newton_schulz_workspace_for(int32_t dtype, int64_t batch, int64_t m, int64_t n, int32_t steps);
 int pp_newton_schulz(const void* g, int32_t dtype, int64_t batch, int64_t m, int64_t n, int32_t steps, double a, double b, double c,
                      double eps, void* out, void* ws, size_t ws_bytes, pp_stream_t stream);
 

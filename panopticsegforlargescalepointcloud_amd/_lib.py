@@ -106,6 +106,7 @@ SIGNATURES = {
     "pp_linear_act_bwd_workspace": (sz, [i32, i64, i32, i32, i32]),
     "pp_linear_act_bwd": (C.c_int, [vp, vp, i32, i64, i32, vp, i32, vp, i32, f32, vp, vp, vp, vp, sz, vp]),
     "pp_newton_schulz_workspace": (sz, [i64, i64, i64]),
+    "pp_newton_schulz_workspace_for": (sz, [i32, i64, i64, i64, i32]),
     "pp_newton_schulz": (C.c_int, [vp, i32, i64, i64, i64, i32, f64, f64, f64, f64, vp, vp, sz, vp]),
     "pp_head_mlp": (C.c_int, [vp, i64, i32, vp, i32, vp, vp, vp, vp, i32, i32, vp, vp, vp]),
     "pp_linear_rows": (C.c_int, [vp, vp, vp, i64, i32, i32, i32, vp, vp]),

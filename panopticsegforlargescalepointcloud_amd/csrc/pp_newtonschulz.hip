@@ -4,7 +4,9 @@
 // of all P: the long matrix is read twice (for S, and to be multiplied by Q) instead of three times a step, and the steps work on
 // matrices of the short side only.  S, P and Q are symmetric and commute, so half of each product's tiles is computed and mirrored.
 // S is held and multiplied in fp64: in the directions of small singular values P is a I, so rounding errors of S grow by a^2 = 11.9 a
-// step there; fp64 leaves 1e-12 of them after five steps, fp32 would leave 1e-2.  |G|^2 is the trace of S.
+// step there; fp64 leaves 1e-12 of them after five steps, fp32 would leave 1e-2.  |G|^2 is the trace of S.  Behind some fifteen steps even
+// fp64's errors have grown to the size of S (the Q of directions that G does not have grows by a each step without end), so longer calls
+// go in rounds: at most NS_ROUND steps are one, more are rounds of NS_ROUND_LONG, between which X is written in fp32 and S formed anew.
 // Above it: the iteration as it is written, on the bf16 matrix pipe with operands in two or three planes (further down).
 #include "pp_gemm.h"
 
@@ -20,6 +22,8 @@ typedef double ns_f64x4 __attribute__((ext_vector_type(4)));
 // product (waves behind the last block repeat it: no branches around the MFMAs).  A product is N / 4 MFMAs of 64 cycles a wave, two
 // waves a SIMD: at N = 96 1.3 us of it, four in a row.
 #define NS_PANEL_MAX 128
+#define NS_ROUND 8
+#define NS_ROUND_LONG 5
 
 template <int SB>
 struct NsPanel {
@@ -37,11 +41,12 @@ struct NsPanel {
 };
 
 struct NsStepArgs {
-  const double *S, *Q;  // [batch][s][s]; Q null: the identity times alpha (first step)
+  const double *S, *Q;  // [batch][s][s]; Q null: the identity times alpha (first step of a round)
   double *S2, *Q2;      // S2 null: not wanted (last step)
   int64_t s;
   double a, b, c;
   double eps;           // first step: S is the unscaled one, alpha = 1 / (sqrt(trace S) + eps)
+  int scaled;           // later rounds: S is that of an X of this iteration, alpha = 1
 };
 
 // a symmetric [s][s] matrix into the LDS, zeros around it; 512 threads
@@ -80,7 +85,7 @@ __global__ __launch_bounds__(512) void k_ns_step(NsStepArgs g) {
   ns_square<SB>(S, gS, s);
   double alpha = 1.0;
   __syncthreads();
-  if (first) {
+  if (first && !g.scaled) {
     double v = 0.0;
     for (int i = threadIdx.x; i < N; i += 512) v += S[P::at(i, i)];
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
@@ -239,9 +244,9 @@ __global__ __launch_bounds__(512) void k_ns_part_gram(const T* __restrict__ g, i
 }
 
 // out = X Q (tall) or Q X of a part; alpha is in Q
-template <typename T, int SB>
+template <typename T, typename O, int SB>
 __global__ __launch_bounds__(512) void k_ns_part_apply(const T* __restrict__ g, int64_t m, int64_t n, int vec, const double* __restrict__ Q,
-                                                       T* __restrict__ out) {
+                                                       O* __restrict__ out) {
   typedef NsPanel<SB> P;
   typedef NsPart<SB, true> X;
   constexpr int N = SB * 16, TILES = SB * (NS_LONG / 16), PER = TILES / 8 + (TILES % 8 != 0);
@@ -272,7 +277,7 @@ __global__ __launch_bounds__(512) void k_ns_part_apply(const T* __restrict__ g, 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = (tall ? tl : ts) * 16 + q + 4 * e, c = (tall ? ts : tl) * 16 + j;
-      if (r < (tall ? len : (int)s) && c < (tall ? (int)s : len)) out[corner + r * n + c] = (T)(float)acc[i][e];
+      if (r < (tall ? len : (int)s) && c < (tall ? (int)s : len)) out[corner + r * n + c] = (O)(float)acc[i][e];
     }
   }
 }
@@ -528,11 +533,15 @@ static size_t ns_large_ws(PPArena* ws, int planes, int64_t batch, int64_t m, int
   return total;
 }
 
-extern "C" size_t pp_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n) {
+extern "C" size_t pp_newton_schulz_workspace_for(int32_t dtype, int64_t batch, int64_t m, int64_t n, int32_t steps) {
   if (batch < 0 || m < 1 || n < 1 || m > 65536 * 64 || n > 65536 * 64) return 0;
   const int64_t s = m < n ? m : n, l = m < n ? n : m;
-  if (s > NS_PANEL_MAX) return ns_large_ws(nullptr, 3, batch > 0 ? batch : 1, m, n, nullptr) + 256;
-  return pp_align((size_t)ns_parts(l) * batch * s * s * sizeof(double)) + 4 * pp_align((size_t)batch * s * s * sizeof(double)) + 256;
+  if (s > NS_PANEL_MAX) return ns_large_ws(nullptr, dtype == PP_F32 ? 3 : 2, batch > 0 ? batch : 1, m, n, nullptr) + 256;
+  return pp_align((size_t)ns_parts(l) * batch * s * s * sizeof(double)) + 4 * pp_align((size_t)batch * s * s * sizeof(double)) +
+         (steps > NS_ROUND ? 2 * pp_align((size_t)batch * m * n * sizeof(float)) : 0) + 256;
+}
+extern "C" size_t pp_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n) {
+  return pp_newton_schulz_workspace_for(PP_F32, batch, m, n, NS_ROUND + 1);  // (what needs most)
 }
 
 template <int SB>
@@ -550,12 +559,12 @@ static int ns_part_gram_launch(const T* g, int64_t m, int64_t n, int splits, int
   PP_LAUNCH_CHECK();
   return PP_OK;
 }
-template <typename T, int SB>
-static int ns_part_apply_launch(const T* g, int64_t m, int64_t n, int vec, const double* Q, T* out, unsigned batch, hipStream_t st) {
+template <typename T, typename O, int SB>
+static int ns_part_apply_launch(const T* g, int64_t m, int64_t n, int vec, const double* Q, O* out, unsigned batch, hipStream_t st) {
   const size_t lds = (size_t)SB * 16 * SB * 16 * sizeof(double) + NsPart<SB, true>::FLOATS * sizeof(float);
-  PP_HIP(hipFuncSetAttribute((const void*)k_ns_part_apply<T, SB>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  PP_HIP(hipFuncSetAttribute((const void*)k_ns_part_apply<T, O, SB>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   const int64_t l = m >= n ? m : n;
-  hipLaunchKernelGGL((k_ns_part_apply<T, SB>), dim3((unsigned)((l + NS_LONG - 1) / NS_LONG), batch), dim3(512), lds, st, g, m, n, vec, Q, out);
+  hipLaunchKernelGGL((k_ns_part_apply<T, O, SB>), dim3((unsigned)((l + NS_LONG - 1) / NS_LONG), batch), dim3(512), lds, st, g, m, n, vec, Q, out);
   PP_LAUNCH_CHECK();
   return PP_OK;
 }
@@ -582,9 +591,9 @@ static int ns_part_gram(const T* g, int64_t m, int64_t n, int64_t s, int splits,
   NS_BY_BLOCKS(NS_CALL)
 #undef NS_CALL
 }
-template <typename T>
-static int ns_part_apply(const T* g, int64_t m, int64_t n, int64_t s, int vec, const double* Q, T* out, unsigned batch, hipStream_t st) {
-#define NS_CALL(SB) ns_part_apply_launch<T, SB>(g, m, n, vec, Q, out, batch, st)
+template <typename T, typename O>
+static int ns_part_apply(const T* g, int64_t m, int64_t n, int64_t s, int vec, const double* Q, O* out, unsigned batch, hipStream_t st) {
+#define NS_CALL(SB) ns_part_apply_launch<T, O, SB>(g, m, n, vec, Q, out, batch, st)
   NS_BY_BLOCKS(NS_CALL)
 #undef NS_CALL
 }
@@ -665,30 +674,46 @@ static int ns_large(const T* g, int64_t batch, int64_t m, int64_t n, int steps, 
   return PP_OK;
 }
 
-template <typename T>
-static int ns_run(const void* g, int64_t batch, int64_t m, int64_t n, int steps, double ca, double cb, double cc, double eps, void* out,
-                  PPArena& ws, hipStream_t st) {
-  const int64_t s = m < n ? m : n, l = m < n ? n : m;
-  if (s > NS_PANEL_MAX) return ns_large<T, sizeof(T) == 2 ? 2 : 3>((const T*)g, batch, m, n, steps, ca, cb, cc, eps, (T*)out, ws, st);
-  const int splits = ns_parts(l);
-  double* part = ws.take<double>((size_t)splits * batch * s * s);
-  double* mats[4];
-  for (double*& p : mats) p = ws.take<double>((size_t)batch * s * s);
-  PP_REQUIRE(part && mats[3], "pp_newton_schulz: workspace layout");
+// one round for short sides up to NS_PANEL_MAX: out = X times the polynomials of its S, `steps` of them
+template <typename T, typename O>
+static int ns_round(const T* x, int64_t batch, int64_t m, int64_t n, NsStepArgs p, int steps, O* out, double* part, double* const (&mats)[4], hipStream_t st) {
+  const int64_t s = p.s;
+  const int splits = ns_parts(m < n ? n : m);
   const unsigned nb = (unsigned)batch;
-  const int vec = n % 4 == 0 && (uintptr_t)g % (4 * sizeof(T)) == 0;
-  int rc = ns_part_gram<T>((const T*)g, m, n, s, splits, vec, part, nb, st);
+  const int vec = n % 4 == 0 && (uintptr_t)x % (4 * sizeof(T)) == 0;
+  int rc = ns_part_gram<T>(x, m, n, s, splits, vec, part, nb, st);
   if (rc != PP_OK) return rc;
   hipLaunchKernelGGL(k_ns_sum, dim3((unsigned)((s * s + 31) / 32), nb), dim3(256), 0, st, part, splits, s, mats[0]);
   PP_LAUNCH_CHECK();
-  NsStepArgs p{};
-  p.s = s; p.a = ca; p.b = cb; p.c = cc; p.eps = eps;
   for (int k = 0; k < steps; ++k) {  // S in mats[0], mats[1] in turn, Q in mats[2], mats[3]
     p.S = mats[k & 1]; p.S2 = k == steps - 1 ? nullptr : mats[~k & 1];
     p.Q = k == 0 ? nullptr : mats[2 + (~k & 1)]; p.Q2 = mats[2 + (k & 1)];
     if ((rc = ns_step(p, nb, st)) != PP_OK) return rc;
   }
-  return ns_part_apply<T>((const T*)g, m, n, s, vec, mats[2 + (~steps & 1)], (T*)out, nb, st);
+  return ns_part_apply<T, O>(x, m, n, s, vec, mats[2 + (~steps & 1)], out, nb, st);
+}
+
+template <typename T>
+static int ns_run(const void* g, int64_t batch, int64_t m, int64_t n, int steps, double ca, double cb, double cc, double eps, void* out,
+                  PPArena& ws, hipStream_t st) {
+  const int64_t s = m < n ? m : n;
+  if (s > NS_PANEL_MAX) return ns_large<T, sizeof(T) == 2 ? 2 : 3>((const T*)g, batch, m, n, steps, ca, cb, cc, eps, (T*)out, ws, st);
+  double* part = ws.take<double>((size_t)ns_parts(m < n ? n : m) * batch * s * s);
+  double* mats[4];
+  for (double*& p : mats) p = ws.take<double>((size_t)batch * s * s);
+  PP_REQUIRE(part && mats[3], "pp_newton_schulz: workspace layout");
+  NsStepArgs p{};
+  p.s = s; p.a = ca; p.b = cb; p.c = cc; p.eps = eps;
+  if (steps <= NS_ROUND) return ns_round<T, T>((const T*)g, batch, m, n, p, steps, (T*)out, part, mats, st);
+  float* X[2];
+  for (float*& x : X) x = ws.take<float>((size_t)batch * m * n);
+  PP_REQUIRE(X[1], "pp_newton_schulz: workspace layout");
+  int rc = ns_round<T, float>((const T*)g, batch, m, n, p, NS_ROUND_LONG, X[0], part, mats, st);
+  p.scaled = 1;
+  int at = 0;
+  for (steps -= NS_ROUND_LONG; rc == PP_OK && steps > NS_ROUND_LONG; steps -= NS_ROUND_LONG, at ^= 1)
+    rc = ns_round<float, float>(X[at], batch, m, n, p, NS_ROUND_LONG, X[at ^ 1], part, mats, st);
+  return rc == PP_OK ? ns_round<float, T>(X[at], batch, m, n, p, steps, (T*)out, part, mats, st) : rc;
 }
 
 extern "C" int pp_newton_schulz(const void* g, int32_t dtype, int64_t batch, int64_t m, int64_t n, int32_t steps, double ca, double cb,
@@ -700,7 +725,7 @@ extern "C" int pp_newton_schulz(const void* g, int32_t dtype, int64_t batch, int
   PP_REQUIRE(eps >= 0.0, "pp_newton_schulz: eps must not be negative");
   if (batch == 0) return PP_OK;
   PP_REQUIRE(g && out && ws && (uintptr_t)ws % 16 == 0, "pp_newton_schulz: null or unaligned pointer");
-  if (ws_bytes < pp_newton_schulz_workspace(batch, m, n)) {
+  if (ws_bytes < pp_newton_schulz_workspace_for(dtype, batch, m, n, steps)) {
     pp_set_error("pp_newton_schulz: workspace too small");
     return PP_ERR_WORKSPACE;
   }

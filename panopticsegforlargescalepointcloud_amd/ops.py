@@ -1426,7 +1426,7 @@ def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7)
     a, b, c = coefficients
     g = g if g.is_contiguous() else g.contiguous()
     out = torch.empty_like(g)
-    wsb = lib.pp_newton_schulz_workspace(batch, m, n)
+    wsb = lib.pp_newton_schulz_workspace_for(code, batch, m, n, int(steps))
     ws = _ws(wsb, g.device)
     _lib.check(lib.pp_newton_schulz(_at(g), code, batch, m, n, int(steps), float(a), float(b), float(c), float(eps), _at(out), _at(ws),
                                     ws.numel(), _stream()), "pp_newton_schulz")

@@ -312,3 +312,68 @@ def test_tangents_are_refused_not_dropped():
                 call()
         assert torch.equal(modules.linear_act(x, w), ops.linear_act_fwd(x, w))
     assert torch.equal(modules.group_norm_act(x, off, 2), ops.group_norm_fwd(x, off, 2)[0])
+
+
+def rounds(g, steps, coefficients):
+    """the iteration in 64 bits, and what the rounding of X to fp32 after every fifth step can make of it: an error grows by at most
+    max |p'(sigma)| over the singular values that a step meets, p(x) = a x + b x^3 + c x^5"""
+    a, b, c = coefficients
+    x = g.double().cpu()
+    x = x / (x.norm() + 1e-7)
+    tall = x.shape[0] > x.shape[1]
+    x = x.t() if tall else x
+    bound = 0.0
+    for k in range(steps):
+        s = x @ x.t()
+        lam = torch.linalg.eigvalsh(s).clamp(min=0)
+        bound = bound * float((a + 3 * b * lam + 5 * c * lam * lam).abs().max()) + 1e-11  # (a round of five in fp64)
+        x = a * x + (b * s + c * (s @ s)) @ x
+        if steps > 8 and (k + 1) % 5 == 0 and k + 1 < steps:
+            bound += u * float(x.norm())
+    return (x.t() if tall else x), bound
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n", [(64, 64), (300, 48), (40, 333), (128, 1000)])
+def test_newton_schulz_of_many_steps(dtype, m, n):
+    gen = torch.Generator().manual_seed(m + n)
+    g = torch.randn((m, n), generator=gen)
+    if m == n:
+        g = g + 8 * torch.eye(m)
+    g = g.to(dtype)
+    for coefficients in (ops.NEWTON_SCHULZ_COEFFICIENTS, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5)):
+        for steps in (8, 9, 10, 11, 13, 30):
+            if steps == 30 and coefficients[0] > 3:
+                continue  # (its singular values never settle: errors go on growing, in every precision)
+            want, bound = rounds(g, steps, coefficients)
+            got = ops.newton_schulz(g.cuda(), steps, coefficients).double().cpu()
+            assert float((got - want).norm()) <= bound + (u + HALF_STEP[dtype]) * float(want.norm()) + TINY[dtype] * want.numel() ** 0.5, (steps, coefficients)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_newton_schulz_of_many_steps_keeps_missing_directions_small(dtype):
+    """a matrix that lacks directions: they stay what rounding makes of them, and no singular value leaves the range that the polynomial maps
+    to itself (p has its largest value, 1.21, at 0.56, and stays above 0.68 from there to 1.21)"""
+    gen = torch.Generator().manual_seed(7)
+    draw = lambda *s: torch.randn(s, generator=gen)  # noqa: E731
+    twice, zero = draw(64, 64), draw(200, 48)
+    twice[:, :32] = twice[:, 32:]
+    zero[:, 5] = zero[:, 9] = 0
+    for g in (twice, zero, draw(90, 1) @ draw(1, 60), draw(300, 10) @ draw(10, 64), draw(7, 1), torch.zeros(20, 30)):
+        for steps in (9, 12, 16, 20, 40, 100):
+            out = ops.newton_schulz(g.to(dtype).cuda(), steps)
+            assert bool(torch.isfinite(out).all()), (tuple(g.shape), steps)
+            # bfloat16's half step of every entry: at most 2^-8 |out|_F, with |out|_F^2 <= 64 values of 1.21^2
+            assert float(torch.linalg.svdvals(out.double().cpu()).max()) <= 1.21 + (HALF_STEP[dtype] + 4 * u) * 1.21 * 8, (tuple(g.shape), steps)
+            if g is zero:
+                assert int(out[:, 5].count_nonzero()) == 0
+    static = twice.to(dtype).cuda()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.newton_schulz(static, 21)
+    for k in range(3):
+        static.copy_(twice.roll(k, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.newton_schulz(static, 21)), k
