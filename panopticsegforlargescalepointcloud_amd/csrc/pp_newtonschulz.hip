@@ -207,15 +207,17 @@ struct NsPart {
   }
 };
 
-// S of a part: its tiles on and below the diagonal, the eight waves in turn
+// S of every splits-th part: its tiles on and below the diagonal, the eight waves in turn.  A workgroup per part as long as all of them find
+// room on the chip at once (NS_GRAM_BLOCKS: four of a compute unit), a whole number of parts each behind that: what they leave behind
+// for k_ns_sum is s^2 fp64 a workgroup, which a workgroup per part made six times the matrix itself ([4 M, 96] x 6: 27 GB)
+#define NS_GRAM_BLOCKS 1024
 template <typename T, int SB>
 __global__ __launch_bounds__(512) void k_ns_part_gram(const T* __restrict__ g, int64_t m, int64_t n, int splits, int vec, double* __restrict__ part) {
   constexpr int TILES = SB * (SB + 1) / 2, PER = (TILES + 7) / 8;
   typedef NsPart<SB, false> X;
   __shared__ float x[X::FLOATS];
   const bool tall = m >= n;
-  const int64_t s = tall ? n : m, l = tall ? m : n, l0 = (int64_t)blockIdx.x * NS_LONG, batch = blockIdx.y;
-  X::load(x, g + batch * m * n + (tall ? l0 * n : l0), tall, n, (int)s, (int)(l - l0 < NS_LONG ? l - l0 : NS_LONG), vec);
+  const int64_t s = tall ? n : m, l = tall ? m : n, batch = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, q = lane >> 4;
   int ta[PER], tb[PER];
 #pragma unroll
@@ -226,13 +228,17 @@ __global__ __launch_bounds__(512) void k_ns_part_gram(const T* __restrict__ g, i
     tb[i] = t;
   }
   ns_f64x4 acc[PER] = {};
-  __syncthreads();
+  for (int64_t l0 = (int64_t)blockIdx.x * NS_LONG; l0 < l; l0 += (int64_t)splits * NS_LONG) {
+    X::load(x, g + batch * m * n + (tall ? l0 * n : l0), tall, n, (int)s, (int)(l - l0 < NS_LONG ? l - l0 : NS_LONG), vec);
+    __syncthreads();
 #pragma unroll 4
-  for (int k = 0; k < NS_LONG; k += 4)
+    for (int k = 0; k < NS_LONG; k += 4)
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      acc[i] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)x[X::at(tall, ta[i] * 16 + j, k + q)], (double)x[X::at(tall, tb[i] * 16 + j, k + q)], acc[i],
-                                                    0, 0, 0);
+      for (int i = 0; i < PER; ++i)
+        acc[i] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)x[X::at(tall, ta[i] * 16 + j, k + q)], (double)x[X::at(tall, tb[i] * 16 + j, k + q)],
+                                                      acc[i], 0, 0, 0);
+    __syncthreads();  // the part has been read
+  }
   double* o = part + (batch * splits + blockIdx.x) * s * s;
 #pragma unroll
   for (int i = 0; i < PER; ++i)
@@ -498,7 +504,13 @@ __global__ __launch_bounds__(256) void k_ns_square(const float* __restrict__ par
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------
-static int ns_parts(int64_t l) { return (int)((l + NS_LONG - 1) / NS_LONG); }
+// workgroups of a matrix's Gram matrix
+static int ns_gram_splits(int64_t batch, int64_t l) {
+  const int64_t parts = (l + NS_LONG - 1) / NS_LONG, room = batch > 0 && batch < NS_GRAM_BLOCKS ? NS_GRAM_BLOCKS / batch : 1;
+  if (parts <= room) return (int)parts;
+  const int64_t each = (parts + room - 1) / room;
+  return (int)((parts + each - 1) / each);
+}
 static int64_t ns_lower(int64_t s, int64_t t) {
   const int64_t k = (s + t - 1) / t;
   return k * (k + 1) / 2;
@@ -537,7 +549,7 @@ extern "C" size_t pp_newton_schulz_workspace_for(int32_t dtype, int64_t batch, i
   if (batch < 0 || m < 1 || n < 1 || m > 65536 * 64 || n > 65536 * 64) return 0;
   const int64_t s = m < n ? m : n, l = m < n ? n : m;
   if (s > NS_PANEL_MAX) return ns_large_ws(nullptr, dtype == PP_F32 ? 3 : 2, batch > 0 ? batch : 1, m, n, nullptr) + 256;
-  return pp_align((size_t)ns_parts(l) * batch * s * s * sizeof(double)) + 4 * pp_align((size_t)batch * s * s * sizeof(double)) +
+  return pp_align((size_t)ns_gram_splits(batch, l) * batch * s * s * sizeof(double)) + 4 * pp_align((size_t)batch * s * s * sizeof(double)) +
          (steps > NS_ROUND ? 2 * pp_align((size_t)batch * m * n * sizeof(float)) : 0) + 256;
 }
 extern "C" size_t pp_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n) {
@@ -678,7 +690,7 @@ static int ns_large(const T* g, int64_t batch, int64_t m, int64_t n, int steps, 
 template <typename T, typename O>
 static int ns_round(const T* x, int64_t batch, int64_t m, int64_t n, NsStepArgs p, int steps, O* out, double* part, double* const (&mats)[4], hipStream_t st) {
   const int64_t s = p.s;
-  const int splits = ns_parts(m < n ? n : m);
+  const int splits = ns_gram_splits(batch, m < n ? n : m);
   const unsigned nb = (unsigned)batch;
   const int vec = n % 4 == 0 && (uintptr_t)x % (4 * sizeof(T)) == 0;
   int rc = ns_part_gram<T>(x, m, n, s, splits, vec, part, nb, st);
@@ -698,7 +710,7 @@ static int ns_run(const void* g, int64_t batch, int64_t m, int64_t n, int steps,
                   PPArena& ws, hipStream_t st) {
   const int64_t s = m < n ? m : n;
   if (s > NS_PANEL_MAX) return ns_large<T, sizeof(T) == 2 ? 2 : 3>((const T*)g, batch, m, n, steps, ca, cb, cc, eps, (T*)out, ws, st);
-  double* part = ws.take<double>((size_t)ns_parts(m < n ? n : m) * batch * s * s);
+  double* part = ws.take<double>((size_t)ns_gram_splits(batch, m < n ? n : m) * batch * s * s);
   double* mats[4];
   for (double*& p : mats) p = ws.take<double>((size_t)batch * s * s);
   PP_REQUIRE(part && mats[3], "pp_newton_schulz: workspace layout");

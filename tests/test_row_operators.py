@@ -82,3 +82,20 @@ def test_newton_schulz_entry_refuses():
     assert lib.pp_newton_schulz_workspace(1, 0, 4) == 0
     with pytest.raises(_lib.PanopticHipError):
         ops.newton_schulz(torch.zeros(4, 4))
+
+
+def test_newton_schulz_workspace_stays_near_the_input():
+    """short sides up to 128: partial Gram matrices of at most 1024 workgroups (one a matrix in larger batches), five more matrices a batch
+    element; more than eight steps: two fp32 copies beside them.  Above 128: two X and two S-sized matrices of two (16 bits) or three planes"""
+    lib = _lib.load()
+    for batch, m, n in ((6, 4_000_000, 96), (1, 128, 4_194_304), (8, 1728, 64), (3, 5184, 96), (3000, 100, 100), (1, 7, 1)):
+        s, l = min(m, n), max(m, n)
+        gram = min(batch * -(-l // 64), max(1024, batch)) * s * s * 8
+        for dtype in (0, 1, 2):
+            short = lib.pp_newton_schulz_workspace_for(dtype, batch, m, n, 5)
+            assert 4 * batch * s * s * 8 <= short <= gram + 4 * batch * s * s * 8 + 4096
+            assert short + 8 * batch * m * n <= lib.pp_newton_schulz_workspace_for(dtype, batch, m, n, 9) <= lib.pp_newton_schulz_workspace(batch, m, n)
+    assert lib.pp_newton_schulz_workspace_for(1, 6, 4_000_000, 96, 5) < 100 << 20
+    low, full = (lib.pp_newton_schulz_workspace_for(dtype, 2, 4096, 1024, 5) for dtype in (1, 0))
+    assert low < full == lib.pp_newton_schulz_workspace(2, 4096, 1024) and low >= 2 * 2 * 2 * (4096 * 1024 + 1024 * 1024) * 2
+    assert lib.pp_newton_schulz_workspace_for(0, -1, 4, 4, 5) == 0

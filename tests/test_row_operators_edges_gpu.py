@@ -377,3 +377,15 @@ def test_newton_schulz_of_many_steps_keeps_missing_directions_small(dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, ops.newton_schulz(static, 21)), k
+
+
+@pytest.mark.parametrize("dtype,batch,m,n", [(torch.float32, 1, 70_001, 40), (torch.bfloat16, 5, 33, 15_000), (torch.float16, 1100, 200, 24),
+                                            (torch.float32, 2, 65_600, 128)])
+def test_newton_schulz_of_more_parts_than_workgroups(dtype, batch, m, n):
+    """a workgroup takes several parts of 64 of the long side (whole numbers of them, and a short last one)"""
+    gen = torch.Generator().manual_seed(n)
+    g = torch.randn((batch, m, n), generator=gen).to(dtype)
+    out = ops.newton_schulz(g.cuda()).double().cpu()
+    for k in {0, batch // 2, batch - 1}:
+        want, bound = rounds(g[k], 5, ops.NEWTON_SCHULZ_COEFFICIENTS)
+        assert float((out[k] - want).norm()) <= bound + (u + HALF_STEP[dtype]) * float(want.norm()) + TINY[dtype] * want.numel() ** 0.5, k
