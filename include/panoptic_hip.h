@@ -424,8 +424,10 @@ int pp_linear_act_bwd(const void* x, const void* dy, int32_t dtype, int64_t n, i
 /* ------------------------------------------------------------------------------------------------
  * Orthogonalisation of weight updates by Newton-Schulz products   (training.Muon)
  * g, out [batch,m,n] of element type `dtype`.  X = g / (|g| + eps) per matrix (Frobenius norm), then `steps` times
- * X <- a X + (b A + c A^2) X with A = X X^T on the shorter side (at most 8192).  Computed on the Gram matrix of the shorter side in
- * float64; results repeat bit for bit.
+ * X <- a X + (b A + c A^2) X with A = X X^T on the shorter side (at most 8192).  Shorter sides up to 128: on the Gram matrix of the shorter
+ * side in float64, formed anew from X (float32) every fifth step where there are more than eight.  Above: the iteration as it is written,
+ * X, A and the polynomial as sums of bfloat16 planes -- two for 16-bit types (16 bits, 2^-18 of a value), three for float32 (24 bits,
+ * 2^-26), rounded to them in every step -- with fp32 accumulation.  Results repeat bit for bit.
  * ---------------------------------------------------------------------------------------------- */
 size_t pp_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n);  /* for any type and number of steps */
 size_t pp_newton_schulz_workspace_for(int32_t dtype, int64_t batch, int64_t m, int64_t n, int32_t steps);

@@ -1412,7 +1412,9 @@ NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7):
     """Orthogonalises a matrix [m, n] or a batch of them [batch, m, n] (float32, bfloat16, float16): X = g / (|g| + eps), then `steps`
     times X <- a X + (b A + c A^2) X with A = X X^T (csrc/pp_newtonschulz.hip).  With the default coefficients five steps bring every
-    singular value above 1e-3 of the norm to 0.7 .. 1.2.  Same shape and type as g; the shorter side is at most 8192."""
+    singular value above 1e-3 of the norm to 0.7 .. 1.2.  Same shape and type as g; the shorter side is at most 8192.  Up to a shorter side
+    of 128 the steps run in float64; above it in two (16-bit types, 16 bits of each value) or three (float32, 24 bits) bfloat16 planes
+    with float32 sums."""
     lib = _lib.load()
     code = _row_dtype(g, "g")
     if g.dim() not in (2, 3) or 0 in g.shape[-2:]:

@@ -389,3 +389,26 @@ def test_newton_schulz_of_more_parts_than_workgroups(dtype, batch, m, n):
     for k in {0, batch // 2, batch - 1}:
         want, bound = rounds(g[k], 5, ops.NEWTON_SCHULZ_COEFFICIENTS)
         assert float((out[k] - want).norm()) <= bound + (u + HALF_STEP[dtype]) * float(want.norm()) + TINY[dtype] * want.numel() ** 0.5, k
+
+
+@pytest.mark.parametrize("batch,m,n", [(4, 160, 4_194_304), (4, 4_194_304, 160)])
+def test_newton_schulz_above_a_short_side_of_128_past_32_bits(batch, m, n):
+    """more than 2^31 elements on the plane form: the same matrix at the start and at the end of a batch"""
+    s, l = min(m, n), max(m, n)
+    one = torch.zeros((l, s), dtype=torch.bfloat16, device="cuda")
+    rows = torch.arange(l // s * s, device="cuda")
+    one[rows, rows % s] = 0.5
+    g = (one if m > n else one.t()).repeat(batch, 1, 1)
+    assert g.numel() > 2 ** 31  # (the last matrix passes it)
+    out = ops.newton_schulz(g)
+    assert all(torch.equal(out[0], out[i]) for i in range(1, batch))
+    # orthogonal columns of one length: every singular value is t = 1 / sqrt(s) of the norm, and so is every result
+    t = s ** -0.5
+    for _ in range(5):
+        a, b, c = ops.NEWTON_SCHULZ_COEFFICIENTS
+        t = a * t + b * t ** 3 + c * t ** 5
+    value = t / (l // s) ** 0.5
+    have = out[batch - 1] if m > n else out[batch - 1].t()
+    # bfloat16's half step, and two planes: 2^-16 of three operands a step, 4 times as much in the later ones: below 2^-8 in all
+    assert float((have[rows, rows % s].double() / value - 1).abs().max()) <= 2 ** -7
+    assert int(have.count_nonzero()) == rows.numel()
