@@ -1406,6 +1406,7 @@ def linear_act_bwd(x, dy, weight, bias=None, act=0, slope=0.0, want_input=True, 
 
 
 NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+NEWTON_SCHULZ_SHORT_SIDE = 8192  # at most
 
 
 @_on_device_of
@@ -1421,8 +1422,8 @@ def newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps=1e-7)
         raise ValueError("newton_schulz: g must be [m, n] or [batch, m, n], got %s" % (tuple(g.shape),))
     m, n = g.shape[-2:]
     batch = g.shape[0] if g.dim() == 3 else 1
-    if min(m, n) > 8192:
-        raise ValueError("newton_schulz: the shorter side is at most 8192, got %d" % min(m, n))
+    if min(m, n) > NEWTON_SCHULZ_SHORT_SIDE:
+        raise ValueError("newton_schulz: the shorter side is at most %d, got %d" % (NEWTON_SCHULZ_SHORT_SIDE, min(m, n)))
     if steps < 1:
         raise ValueError("newton_schulz: at least one step, got %d" % steps)
     a, b, c = coefficients

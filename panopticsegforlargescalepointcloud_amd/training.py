@@ -191,7 +191,7 @@ def matrix_parameters(model):
 
 def _matrix_shape(p):
     """a weight as a matrix: kernels [K, Cin, Cout] as [K Cin, Cout], weights of linear layers as they are"""
-    return (p.numel() // p.shape[-1] if p.dim() > 2 else p.shape[0]), p.shape[-1]
+    return p.shape[:-1].numel(), p.shape[-1]
 
 
 class Muon(torch.optim.Optimizer):
@@ -209,8 +209,10 @@ class Muon(torch.optim.Optimizer):
     def add_param_group(self, group):
         super().add_param_group(group)
         for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
-                raise ValueError("Muon: parameters need at least two dimensions, got shape %s" % (tuple(p.shape),))
+            if p.dim() < 2 or p.numel() == 0 or min(_matrix_shape(p)) > ops.NEWTON_SCHULZ_SHORT_SIDE:
+                del self.param_groups[-1]
+                raise ValueError("Muon: parameters need at least two dimensions, some values and a shorter side of at most %d, got shape %s"
+                                 % (ops.NEWTON_SCHULZ_SHORT_SIDE, tuple(p.shape)))
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)  # (gives the momentum the parameters' type: put back what was saved)
@@ -225,12 +227,15 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        moving = [p for group in self.param_groups for p in group["params"] if p.grad is not None]  # refused before anything is changed
+        if any(p.grad.is_sparse for p in moving):
+            raise RuntimeError("Muon does not take sparse gradients")
+        if not all(p.is_cuda for p in moving):
+            raise RuntimeError("Muon: parameters must be on a HIP device (there is no CPU fallback)")
         for group in self.param_groups:
             by_shape = {}
             for p in group["params"]:
                 if p.grad is not None:
-                    if p.grad.is_sparse:
-                        raise RuntimeError("Muon does not take sparse gradients")
                     by_shape.setdefault((p.device, p.dtype, _matrix_shape(p)), []).append(p)
             for (_, _, (m, n)), ps in by_shape.items():
                 buffers = []

@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 import torch
 
-from panopticsegforlargescalepointcloud_amd import _lib, modules, ops
+from panopticsegforlargescalepointcloud_amd import _lib, modules, ops, training
 
 INVALID, WORKSPACE = 1, 4
 P = C.c_void_p(4096)  # never read: every call below is refused before a launch
@@ -99,3 +99,28 @@ def test_newton_schulz_workspace_stays_near_the_input():
     low, full = (lib.pp_newton_schulz_workspace_for(dtype, 2, 4096, 1024, 5) for dtype in (1, 0))
     assert low < full == lib.pp_newton_schulz_workspace(2, 4096, 1024) and low >= 2 * 2 * 2 * (4096 * 1024 + 1024 * 1024) * 2
     assert lib.pp_newton_schulz_workspace_for(0, -1, 4, 4, 5) == 0
+
+
+def test_muon_refuses_before_it_changes_anything():
+    def param(*shape):
+        return torch.nn.Parameter(torch.ones(shape))
+    good = param(4, 3)
+    for bad in (param(4), param(0, 3), param(3, 0), param(2, 0, 3), param(9000, 1).expand(9000, 9000).detach().requires_grad_()):
+        with pytest.raises(ValueError, match="Muon"):
+            training.Muon([good, bad])
+        opt = training.Muon([good])
+        with pytest.raises(ValueError, match="Muon"):
+            opt.add_param_group({"params": [bad]})
+        assert len(opt.param_groups) == 1
+    sparse = param(4, 3)
+    sparse.grad = torch.ones(4, 3).to_sparse()
+    good.grad = torch.ones(4, 3)
+    opt = training.Muon([good, sparse], weight_decay=0.1)
+    with pytest.raises(RuntimeError, match="sparse"):
+        opt.step()
+    opt = training.Muon([good], weight_decay=0.1)
+    with pytest.raises(RuntimeError, match="device"):
+        opt.step()
+    assert not opt.state and bool((good == 1).all())
+    matrices, others = training.matrix_parameters(torch.nn.ParameterList([good, param(3, 0), param(0, 3), param(2, 0, 3), param(5)]))
+    assert len(matrices) == 1 and len(others) == 4
