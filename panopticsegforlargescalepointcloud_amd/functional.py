@@ -72,12 +72,13 @@ class _LinearActFn(torch.autograd.Function):
 
 def linear_act(x, weight, bias=None, activation="none", slope=0.2, residual=None):
     """y = act(x W^T + bias) + residual as one launch, differentiable in all four operands.  x [..., cin], weight [cout, cin] (the
-    layout of torch.nn.Linear), bias [cout] or None, residual [..., cout] or None, all of one type (float32, bfloat16, float16); under
-    torch.autocast they are brought to its type, as torch.nn.functional.linear's are.
+    layout of torch.nn.Linear), bias [cout] or None, residual [..., cout] or None, all of one type (float32, bfloat16, float16), which is
+    the result's.  Under torch.autocast operands of different types are brought to its type; operands of one type stay as they are
+    (fp32 features go on to sparse convolutions, which take nothing else).
     activation: none, relu, leaky_relu (with `slope`), silu or gelu (exact); it acts before the residual is added, as in ResBlock."""
     act = ops.activation_id(activation)
     _refuse_tangents("linear_act", x, weight, bias, residual)
-    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+    if torch.is_autocast_enabled("cuda") and any(t is not None and t.dtype != x.dtype for t in (weight, bias, residual)):
         dtype = torch.get_autocast_dtype("cuda")
         x, weight, bias, residual = (t if t is None or t.dtype == torch.float64 else t.to(dtype) for t in (x, weight, bias, residual))
     if x.dim() != 2:

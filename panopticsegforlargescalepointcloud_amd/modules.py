@@ -84,7 +84,7 @@ class _SkinnyLinearFn(torch.autograd.Function):
 class LinearAct(nn.Linear):
     """torch.nn.Linear (same parameters, same state_dict keys) with the activation and a residual in its epilogue: one launch forward,
     the pre-activation recomputed backward (functional.linear_act).  Takes [..., in_features] and sparse tensors, whose residual is a
-    sparse tensor on the same coordinate map; follows torch.autocast as its parent does."""
+    sparse tensor on the same coordinate map; operands of different types under torch.autocast, as functional.linear_act does."""
 
     def __init__(self, in_features, out_features, bias=True, activation="none", slope=0.2, **kwargs):
         super().__init__(in_features, out_features, bias=bias, **kwargs)

