@@ -413,3 +413,39 @@ def test_newton_schulz_above_a_short_side_of_128_past_32_bits(batch, m, n):
     # bfloat16's half step, and two planes: 2^-16 of three operands a step, 4 times as much in the later ones: below 2^-8 in all
     assert float((have[rows, rows % s].double() / value - 1).abs().max()) <= 2 ** -7
     assert int(have.count_nonzero()) == rows.numel()
+
+
+@pytest.mark.parametrize("c,groups", [(8, 8), (8, 2), (7, 7), (96, 32), (300, 100)])
+@pytest.mark.parametrize("lengths,shuffled", [([70_000], False), ([3, 40, 0, 30_000, 1], True), ([400_000, 200_000], False)])
+def test_statistics_far_from_zero(c, groups, lengths, shuffled):
+    """channels of one value, and of a small spread, around numbers up to 1e7: the mean is rounded once, 1 / std is off by what fp64 sums of
+    distances to a value of the group leave, far below u, and its own rounding; without a spread it is 1 / sqrt(eps)"""
+    n = sum(lengths)
+    gen = torch.Generator(device="cuda").manual_seed(n + c)
+    at = torch.tensor([0.3, 1000.1, 30000.7, 100000.3, 1000001.0, 1e7 + 1], device="cuda").repeat_interleave(c // groups).repeat(c)[:c]
+    off = torch.tensor([0] + lengths, device="cuda").cumsum(0)
+    order = torch.randperm(n, generator=gen, device="cuda") if shuffled else None
+    w = 1 + torch.rand(c, generator=gen, device="cuda")
+    dy = torch.randn((n, c), generator=gen, device="cuda")
+    for spread in (0.0, 3.0):
+        x = at + spread * torch.randn((n, c), generator=gen, device="cuda") if spread else at.expand(n, c).contiguous()
+        _, mean, rstd = ops.group_norm_fwd(x, off, groups, w, None, 1e-5, 0, 0.0, order)
+        dx = ops.group_norm_bwd(x, dy, off, groups, w, None, mean, rstd, 0, 0.0, order)[0]
+        for e, (lo, hi) in enumerate(zip(off[:-1].tolist(), off[1:].tolist())):
+            if hi == lo:
+                assert int(rstd[e].count_nonzero()) == 0
+                continue
+            rows = torch.arange(lo, hi, device="cuda") if order is None else order[lo:hi]
+            v = x[rows].double().view(hi - lo, groups, -1)
+            want = v.mean((0, 2))
+            var = ((v - want[:, None]) ** 2).mean((0, 2))
+            r = 1 / torch.sqrt(var + 1e-5)
+            assert bool(((mean[e].double() - want).abs() <= 2 * u * want.abs()).all())
+            # a group of one value has mean v itself (n v / n rounds in this reference only)
+            r = torch.where(torch.tensor(spread == 0.0, device="cuda"), 1e-5 ** -0.5, r)
+            assert bool(((rstd[e].double() - r).abs() <= 2 * u * r).all()), (rstd[e].double() / r - 1).abs().max()
+            if spread == 0.0:  # xh is 0: dx = rstd (h - mean(h))
+                h = (dy[rows].double() * w).view(hi - lo, groups, -1)
+                m = h.mean((0, 2), keepdim=True)
+                d = dx[rows].double().view(hi - lo, groups, -1)
+                assert bool(((d - r[:, None] * (h - m)).abs() <= 8 * u * r[:, None] * (h.abs() + m.abs())).all())
