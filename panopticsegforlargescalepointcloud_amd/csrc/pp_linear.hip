@@ -42,7 +42,8 @@ template <typename T> struct LinChunk { gm_u32x4 p[LinType<T>::PLANES]; };
 // hi, mid and lo, each the nearest bf16 to what is left: hi + mid + lo is v exactly (24 bits in 8 and two signs), |mid| <= 2^-8 |v| and
 // |lo| <= 2^-16 |v| of either sign, so that the products left out, mid lo + lo mid + lo lo, are at most 2^-23 of v w and cancel in long
 // sums (cut off instead of rounded the terms all have v's sign: up to 2^-21, always towards 0).  The same number of instructions: the
-// conversion makes two values at once.  hi overflows above the largest bf16: see LinEpilogue::exact
+// conversion makes two values at once.  hi overflows above the largest bf16: see LinEpilogue::exact.  A
+// bf16 ends at 2^-133: what of a term lies below is lost, so operands below 2^-109 are kept to 2^-134, not to 24 bits
 typedef float lin_f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 lin_bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void lin_pack(const float (&v)[8], LinChunk<float>& c) {
