@@ -6,7 +6,7 @@
 // spread over all banks; the next step's loads are in flight while this step's fragments are multiplied.
 // fp32 operands are split exactly into three bf16 terms (8 + 8 + 8 bits) when they are staged, and a product is the six largest of its
 // nine bf16 products (the others are at most 2^-23 of it), accumulated in fp32: an fp32-accurate evaluation at 2.7 times the rate of the fp32 matrix instructions.
-// Infinities and NaN do what they do in a plain sum (LinEpilogue::exact).  bf16 and fp16 operands are multiplied as they are, accumulated in fp32.
+// Infinities and NaN do what they do in a plain sum (lin_exact).  bf16 and fp16 operands are multiplied as they are, accumulated in fp32.
 // Nothing is kept for the backward pass but x: z is recomputed from it (the layers are bound by memory, a stored z would cost a write
 // and a read of its own, and its rounding would enter the gradients).  dz is rounded to the element type once, as the matrix
 // instructions take it.  The weight gradient's rows are cut into parts, whose sums are added in a fixed order: results repeat.
@@ -42,8 +42,8 @@ template <typename T> struct LinChunk { gm_u32x4 p[LinType<T>::PLANES]; };
 // hi, mid and lo, each the nearest bf16 to what is left: hi + mid + lo is v exactly (24 bits in 8 and two signs), |mid| <= 2^-8 |v| and
 // |lo| <= 2^-16 |v| of either sign, so that the products left out, mid lo + lo mid + lo lo, are at most 2^-23 of v w and cancel in long
 // sums (cut off instead of rounded the terms all have v's sign: up to 2^-21, always towards 0).  The same number of instructions: the
-// conversion makes two values at once.  hi overflows above the largest bf16: see LinEpilogue::exact.  A
-// bf16 ends at 2^-133: what of a term lies below is lost, so operands below 2^-109 are kept to 2^-134, not to 24 bits
+// conversion makes two values at once.  hi overflows above the largest bf16: see lin_exact.  A bf16 ends at 2^-133: what of a term lies
+// below is lost, so operands below 2^-109 are kept to 2^-134, not to 24 bits
 typedef float lin_f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 lin_bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void lin_pack(const float (&v)[8], LinChunk<float>& c) {
@@ -227,38 +227,8 @@ struct LinEpilogue {
       }
     }
   }
-  // fp32: where a term is infinite, NaN or so large that its first plane overflows, its planes make the products NaN.  Such results are
-  // made again from the operands as they are, one multiplication and addition at a time (in fp64: a sum that fp32 holds is not lost
-  // half way).  Nothing else is: the check is one comparison per value of the epilogue
-  __device__ __forceinline__ void exact(int64_t r, float (&v)[8]) const {
-    float sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum += v[e];
-    if (sum == sum) return;
-    constexpr bool AS = MODE == LIN_PART, BS = MODE == LIN_PART || MODE == LIN_STORE;
-    const float *A = (const float*)a.a, *B = (const float*)a.b;
-    const int64_t k0 = MODE == LIN_PART ? split * a.k_per_split : 0, k1 = MODE == LIN_PART && k0 + a.k_per_split < a.k ? k0 + a.k_per_split : a.k;
-    double s[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s[e] = 0.0;
-#pragma unroll 1
-    for (int64_t k = k0; k < k1; ++k) {
-      const double x = (double)A[AS ? k * a.lda + r : r * a.lda + k];
-      bool all_nan = true;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < valid) {
-          s[e] = fma(x, (double)B[BS ? k * a.ldb + c + e : (c + e) * a.ldb + k], s[e]);
-          all_nan &= s[e] != s[e];
-        }
-      if (all_nan) break;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < valid ? (v[e] == v[e] ? v[e] : (float)s[e]) : 0.f;
-  }
   __device__ __forceinline__ void put(int64_t r, Row& w, float (&v)[8]) {
     if (r >= a.m) return;
-    if constexpr (sizeof(T) == 4) exact(r, v);
     if constexpr (FUSED) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += b[e];
@@ -315,6 +285,36 @@ struct LinEpilogue {
   }
 };
 
+// fp32: where a term is infinite, NaN or so large that its first plane overflows, its planes make the products NaN.  Such results of a wave are
+// made again from the operands as they are, one multiplication and addition at a time (in fp64: a sum that fp32 holds is not lost half
+// way).  In front of the epilogue: inside its loop it made 325 k x 96 -> 96 training 2 % longer
+template <bool AS, bool BS, int FM, int FN>
+__device__ __forceinline__ void lin_exact(const LinArgs& a, gm_f32x4 (&acc)[FM][FN], int64_t row0, int64_t col0, int64_t k0, int64_t k1) {
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sum += (acc[i][j][0] + acc[i][j][1]) + (acc[i][j][2] + acc[i][j][3]);
+  if (!__any(sum != sum)) return;
+  const int lane = threadIdx.x & 63;
+  const float *A = (const float*)a.a, *B = (const float*)a.b;
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int64_t r = row0 + 16 * i + (lane & 15), c = col0 + 16 * j + 4 * (lane >> 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (acc[i][j][e] == acc[i][j][e] || r >= a.m || c + e >= a.n) continue;
+        double s = 0.0;
+#pragma unroll 1
+        for (int64_t k = k0; k < k1 && s == s; ++k)
+          s = fma((double)A[AS ? k * a.lda + r : r * a.lda + k], (double)B[BS ? k * a.ldb + c + e : (c + e) * a.ldb + k], s);
+        acc[i][j][e] = (float)s;
+      }
+    }
+}
+
 // BM x BN tile, four waves of WM x WN each.  AS / BS: the contraction runs down the columns of A / B
 template <typename T, bool AS, bool BS, int MODE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
@@ -330,6 +330,7 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
     k = (int64_t)blockIdx.z * a.k_per_split;
     k1 = k + a.k_per_split < a.k ? k + a.k_per_split : a.k;
   }
+  const int64_t k0 = k;
   const T *pa = (const T*)a.a, *pb = (const T*)a.b;
   gm_f32x4 acc[FM][FN];
 #pragma unroll
@@ -366,6 +367,7 @@ __global__ __launch_bounds__(256, 2) void k_linear_tile(LinArgs a) {
       }
     }
   }
+  if constexpr (sizeof(T) == 4) lin_exact<AS, BS, FM, FN>(a, acc, m0 + wm, n0 + wn, k0, k1);
   LinEpilogue<T, MODE> epi;
   epi.a = a;
   __syncthreads();
