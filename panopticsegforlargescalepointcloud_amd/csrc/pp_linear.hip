@@ -724,10 +724,12 @@ static int lin_tile(const LinArgs& a, int splits, hipStream_t s) {
 
 // parts of the weight gradient's contraction: about two workgroups per compute unit, at least 256 rows (wide kernel: 512) each, and at most
 // as many as a chain of fp32 additions stands: 2048 in fp32 (64 steps of six: terms of one sign lose 384 2^-24 of their sum at most; they
-// lost 9e-5 of 10 M rows in 512 parts), 65536 in 16 bits (2048 steps: 2048 2^-24, a quarter of fp16's half step)
+// lost 9e-5 of 10 M rows in 512 parts), 65536 in 16 bits (2048 steps: 2048 2^-24, a quarter of fp16's half step); longer ones where a matrix
+// is so wide that its parts would take more room than the rows themselves
 static int lin_splits(int64_t n, int cin, int cout, bool wide, size_t bytes) {
   const int64_t tiles = (int64_t)((cout + 127) / 128) * ((cin + (cin > 64 ? 127 : 63)) / (cin > 64 ? 128 : 64));
-  const int64_t rows = wide ? 512 : 256, most = bytes == 4 ? 2048 : 65536;
+  const int64_t rows = wide ? 512 : 256, chain = bytes == 4 ? 2048 : 65536, room = (int64_t)cin * cout / ((int64_t)cin + cout);
+  const int64_t most = chain > room ? chain : room;
   int64_t s = 512 / tiles;
   if (s > (n + rows - 1) / rows) s = (n + rows - 1) / rows;
   if (s < (n + most - 1) / most) s = (n + most - 1) / most;

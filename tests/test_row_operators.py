@@ -124,3 +124,15 @@ def test_muon_refuses_before_it_changes_anything():
     assert not opt.state and bool((good == 1).all())
     matrices, others = training.matrix_parameters(torch.nn.ParameterList([good, param(3, 0), param(0, 3), param(2, 0, 3), param(5)]))
     assert len(matrices) == 1 and len(others) == 4
+
+
+@pytest.mark.parametrize("n,cin,cout", [(1_000_000, 8192, 8192), (1_000_000, 16384, 4096), (10_000_000, 64, 64), (300_000, 4096, 4096), ((1 << 31) - 1, 8, 8)])
+def test_linear_act_workspace_stays_near_the_input(n, cin, cout):
+    """parts of the weight gradient: no more than the rows of x and dz, or two workgroups' worth of every compute unit; dz; parts of the bias"""
+    lib = _lib.load()
+    tiles = -(-cout // 128) * -(-cin // (128 if cin > 64 else 64))
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        parts = max(4 * n * (cin + cout), -(-512 // tiles) * cin * cout * 4) + 33 * cin * cout * 4
+        dz = n * -(-cout // 8) * 8 * size
+        bias = (max(n // 128 + 1, 512, n // 131072 + 1) + 32) * cout * 4
+        assert lib.pp_linear_act_bwd_workspace(dtype, n, cin, cout, 3) <= parts + dz + bias + 4096
