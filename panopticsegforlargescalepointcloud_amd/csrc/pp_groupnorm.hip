@@ -176,11 +176,35 @@ struct GnRaw {
   __device__ __forceinline__ float operator[](int u) const { return (float)v[u]; }
 };
 
+// the pivots of a thread's channels in element s: the first channel of the group in the element's first row r, at position o (0 where there is none,
+// r < 0).  The chunk that begins the element at o leaves them for the second pass
+template <bool ORDER>
+__device__ __forceinline__ int64_t gn_first_row(const GnArgs& a, int64_t s, int64_t* o) {
+  *o = gn_clamp(a.off[s], a.n);
+  int64_t r = *o < a.n ? *o : -1;
+  if (ORDER && r >= 0) r = a.order[*o];
+  return r < a.n ? r : -1;
+}
+template <typename T, int VEC, int NC, typename Lane>
+__device__ __forceinline__ void gn_pivots(const GnArgs& a, const Lane& ln, int64_t s, int64_t r, bool begins, float (&pv)[NC][VEC]) {
+  const int cg = a.c / a.g;
+#pragma unroll
+  for (int k = 0; k < NC; ++k)
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) pv[k][u] = r >= 0 ? (float)((const T*)a.x)[r * a.c + ln.group[k][u] * cg] : 0.f;
+  if (!begins || ln.rin != 0) return;
+#pragma unroll
+  for (int k = 0; k < NC; ++k)
+#pragma unroll
+    for (int u = 0; u < VEC; ++u)
+      if (ln.has(k, a.c) && ln.channel(k) + u == ln.group[k][u] * cg) a.pivot[s * a.g + ln.group[k][u]] = pv[k][u];
+}
+
 // A thread's sums over the rows [p, e) of an element -> LDS red[2][rps][c], times the channel's weight backward.
-// FORWARD: d, d^2 with the pivot in mu; else dz, dz xh, which are added to the thread's totals as they are
+// FORWARD: d, d^2, the pivots read behind the first rows; else dz, dz xh, which are added to the thread's totals as they are
 template <typename T, int VEC, int NC, bool FORWARD, bool ORDER, typename Lane>
 __device__ __forceinline__ void gn_rows_sum(const GnArgs& a, const GnChunk<T, ORDER>& chunk, const Lane& ln, const GnAffine<VEC, NC>& af, int p, int e,
-                                            const float (&mu)[NC][VEC], const float (&rs)[NC][VEC], double* __restrict__ red,
+                                            int64_t s, float (&mu)[NC][VEC], const float (&rs)[NC][VEC], double* __restrict__ red,
                                             double (&t0)[FORWARD ? 1 : NC][VEC], double (&t1)[FORWARD ? 1 : NC][VEC]) {
   if (!ln.on) return;
   double s0[NC][VEC], s1[NC][VEC];
@@ -189,6 +213,9 @@ __device__ __forceinline__ void gn_rows_sum(const GnArgs& a, const GnChunk<T, OR
 #pragma unroll
     for (int u = 0; u < VEC; ++u) s0[k][u] = s1[k][u] = 0.0;
   constexpr int U = NC > 1 ? 1 : FORWARD || sizeof(T) == 2 ? 4 : 2;  // rows in flight
+  int64_t o = 0, first = 0;
+  if (FORWARD) first = gn_first_row<ORDER>(a, s, &o);
+  bool pivots = false;
   GnRows<ORDER, U> rows(a, chunk, p + ln.rin, e, ln.rps);
   while (rows.more()) {
     GnRaw<T, VEC> xr[U][NC], dr[U][NC];
@@ -202,6 +229,10 @@ __device__ __forceinline__ void gn_rows_sum(const GnArgs& a, const GnChunk<T, OR
           xr[i][k].load(chunk.x + (at[i] + ln.channel(k)));
           if (!FORWARD) dr[i][k].load(chunk.dy + (at[i] + ln.channel(k)));
         }
+    if (FORWARD && !pivots) {
+      gn_pivots<T, VEC, NC>(a, ln, s, first, chunk.start + p == o, mu);
+      pivots = true;
+    }
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
@@ -354,29 +385,6 @@ __device__ __forceinline__ void gn_per_channel(const GnArgs& a, const Lane& ln, 
     for (int u = 0; u < VEC; ++u) v[k][u] = row[ln.group[k][u] * stride];
 }
 
-// the pivots of a thread's channels in element s: the first channel of the group in the element's first row (0 where the order holds no row
-// there).  The chunk with that row (first_rows) leaves them for the second pass
-template <typename T, int VEC, int NC, bool ORDER, typename Lane>
-__device__ __forceinline__ void gn_pivots(const GnArgs& a, const Lane& ln, int64_t s, int64_t chunk_position, float (&pv)[NC][VEC]) {
-  const int64_t o = gn_clamp(a.off[s], a.n);
-  int64_t r = o < a.n ? o : -1;
-  if (ORDER && r >= 0) {
-    r = a.order[o];
-    if (r >= a.n) r = -1;
-  }
-  const int cg = a.c / a.g;
-#pragma unroll
-  for (int k = 0; k < NC; ++k)
-#pragma unroll
-    for (int u = 0; u < VEC; ++u) pv[k][u] = r >= 0 ? (float)((const T*)a.x)[r * a.c + ln.group[k][u] * cg] : 0.f;
-  if (chunk_position != o || !ln.on || ln.rin != 0) return;
-#pragma unroll
-  for (int k = 0; k < NC; ++k)
-#pragma unroll
-    for (int u = 0; u < VEC; ++u)
-      if (ln.has(k, a.c) && ln.channel(k) + u == ln.group[k][u] * cg) a.pivot[s * a.g + ln.group[k][u]] = pv[k][u];
-}
-
 // ---- first pass: the sums of a chunk's elements ---------------------------------------------------------------------------------------
 template <typename T, int VEC, int NC, bool FORWARD, bool ORDER>
 __global__ __launch_bounds__(256, NC == 1 ? 4 : 1) void k_gn_chunk_sums(GnArgs a) {
@@ -390,13 +398,11 @@ __global__ __launch_bounds__(256, NC == 1 ? 4 : 1) void k_gn_chunk_sums(GnArgs a
     if (!chunk.element(a, p, &hi, &s, &e)) continue;
     const int64_t slot = (int64_t)blockIdx.x + s;
     float mu[NC][VEC] = {}, rs[NC][VEC] = {};
-    if (FORWARD) {
-      gn_pivots<T, VEC, NC, ORDER>(a, ln, s, chunk.start + p, mu);
-    } else {
+    if (!FORWARD) {
       gn_per_channel<VEC, NC>(a, ln, a.mean, 1, s, mu);
       gn_per_channel<VEC, NC>(a, ln, a.rstd, 1, s, rs);
     }
-    gn_rows_sum<T, VEC, NC, FORWARD, ORDER>(a, chunk, ln, af, p, e, mu, rs, red, t0, t1);
+    gn_rows_sum<T, VEC, NC, FORWARD, ORDER>(a, chunk, ln, af, p, e, s, mu, rs, red, t0, t1);
     __syncthreads();
     gn_group_sums(a, ln.rps, red, [&](int g, double v0, double v1) {
       a.slots[(slot * a.g + g) * 2] = v0;
@@ -621,7 +627,7 @@ extern "C" size_t pp_group_norm_workspace(int64_t n, int64_t b, int32_t c, int32
 
 // The second pass adds an element's slots itself where that is at most GN_INLINE bytes for an element of average length, and all of its
 // workgroups fit on the chip at once (a launch less); a longer one is better off with the registers that takes, so that more waves hide
-// its loads (2.5 M x 96 bf16, 64 elements, gelu: rows 417 us inline, 297 us even with spills at half as many registers)
+// its loads (2.5 M x 96 bf16, 64 elements, gelu: rows 400 us inline, 275 us at half as many registers)
 #define GN_INLINE (64 * 1024)
 template <typename T, int VEC, int NC, bool FORWARD, bool ORDER>
 static void gn_sums(const GnArgs& a, hipStream_t s) {
@@ -636,7 +642,7 @@ static int gn_launch(GnArgs& a, hipStream_t s) {
   a.blocks = a.out ? (int)((a.n + a.rows_per_block - 1) / a.rows_per_block) : 0;  // (backward without dx: no second pass)
   const bool in = a.b > 0 && a.blocks <= GN_MAX_CHUNKS && (a.chunks / a.b + 2) * a.g * (int64_t)(2 * sizeof(double)) <= GN_INLINE;
   if (a.chunks) {
-    // eight channels of 16 bits at a time where the loads bound, as in long forward sums (2.5 M x 96: 119 us, 160 us with four); elsewhere
+    // eight channels of 16 bits at a time where the loads bound, as in long forward sums (2.5 M x 96: 134 us, 166 us with four); elsewhere
     // the registers they take cost more waves than they are worth (see gn_order)
     constexpr int WIDE = FORWARD && sizeof(T) == 2 && VEC == 4 ? 8 : VEC;
     if (WIDE != VEC && !in && a.c % WIDE == 0 && (uintptr_t)a.x % 16 == 0)
@@ -666,7 +672,7 @@ static int gn_launch(GnArgs& a, hipStream_t s) {
 }
 
 // Vectors of four channels where every row starts on one; single elements else.  (Eight channels of 16 bits are the wider load, but the
-// registers they take leave half the waves: 1500 elements, 180 k x 64 bf16, backward sums 97 us with eight, 52 us with four.)
+// registers they take leave half the waves: 1500 elements, 180 k x 64 bf16, backward sums 140 us with eight, 38 us with four.)
 template <typename T, int VEC, int NC, bool FORWARD>
 static int gn_order(GnArgs& a, hipStream_t s) {
   return a.order ? gn_launch<T, VEC, NC, FORWARD, true>(a, s) : gn_launch<T, VEC, NC, FORWARD, false>(a, s);
