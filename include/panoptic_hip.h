@@ -43,7 +43,7 @@ enum {
 
 /* Element types and activations of the row operators (pp_group_norm_*, pp_linear_act_*, pp_newton_schulz). */
 enum { PP_F32 = 0, PP_BF16 = 1, PP_F16 = 2 };
-enum { PP_ACT_NONE = 0, PP_ACT_RELU = 1, PP_ACT_LEAKY = 2, PP_ACT_SILU = 3, PP_ACT_GELU = 4 /* exact, by erf */ };
+enum { PP_ACT_NONE = 0, PP_ACT_RELU = 1, PP_ACT_LEAKY = 2, PP_ACT_SILU = 3, PP_ACT_GELU = 4 /* z Phi(z), Phi to 1.5 2^-24 */ };
 
 /* Library identity / diagnostics.  pp_version: "panoptic_hip <n> gfx950". */
 const char* pp_version(void);
@@ -413,6 +413,8 @@ int pp_group_norm_bwd(const void* x, const void* dy, int32_t dtype, int64_t n, i
  * Up to 2^31 - 1 rows, 2^20 channels.  fwd: y = act(x weight^T + bias) + residual, fp32 accumulation, one rounding.
  * bwd: dz = dy act'(x weight^T + bias) (recomputed), dbias = column sums of it; then rounded to the element type: dx = dz weight,
  *      dweight = dz^T x; each of dx, dweight, dbias nullable.  The residual's gradient is dy itself.  Results repeat bit for bit.
+ * PP_F32: six of the nine products of three-term bfloat16 splits, at most 2^-23 of each product left out.  Infinities and NaN do what
+ * they do in a plain sum, in every type.
  * ---------------------------------------------------------------------------------------------- */
 int pp_linear_act_fwd(const void* x, int32_t dtype, int64_t n, int32_t cin, const void* weight, int32_t cout, const void* bias,
                       int32_t act, float slope, const void* residual, void* y, pp_stream_t stream);

@@ -627,7 +627,7 @@ extern "C" size_t pp_group_norm_workspace(int64_t n, int64_t b, int32_t c, int32
 
 // The second pass adds an element's slots itself where that is at most GN_INLINE bytes for an element of average length, and all of its
 // workgroups fit on the chip at once (a launch less); a longer one is better off with the registers that takes, so that more waves hide
-// its loads (2.5 M x 96 bf16, 64 elements, gelu: rows 400 us inline, 275 us at half as many registers)
+// its loads (2.5 M x 96 bf16, 64 elements, gelu: rows 407 us inline, 279 us at half as many registers)
 #define GN_INLINE (64 * 1024)
 template <typename T, int VEC, int NC, bool FORWARD, bool ORDER>
 static void gn_sums(const GnArgs& a, hipStream_t s) {
@@ -642,7 +642,7 @@ static int gn_launch(GnArgs& a, hipStream_t s) {
   a.blocks = a.out ? (int)((a.n + a.rows_per_block - 1) / a.rows_per_block) : 0;  // (backward without dx: no second pass)
   const bool in = a.b > 0 && a.blocks <= GN_MAX_CHUNKS && (a.chunks / a.b + 2) * a.g * (int64_t)(2 * sizeof(double)) <= GN_INLINE;
   if (a.chunks) {
-    // eight channels of 16 bits at a time where the loads bound, as in long forward sums (2.5 M x 96: 134 us, 166 us with four); elsewhere
+    // eight channels of 16 bits at a time where the loads bound, as in long forward sums (2.5 M x 96: 126 us, 170 us with four); elsewhere
     // the registers they take cost more waves than they are worth (see gn_order)
     constexpr int WIDE = FORWARD && sizeof(T) == 2 && VEC == 4 ? 8 : VEC;
     if (WIDE != VEC && !in && a.c % WIDE == 0 && (uintptr_t)a.x % 16 == 0)

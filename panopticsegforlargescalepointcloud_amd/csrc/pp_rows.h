@@ -1,5 +1,6 @@
 // Element types and activations of the row operators (pp_groupnorm.hip, pp_linear.hip): features are [rows, channels] in fp32, bf16
-// or fp16, arithmetic is fp32 (sums that run over many rows: fp64), and a result is rounded once, when it is stored.
+// or fp16, arithmetic is fp32 (sums that run over many rows: fp64, or fp32 chains of a bounded length that are added in fp64), and a result is
+// rounded once, when it is stored (the linear layer's dz once more, as the operand of its products: see there).
 #pragma once
 #include "pp_common.h"
 
