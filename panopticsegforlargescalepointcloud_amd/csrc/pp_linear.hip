@@ -290,6 +290,7 @@ struct LinEpilogue {
 // fp32: where a term is infinite, NaN or so large that its first plane overflows, its planes make the products NaN.  Such results of a wave are
 // made again from the operands as they are, one multiplication and addition at a time (in fp64: a sum that fp32 holds is not lost half
 // way).  In front of the epilogue: inside its loop it made 325 k x 96 -> 96 training 2 % longer
+// (8192 x 1024 -> 1024 forward 0.12 ms, 0.15 with a NaN in every row, where a sum ends at it, 8.3 with an infinity in every row)
 template <bool AS, bool BS, int FM, int FN>
 __device__ __forceinline__ void lin_exact(const LinArgs& a, gm_f32x4 (&acc)[FM][FN], int64_t row0, int64_t col0, int64_t k0, int64_t k1) {
   float sum = 0.f;
@@ -305,15 +306,31 @@ __device__ __forceinline__ void lin_exact(const LinArgs& a, gm_f32x4 (&acc)[FM][
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int64_t r = row0 + 16 * i + (lane & 15), c = col0 + 16 * j + 4 * (lane >> 4);
+      float any = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (acc[i][j][e] == acc[i][j][e] || r >= a.m || c + e >= a.n) continue;
-        double s = 0.0;
+      for (int e = 0; e < 4; ++e) any += acc[i][j][e];
+      if (any == any || r >= a.m) continue;
+      double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll 1
-        for (int64_t k = k0; k < k1 && s == s; ++k)
-          s = fma((double)A[AS ? k * a.lda + r : r * a.lda + k], (double)B[BS ? k * a.ldb + c + e : (c + e) * a.ldb + k], s);
-        acc[i][j][e] = (float)s;
+      for (int64_t k = k0; k < k1; k += 4) {  // (four terms of four results on their way at once: an operand may hold infinities in every row)
+        float x[4], y[4][4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          x[h] = k + h < k1 ? A[AS ? (k + h) * a.lda + r : r * a.lda + k + h] : 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[h][e] = k + h < k1 && c + e < a.n ? B[BS ? (k + h) * a.ldb + c + e : (c + e) * a.ldb + k + h] : 0.f;
+        }
+        bool done = true;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) s[e] = fma((double)x[h], (double)y[h][e], s[e]);
+          done &= s[e] != s[e];
+        }
+        if (done) break;
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = acc[i][j][e] == acc[i][j][e] ? acc[i][j][e] : (float)s[e];
     }
 }
 
