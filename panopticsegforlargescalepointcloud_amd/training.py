@@ -182,10 +182,11 @@ def enable_sync_bn(group=True):
 
 def matrix_parameters(model):
     """(matrices, others) of a model's parameters: convolution kernels and weights of linear layers for `Muon`, and the rest --
-    vectors, and matrices with one row or column -- for an optimizer that works on single values."""
+    vectors, matrices with one row or column, and those whose shorter side is more than `Muon` takes -- for an optimizer that works on
+    single values."""
     matrices, others = [], []
     for p in model.parameters():
-        (matrices if p.dim() >= 2 and min(_matrix_shape(p)) > 1 else others).append(p)
+        (matrices if p.dim() >= 2 and 1 < min(_matrix_shape(p)) <= ops.NEWTON_SCHULZ_SHORT_SIDE else others).append(p)
     return matrices, others
 
 

@@ -136,3 +136,12 @@ def test_linear_act_workspace_stays_near_the_input(n, cin, cout):
         dz = n * -(-cout // 8) * 8 * size
         bias = (max(n // 128 + 1, 512, n // 131072 + 1) + 32) * cout * 4
         assert lib.pp_linear_act_bwd_workspace(dtype, n, cin, cout, 3) <= parts + dz + bias + 4096
+
+
+def test_matrix_parameters_are_what_muon_takes():
+    def param(*shape):
+        return torch.nn.Parameter(torch.empty(shape, device="meta"))
+    model = torch.nn.ParameterList([param(8192, 9000), param(9000, 8193), param(27, 400, 8193), param(27, 64, 96), param(2, 2), param(1, 7), param(6)])
+    matrices, others = training.matrix_parameters(model)
+    assert [tuple(p.shape) for p in matrices] == [(8192, 9000), (27, 64, 96), (2, 2)] and len(others) == 4
+    training.Muon(matrices)
